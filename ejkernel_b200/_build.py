@@ -47,7 +47,7 @@ def sources() -> list[Path]:
 
 def _digest() -> str:
     h = hashlib.sha256()
-    for f in sorted(list(CSRC.glob("*")) + [ROOT / "include" / "ejk_rpa.h"]):
+    for f in sorted(list(CSRC.glob("*")) + list((ROOT / "include").glob("*.h"))):
         if f.is_file():
             h.update(f.name.encode())
             h.update(f.read_bytes())

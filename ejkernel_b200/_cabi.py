@@ -9,16 +9,17 @@ missing or cannot be loaded the import of the CUDA operator fails loudly.
 from __future__ import annotations
 
 import ctypes
-from ctypes import POINTER, Structure, c_char_p, c_float, c_int, c_int32, c_size_t, c_void_p
+from ctypes import POINTER, Structure, c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_void_p
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "lib" / "libejk_rpa.so"
 
-BF16, F16, E4M3 = 0, 1, 2
+BF16, F16, E4M3, I8 = 0, 1, 2, 3
 STATIC_SCRATCH_BYTES = 32 << 20
 E_SCRATCH = -9
 
 ST_NUM_SEQS, ST_QLEN, ST_KVLEN, ST_PAGE_ID, ST_INTERNAL, ST_TIMEOUT = 1, 2, 4, 8, 16, 32
+ST_POOL, ST_NONFINITE = 64, 128  # include/ejk_q8.h
 STATUS_TEXT = {
     ST_NUM_SEQS: "num_seqs exceeds block_tables.shape[0]",
     ST_QLEN: "a sequence has q_len < 0, q_len > kv_len or query rows past total_tokens",
@@ -26,6 +27,8 @@ STATUS_TEXT = {
     ST_PAGE_ID: "a page id outside [0, num_pages) was read from block_tables",
     ST_INTERNAL: "the device planner ran out of workspace",
     ST_TIMEOUT: "a bounded wait inside a kernel ran out; outputs are invalid",
+    ST_POOL: "the free list ran out of pages, or of room for returned ones",
+    ST_NONFINITE: "a NaN or an infinity was written to the 8-bit cache",
 }
 
 EXPORTS = (
@@ -43,6 +46,15 @@ EXPORTS = (
     "ejk_rpa_v3_launch",
     "ejk_page_attention_launch",
     "ejk_rpa_stream_probe",
+)
+
+# declared in include/ejk_q8.h
+Q8_EXPORTS = (
+    "ejk_q8_workspace_bytes",
+    "ejk_q8_attention_launch",
+    "ejk_q8_write_launch",
+    "ejk_q8_read_launch",
+    "ejk_page_tables_launch",
 )
 
 
@@ -72,6 +84,22 @@ class Attrs(Structure):
         ("num_queries_per_block", c_int32),
         ("q_scale", c_float),
         ("out_scale", c_float),
+    ]
+
+
+class Q8Shape(Structure):
+    _fields_ = [
+        ("total_tokens", c_int32),
+        ("max_num_seqs", c_int32),
+        ("pages_per_seq", c_int32),
+        ("num_pages", c_int32),
+        ("page_size", c_int32),
+        ("num_q_heads", c_int32),
+        ("num_kv_heads", c_int32),
+        ("head_dim", c_int32),
+        ("dtype", c_int32),
+        ("code_dtype", c_int32),
+        ("scale_block", c_int32),
     ]
 
 
@@ -163,6 +191,46 @@ def load() -> ctypes.CDLL:
     lib.ejk_rpa_profile_read_kernels.argtypes = [POINTER(c_float)] * 4
     lib.ejk_rpa_stream_probe.restype = c_int
     lib.ejk_rpa_stream_probe.argtypes = [c_void_p, c_size_t, c_void_p, c_void_p]
+    lib.ejk_q8_workspace_bytes.restype = c_size_t
+    lib.ejk_q8_workspace_bytes.argtypes = [POINTER(Q8Shape)]
+    lib.ejk_q8_attention_launch.restype = c_int
+    lib.ejk_q8_attention_launch.argtypes = [
+        c_void_p, c_void_p, c_void_p,  # queries, kv_pages, kv_scales
+        c_void_p, c_void_p, c_void_p, c_void_p,  # context_lens, block_tables, query_start_loc, num_seqs
+        c_void_p,  # softmax_aux
+        c_void_p,  # out
+        c_void_p,  # workspace
+        c_size_t,
+        c_void_p,  # status
+        POINTER(Q8Shape),
+        POINTER(Attrs),
+        c_void_p,  # stream
+    ]
+    lib.ejk_q8_write_launch.restype = c_int
+    lib.ejk_q8_write_launch.argtypes = [
+        c_void_p, c_void_p, c_int64, c_int64,  # keys, values and their row strides
+        c_void_p, c_void_p, c_void_p,  # kv_pages, kv_scales, slots
+        c_void_p,  # status
+        POINTER(Q8Shape),
+        c_void_p,  # stream
+    ]
+    lib.ejk_q8_read_launch.restype = c_int
+    lib.ejk_q8_read_launch.argtypes = [
+        c_void_p, c_void_p, c_void_p,  # kv_pages, kv_scales, slots
+        c_void_p, c_void_p,  # keys, values
+        c_void_p,  # status
+        POINTER(Q8Shape),
+        c_void_p,  # stream
+    ]
+    lib.ejk_page_tables_launch.restype = c_int
+    lib.ejk_page_tables_launch.argtypes = [
+        c_void_p, c_void_p, c_void_p, c_void_p,  # query_lens, context_lens, block_tables, free_pages
+        c_void_p, c_void_p, c_void_p,  # num_free, num_seqs, finished
+        c_void_p, c_void_p, c_void_p, c_void_p,  # new_context_lens, query_start_loc, slots, new_num_free
+        c_void_p,  # status
+        c_int32, c_int32, c_int32, c_int32, c_int32,  # max_num_seqs, pages_per_seq, page_size, capacity, total_tokens
+        c_void_p,  # stream
+    ]
     _lib = lib
     return lib
 

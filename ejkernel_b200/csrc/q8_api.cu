@@ -1,0 +1,185 @@
+// C ABI of the operators around the 8-bit cache (declared in include/ejk_q8.h).
+#include <cmath>
+#include <cstring>
+
+#include "q8_types.cuh"
+
+namespace ejk {
+namespace {
+
+int log2_exact(int x) {
+  if (x <= 0 || (x & (x - 1))) return -1;
+  int s = 0;
+  while ((1 << s) < x) ++s;
+  return s;
+}
+
+// what every operator on the cache needs
+int check_cache(const ejk_q8_shape& s) {
+  if (s.num_pages <= 0 || s.page_size <= 0 || s.num_kv_heads <= 0) return EJK_RPA_E_SHAPE;
+  if ((long long)s.num_pages * s.page_size > 0x7fffffffLL || s.num_kv_heads > 0x7fff) return EJK_RPA_E_SHAPE;
+  if (s.head_dim != 64 && s.head_dim != 128 && s.head_dim != 256) return EJK_RPA_E_HEAD_DIM;
+  if (s.dtype != EJK_RPA_BF16 && s.dtype != EJK_RPA_F16) return EJK_RPA_E_DTYPE;
+  if (s.code_dtype != EJK_RPA_E4M3 && s.code_dtype != EJK_Q8_I8) return EJK_RPA_E_DTYPE;
+  if (log2_exact(s.scale_block) < 0 || s.page_size % s.scale_block) return EJK_RPA_E_SHAPE;
+  return 0;
+}
+
+Q8Cache cache_of(const void* pages, const float* scales, const ejk_q8_shape& s) {
+  Q8Cache c;
+  c.pages = static_cast<uint8_t*>(const_cast<void*>(pages));
+  c.scales = const_cast<float*>(scales);
+  c.num_pages = s.num_pages;
+  c.page_size = s.page_size;
+  c.Hkv = s.num_kv_heads;
+  c.D = s.head_dim;
+  c.block_shift = log2_exact(s.scale_block);
+  return c;
+}
+
+// the planner and the merge kernel see the call as one of ejk_rpa_launch over a 16-bit pool
+ejk_rpa_shape as_rpa(const ejk_q8_shape& s) {
+  return {s.total_tokens, s.max_num_seqs, s.pages_per_seq, s.num_pages, s.page_size,
+          s.num_q_heads, s.num_kv_heads, s.head_dim, s.dtype, 0};
+}
+
+int check_attention(const ejk_q8_shape& s) {
+  if (int e = check_cache(s)) return e;
+  if (s.num_q_heads > 0xffff) return EJK_RPA_E_SHAPE;  // a grid dimension
+  return check_rpa_shape(as_rpa(s));
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+bool finite(float x) { return x == x && !std::isinf(x); }
+
+}  // namespace
+}  // namespace ejk
+
+using namespace ejk;
+
+extern "C" {
+
+size_t ejk_q8_workspace_bytes(const ejk_q8_shape* shape) {
+  if (!shape || check_attention(*shape) != 0) return 0;
+  const int n_sm = sm100_sm_count();
+  return n_sm ? workspace_layout(as_rpa(*shape), n_sm).total : 0;
+}
+
+int ejk_q8_attention_launch(const void* queries, const void* kv_pages, const float* kv_scales,
+                            const int32_t* context_lens, const int32_t* block_tables, const int32_t* query_start_loc,
+                            const int32_t* num_seqs, const float* softmax_aux, void* out, void* workspace,
+                            size_t workspace_bytes, int32_t* status, const ejk_q8_shape* shape,
+                            const ejk_rpa_attrs* attrs, void* stream) {
+  set_last_launches(0);
+  if (!queries || !kv_pages || !kv_scales || !context_lens || !block_tables || !query_start_loc || !num_seqs || !out ||
+      !workspace || !shape || !attrs)
+    return EJK_RPA_E_NULL;
+  if (int e = check_attention(*shape)) return e;
+  const ejk_q8_shape& s = *shape;
+  const ejk_rpa_attrs& a = *attrs;
+  if (!finite(a.softmax_scale) || !finite(a.logits_soft_cap)) return EJK_RPA_E_ARG;
+  if (a.q_scale != 0.f || a.out_scale != 0.f) return EJK_RPA_E_ARG;
+  if (a.num_sinks < 0 || (a.num_sinks > 0 && !softmax_aux)) return EJK_RPA_E_ARG;
+  if (a.num_sinks > 0 && a.sink_rows != s.num_q_heads && a.sink_rows != s.num_kv_heads && a.sink_rows != 1) return EJK_RPA_E_ARG;
+  if (!aligned16(queries) || !aligned16(kv_pages) || !aligned16(kv_scales) || !aligned16(out)) return EJK_RPA_E_ALIGN;
+  const int n_sm = sm100_sm_count();
+  if (!n_sm) return EJK_RPA_E_DEVICE;
+  const WorkspaceLayout L = workspace_layout(as_rpa(s), n_sm);
+  if (workspace_bytes < L.total || (reinterpret_cast<uintptr_t>(workspace) & 255)) return EJK_RPA_E_WORKSPACE;
+
+  Params p;
+  std::memset(&p, 0, sizeof(p));
+  p.q = queries;
+  p.kv = kv_pages;
+  p.context_lens = context_lens;
+  p.block_tables = block_tables;
+  p.query_start_loc = query_start_loc;
+  p.num_seqs = num_seqs;
+  p.sinks = softmax_aux;
+  p.out = out;
+  p.status = status;
+  p.T = s.total_tokens;
+  p.S_max = s.max_num_seqs;
+  p.pages_per_seq = s.pages_per_seq;
+  p.num_pages = s.num_pages;
+  p.page_size = s.page_size;
+  p.Hq = s.num_q_heads;
+  p.Hkv = s.num_kv_heads;
+  p.G = s.num_q_heads / s.num_kv_heads;
+  p.D = p.Dq = p.Dkv = s.head_dim;
+  p.window = a.sliding_window > 0 ? a.sliding_window : 0;
+  p.num_sinks = a.num_sinks;
+  p.sink_rows = a.sink_rows;
+  const float log2e = 1.4426950408889634f;
+  p.out_scale = 1.f;
+  p.scale = a.softmax_scale;
+  p.scale_log2 = a.softmax_scale * log2e;
+  p.cap = a.logits_soft_cap;
+  p.cap_log2 = a.logits_soft_cap * log2e;
+  p.inv_cap_scale = a.logits_soft_cap != 0.f ? a.softmax_scale / a.logits_soft_cap : 0.f;
+  const Q8Cache c = cache_of(kv_pages, kv_scales, s);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  cudaError_t e = launch_q8_gather(p, c, s.dtype, s.code_dtype, st);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  set_last_launches(1);
+  return 0;
+}
+
+int ejk_q8_write_launch(const void* keys, const void* values, int64_t key_stride, int64_t value_stride, void* kv_pages,
+                        float* kv_scales, const int32_t* slots, int32_t* status, const ejk_q8_shape* shape, void* stream) {
+  set_last_launches(0);
+  if (!keys || !values || !kv_pages || !kv_scales || !slots || !shape) return EJK_RPA_E_NULL;
+  if (int e = check_cache(*shape)) return e;
+  const ejk_q8_shape& s = *shape;
+  if (s.total_tokens <= 0) return EJK_RPA_E_SHAPE;
+  const int64_t row = (int64_t)s.num_kv_heads * s.head_dim;
+  if (key_stride < row || value_stride < row) return EJK_RPA_E_SHAPE;
+  if (!aligned16(keys) || !aligned16(values) || !aligned16(kv_pages) || key_stride % 8 || value_stride % 8) return EJK_RPA_E_ALIGN;
+  if (!sm100_sm_count()) return EJK_RPA_E_DEVICE;
+  cudaError_t e = launch_q8_write(keys, values, key_stride, value_stride, cache_of(kv_pages, kv_scales, s), slots, status,
+                                  s.total_tokens, s.dtype, s.code_dtype, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return static_cast<int>(e);
+  set_last_launches(1);
+  return 0;
+}
+
+int ejk_q8_read_launch(const void* kv_pages, const float* kv_scales, const int32_t* slots, void* keys, void* values,
+                       int32_t* status, const ejk_q8_shape* shape, void* stream) {
+  set_last_launches(0);
+  if (!keys || !values || !kv_pages || !kv_scales || !slots || !shape) return EJK_RPA_E_NULL;
+  if (int e = check_cache(*shape)) return e;
+  const ejk_q8_shape& s = *shape;
+  // 256 threads of 8 elements each per block, at most 2^31 - 1 blocks
+  if (s.total_tokens <= 0 || (long long)s.total_tokens * s.num_kv_heads * 2 * (s.head_dim / 8) / 256 >= 0x7fffffffLL)
+    return EJK_RPA_E_SHAPE;
+  if (!aligned16(keys) || !aligned16(values) || !aligned16(kv_pages)) return EJK_RPA_E_ALIGN;
+  if (!sm100_sm_count()) return EJK_RPA_E_DEVICE;
+  cudaError_t e = launch_q8_read(cache_of(kv_pages, kv_scales, s), slots, keys, values, status, s.total_tokens, s.dtype,
+                                 s.code_dtype, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return static_cast<int>(e);
+  set_last_launches(1);
+  return 0;
+}
+
+int ejk_page_tables_launch(const int32_t* query_lens, const int32_t* context_lens, int32_t* block_tables,
+                           int32_t* free_pages, const int32_t* num_free, const int32_t* num_seqs, const uint8_t* finished,
+                           int32_t* new_context_lens, int32_t* query_start_loc, int32_t* slots, int32_t* new_num_free,
+                           int32_t* status, int32_t max_num_seqs, int32_t pages_per_seq, int32_t page_size,
+                           int32_t capacity, int32_t total_tokens, void* stream) {
+  set_last_launches(0);
+  if (!query_lens || !context_lens || !block_tables || !free_pages || !num_free || !num_seqs || !new_context_lens ||
+      !query_start_loc || !new_num_free || (total_tokens > 0 && !slots))
+    return EJK_RPA_E_NULL;
+  if (max_num_seqs <= 0 || max_num_seqs > 0x00ffffff || pages_per_seq <= 0 || page_size <= 0 || capacity <= 0 || total_tokens < 0)
+    return EJK_RPA_E_SHAPE;
+  if ((long long)pages_per_seq * page_size > 0x3fffffffLL || total_tokens > 0x3fffffff) return EJK_RPA_E_SHAPE;
+  if (!sm100_sm_count()) return EJK_RPA_E_DEVICE;
+  cudaError_t e = launch_page_tables(query_lens, context_lens, block_tables, free_pages, num_free, num_seqs, finished,
+                                     new_context_lens, query_start_loc, slots, new_num_free, status, max_num_seqs,
+                                     pages_per_seq, page_size, capacity, total_tokens, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return static_cast<int>(e);
+  set_last_launches(total_tokens > 0 ? 2 : 1);
+  return 0;
+}
+
+}  // extern "C"

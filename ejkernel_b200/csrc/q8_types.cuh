@@ -1,0 +1,91 @@
+// The 8-bit cache: parameters of its kernels and the conversions of its codes.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <stdint.h>
+
+#include "ejk_q8.h"
+#include "rpa_device.cuh"
+#include "rpa_types.h"
+
+namespace ejk {
+
+// Where a row lives: kv_pages [P, Hkv, 2, page, D], kv_scales [P, Hkv, 2, page >> block_shift]
+struct Q8Cache {
+  uint8_t* pages;
+  float* scales;
+  int32_t num_pages, page_size, Hkv, D;
+  int32_t block_shift;  // log2 of the tokens that share a scale
+};
+
+struct CodeE4M3 {
+  static constexpr int kId = EJK_RPA_E4M3;
+  static constexpr float kMax = 448.f;
+  static __device__ __forceinline__ float decode(uint8_t c) {
+    uint32_t h;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;\n" : "=r"(h) : "h"((uint16_t)c));
+    return __half2float(__ushort_as_half((uint16_t)h));
+  }
+  // x is within +-448: the nearest code, ties to even
+  static __device__ __forceinline__ uint8_t encode(float x) {
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;\n" : "=h"(r) : "f"(0.f), "f"(x));
+    return (uint8_t)(r & 0xff);
+  }
+  // biased exponent of the smallest power of two s with amax <= 448 * s: 448 = 1.75 * 2^8
+  static __device__ __forceinline__ int scale_exponent(uint32_t amax_bits) {
+    return (int)(amax_bits >> 23) - 8 + ((amax_bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+  }
+};
+struct CodeI8 {
+  static constexpr int kId = EJK_Q8_I8;
+  static constexpr float kMax = 127.f;
+  static __device__ __forceinline__ float decode(uint8_t c) { return (float)(int8_t)c; }
+  static __device__ __forceinline__ uint8_t encode(float x) { return (uint8_t)(int8_t)__float2int_rn(x); }
+  // 127 = 1.984375 * 2^6
+  static __device__ __forceinline__ int scale_exponent(uint32_t amax_bits) {
+    return (int)(amax_bits >> 23) - 6 + ((amax_bits & 0x7fffffu) > 0x7e0000u ? 1 : 0);
+  }
+};
+template <typename Code>
+__device__ __forceinline__ float power_of_two_scale(float amax) {
+  int e = Code::scale_exponent(__float_as_uint(amax));
+  e = e < 1 ? 1 : e;  // not below 2^-126: scale and 1 / scale stay normal (amax < 2^128, so e <= 249)
+  return __uint_as_float((uint32_t)e << 23);
+}
+// 1 / s of a power of two between 2^-126 and 2^126, exactly
+__device__ __forceinline__ float power_of_two_inverse(float s) {
+  return __uint_as_float((254u << 23) - __float_as_uint(s));
+}
+
+template <typename T>
+__device__ __forceinline__ float to_float(T x);
+template <>
+__device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <>
+__device__ __forceinline__ float to_float<__half>(__half x) { return __half2float(x); }
+
+// host side, shared by the entry points (defined in rpa_api.cu)
+struct LaunchOptions {
+  int waves, min_chunk, prefill_rows, prefill_share, prefill_split, sort_items, overlap, fused_merge, wait_ms, path, test_withhold;
+};
+LaunchOptions launch_options();
+// SM count of the current device; 0: no device, or not an sm_100 one
+int sm100_sm_count();
+int check_rpa_shape(const ejk_rpa_shape& s);
+WorkspaceLayout workspace_layout(const ejk_rpa_shape& s, int n_sm);
+void set_last_launches(int n);
+
+// launchers
+cudaError_t launch_q8_gather(const Params& p, const Q8Cache& c, int dtype, int code, cudaStream_t stream);
+cudaError_t launch_q8_write(const void* keys, const void* values, long long key_stride, long long value_stride,
+                            const Q8Cache& c, const int32_t* slots, int32_t* status, int rows, int dtype, int code,
+                            cudaStream_t stream);
+cudaError_t launch_q8_read(const Q8Cache& c, const int32_t* slots, void* keys, void* values, int32_t* status, int rows,
+                           int dtype, int code, cudaStream_t stream);
+cudaError_t launch_page_tables(const int32_t* query_lens, const int32_t* context_lens, int32_t* tables, int32_t* free_pages,
+                               const int32_t* num_free, const int32_t* num_seqs, const uint8_t* finished,
+                               int32_t* new_lens, int32_t* starts, int32_t* slots, int32_t* new_free, int32_t* status,
+                               int S, int pps, int page, int capacity, int T, cudaStream_t stream);
+
+}  // namespace ejk

@@ -2,6 +2,6 @@
 Only ``_cuda`` exists here; importing it registers its operators."""
 
 from . import _cuda  # noqa: F401  (registers the CUDA implementations)
-from ._registry import Backend, KernelRegistry, KernelSpec, Platform, kernel_registry
+from ._registry import Backend, KernelRegistry, KernelSpec, Platform, kernel_registry, serving_registry
 
-__all__ = ["Backend", "KernelRegistry", "KernelSpec", "Platform", "kernel_registry"]
+__all__ = ["Backend", "KernelRegistry", "KernelSpec", "Platform", "kernel_registry", "serving_registry"]

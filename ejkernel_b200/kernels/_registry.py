@@ -127,3 +127,7 @@ class KernelRegistry:
 
 
 kernel_registry = KernelRegistry()
+
+# Operators of a serving step that the reference does not have.  They are registered apart, so that a listing of
+# ``kernel_registry`` stays a listing of the reference's algorithms.
+serving_registry = KernelRegistry()

@@ -1,4 +1,5 @@
-"""Public operator API, mirroring ``ejkernel.modules`` for the operators this package covers."""
+"""Public operator API, mirroring ``ejkernel.modules`` for the operators this package covers, and
+the serving step over an 8-bit cache, which the reference does not have."""
 
 from .operations import (
     PageAttentionConfig,
@@ -6,6 +7,11 @@ from .operations import (
     RaggedPageAttention,
     RaggedPageAttentionConfig,
     RaggedPageAttentionv3Config,
+    allocate_quantized_kv,
+    build_page_tables,
+    quantized_kv_read,
+    quantized_kv_write,
+    quantized_ragged_page_attention,
     ragged_page_attention,
     ragged_page_attention_v3,
 )
@@ -16,6 +22,11 @@ __all__ = [
     "RaggedPageAttention",
     "RaggedPageAttentionConfig",
     "RaggedPageAttentionv3Config",
+    "allocate_quantized_kv",
+    "build_page_tables",
+    "quantized_kv_read",
+    "quantized_kv_write",
+    "quantized_ragged_page_attention",
     "ragged_page_attention",
     "ragged_page_attention_v3",
 ]
