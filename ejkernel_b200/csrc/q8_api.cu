@@ -87,6 +87,10 @@ int ejk_q8_attention_launch(const void* queries, const void* kv_pages, const flo
   const WorkspaceLayout L = workspace_layout(as_rpa(s), n_sm);
   if (workspace_bytes < L.total || (reinterpret_cast<uintptr_t>(workspace) & 255)) return EJK_RPA_E_WORKSPACE;
 
+  const LaunchOptions opt = launch_options();
+  const bool use_tma = opt.path != 1 && q8_tma_supported(s.page_size);
+  if (opt.path == 2 && !use_tma) return EJK_RPA_E_ARG;
+
   Params p;
   std::memset(&p, 0, sizeof(p));
   p.q = queries;
@@ -119,9 +123,68 @@ int ejk_q8_attention_launch(const void* queries, const void* kv_pages, const flo
   p.inv_cap_scale = a.logits_soft_cap != 0.f ? a.softmax_scale / a.logits_soft_cap : 0.f;
   const Q8Cache c = cache_of(kv_pages, kv_scales, s);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  cudaError_t e = launch_q8_gather(p, c, s.dtype, s.code_dtype, st);
+  if (!use_tma) {
+    cudaError_t e = launch_q8_gather(p, c, s.dtype, s.code_dtype, st);
+    if (e != cudaSuccess) return static_cast<int>(e);
+    set_last_launches(1);
+    return 0;
+  }
+
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  p.header = reinterpret_cast<int32_t*>(ws + L.header_off);
+  p.units = reinterpret_cast<Unit*>(ws + L.units_off);
+  p.punits = reinterpret_cast<Unit*>(ws + L.punits_off);
+  p.merge = reinterpret_cast<MergeItem*>(ws + L.merge_off);
+  p.tickets = reinterpret_cast<int32_t*>(ws + L.tickets_off);
+  p.part_o = reinterpret_cast<float*>(ws + L.part_o_off);
+  p.part_ml = reinterpret_cast<float2*>(ws + L.part_ml_off);
+  p.C2 = 2 * s.num_kv_heads;
+  p.rows_per_tile = L.rows_per_tile;
+  p.max_units = L.max_units;
+  p.max_merge = L.max_merge;
+  p.max_slots = L.max_slots;
+  p.max_punits = L.max_punits;
+  p.target_units = L.target_units;
+  p.target_units_max = L.target_units_max;
+  p.min_chunk = opt.min_chunk;
+  if (a.num_kv_pages_per_block > 0) {  // per-call hint: the smallest KV chunk, in pages
+    long long chunk = (long long)a.num_kv_pages_per_block * s.page_size;
+    chunk = (chunk + kTileTokens - 1) / kTileTokens * kTileTokens;
+    p.min_chunk = chunk > 0x40000000ll ? 0x40000000 : (int)chunk;
+  }
+  p.page_shift = log2_exact(s.page_size);
+  // tokens per TMA box: the largest power of two that divides the page size, at most the 64 tokens that chunks are cut at
+  p.tma_block_tokens = 8;
+  while (p.tma_block_tokens < kTileTokens && s.page_size % (p.tma_block_tokens * 2) == 0) p.tma_block_tokens *= 2;
+  p.tma_block_shift = log2_exact(p.tma_block_tokens);
+  p.wait_timeout_ms = opt.wait_ms;
+  p.test_withhold = opt.test_withhold;
+  p.sort_items = opt.sort_items;
+  {
+    // the chunks of a row tile are combined by the last one to finish where a tile gets two at most, by a kernel of
+    // their own otherwise (the rule of ejk_rpa_launch)
+    const long long by_len = ((long long)s.pages_per_seq * s.page_size + p.min_chunk - 1) / p.min_chunk;
+    const bool few = (long long)L.target_units <= 2ll * s.total_tokens || by_len <= 2;
+    p.fused_merge = (opt.fused_merge == 2 || (opt.fused_merge == 1 && few)) ? 1 : 0;
+  }
+  p.prefill_item_rows = prefill_rows_per_item(s.head_dim);
+  // Kernels of one call are launched as programmatic dependents: each waits on the device for what it needs of the one
+  // before, the planner for whatever precedes the call.
+  const bool pdl = opt.overlap != 0;
+  p.pdl = pdl ? 2 : 0;
+  int launches = 0;
+  cudaError_t e = launch_plan(p, st, pdl);
   if (e != cudaSuccess) return static_cast<int>(e);
-  set_last_launches(1);
+  ++launches;
+  e = launch_q8_splitkv(p, c, s.dtype, s.code_dtype, n_sm, st, pdl);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  ++launches;
+  if (!p.fused_merge) {
+    e = launch_merge(p, s.dtype, n_sm, st, pdl);
+    if (e != cudaSuccess) return static_cast<int>(e);
+    ++launches;
+  }
+  set_last_launches(launches);
   return 0;
 }
 

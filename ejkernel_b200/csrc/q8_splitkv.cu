@@ -1,0 +1,916 @@
+// Split-KV ragged attention over the 8-bit cache: decode rows and short chunks.
+//
+//   x_j  = scale * k_scale_j * (q . k_j),  p_j = 2^(x_j log2 e - m)   (m: running maximum, lazily moved)
+//   O   += (p_j * v_scale_j) v_j,  l += p_j;   out = O / l
+//
+// The kernel is a stream of the cache: every byte of K and V is read once per kv head and costs 2 * G multiply-adds, so
+// DRAM bounds it, and everything else has to stay out of the way.  Work items, queue, partials and merge are those of
+// rpa_splitkv_tma.cu; what differs follows from the codes:
+//   * a stage is 128 tokens of one head, fetched by one producer warp as TMA boxes of up to 64 tokens.  A head's page is
+//     contiguous, so a box of 16 tokens at head_dim 128 is two runs of 2 KB.  The stage's scales come beside it with 4-byte
+//     cp.async copies that arrive on the same mbarrier: no wait of the producer stands between two stages.
+//   * four consumer warps take 32 tokens each.  Codes go to f16 in registers, which is exact for both types, and both
+//     products run on f16 mma.sync with float32 sums.  8-bit operands would halve the mma work, which is not what bounds
+//     the kernel, and would round q and p to 3 bits of mantissa.
+//   * k_scale multiplies the finished dot product, v_scale the probability: two multiplications a token and row, none per
+//     element.  p * v_scale has to fit f16: a warp divides v_scale by a power of two, chosen from the largest scale that
+//     it has met so that the product is at most 2^15, and moves it as it moves m.  What is below 2^-24 of that
+//     range is lost: 2^-32 of the largest |V|.
+//   * bf16 queries go to f16 by a power of two per row (their largest element to [2^14, 2^15)), undone on the logits.
+//
+// Every wait on an mbarrier is bounded in wall time (option "wait_ms"): on expiry the warp raises
+// EJK_RPA_ST_TIMEOUT, sets the CTA's abort flag and returns, and every other wait of the CTA gives up as soon as it sees it.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <atomic>
+#include <type_traits>
+
+#include "q8_types.cuh"
+
+namespace ejk {
+namespace {
+
+constexpr int kConsumerWarps = 4;
+constexpr int kThreads = (kConsumerWarps + 1) * 32;
+constexpr int kRing = 8;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kMergeInFlight = 8;     // partials whose loads the last-arriver merge keeps in flight per row
+constexpr float kLazyRescale = 8.0f;  // rescale the accumulators only when the max grows by 2^8: p <= 2^8
+constexpr int kVBits = 6;             // the largest v_scale met so far is taken to [2^6, 2^7): p * v_scale <= 2^15 < 65504
+
+struct ItemDesc {
+  Unit u;
+  int32_t h;
+  int32_t pad[3];
+};
+
+template <int D, int NT, int NS>
+struct Cfg {
+  static constexpr int TK = 128;                  // tokens per stage
+  static constexpr int TW = TK / kConsumerWarps;  // tokens of a stage per consumer warp
+  static constexpr int RB = D < 128 ? D : 128;    // bytes of a row in one swizzled column (the swizzle span)
+  static constexpr int DC = D / RB;               // columns
+  static constexpr int CH = RB / 16;              // 16-byte chunks of a column's row
+  static constexpr int RT = 8 * NT;
+  static constexpr int STAGE_BYTES = TK * 2 * D;
+  static constexpr int Q_ROW_BYTES = D * 2 + 16;
+  static constexpr int Q_BYTES = RT * Q_ROW_BYTES;
+  static constexpr int OFF_SCALE = NS * STAGE_BYTES;              // per stage: TK scales of K, TK of V (at most)
+  static constexpr int OFF_Q = OFF_SCALE + NS * 2 * TK * 4;
+  static constexpr int OFF_QFAC = OFF_Q + NS * Q_BYTES;           // per stage: 2^-k of each query row
+  static constexpr int OFF_OBUF = OFF_QFAC + NS * RT * 4;
+  static constexpr int OFF_MBUF = OFF_OBUF + RT * D * 4;
+  static constexpr int OFF_LBUF = OFF_MBUF + kConsumerWarps * RT * 4;
+  static constexpr int OFF_ROWSCALE = OFF_LBUF + kConsumerWarps * RT * 4;
+  static constexpr int OFF_ROWM = OFF_ROWSCALE + RT * 4;
+  static constexpr int OFF_ROWL = OFF_ROWM + RT * 4;
+  static constexpr int OFF_RING = (OFF_ROWL + RT * 4 + 63) / 64 * 64;
+  static constexpr int OFF_META = OFF_RING + kRing * (int)sizeof(ItemDesc);
+  static constexpr int OFF_BAR = OFF_META + NS * 8;  // full[NS], empty[NS], cbar
+  static constexpr int OFF_ABORT = OFF_BAR + (2 * NS + 1) * 8;
+  static constexpr int SMEM_BYTES = OFF_ABORT + 16 + 1024;  // + alignment slack
+  static constexpr int CTAS = SMEM_BYTES <= 112 * 1024 ? 2 : 1;
+  static_assert(SMEM_BYTES <= 227 * 1024, "shared memory budget");
+};
+
+__device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2,
+                                            int c3, int c4) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];\n"
+      ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4)
+      : "memory");
+}
+// 4-byte asynchronous copy, and the arrival that follows this thread's copies (counted in the barrier's expected count)
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;\n" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];\n" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t w);
+template <>
+__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <>
+__device__ __forceinline__ float2 unpack2<__half>(uint32_t w) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+
+template <typename T, typename Code, int D, int NT, int NS>
+__global__ void __launch_bounds__(kThreads, (Cfg<D, NT, NS>::CTAS))
+q8_splitkv_kernel(const __grid_constant__ CUtensorMap tmap, const Params p, const Q8Cache cache) {
+  using C = Cfg<D, NT, NS>;
+  constexpr int TK = C::TK, RT = C::RT, TW = C::TW, CH = C::CH;
+  constexpr int KT = D / 16;
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t smem_base = smem_u32(smem);
+  float* obuf = reinterpret_cast<float*>(smem + C::OFF_OBUF);
+  float* mbuf = reinterpret_cast<float*>(smem + C::OFF_MBUF);
+  float* lbuf = reinterpret_cast<float*>(smem + C::OFF_LBUF);
+  float* row_scale = reinterpret_cast<float*>(smem + C::OFF_ROWSCALE);
+  float* row_m = reinterpret_cast<float*>(smem + C::OFF_ROWM);
+  float* row_l = reinterpret_cast<float*>(smem + C::OFF_ROWL);
+  ItemDesc* ring = reinterpret_cast<ItemDesc*>(smem + C::OFF_RING);
+  int2* metas = reinterpret_cast<int2*>(smem + C::OFF_META);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::OFF_ABORT);
+  const uint32_t bar_full = smem_base + C::OFF_BAR;
+  const uint32_t bar_empty = bar_full + NS * 8;
+  const uint32_t bar_c = bar_empty + NS * 8;
+
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int Hkv = p.Hkv, G = p.G;
+  const int pb = p.tma_block_tokens;  // tokens per TMA box (power of two, 8 to 64)
+  const int pb_shift = p.tma_block_shift;
+  const int sb_shift = cache.block_shift;
+  const unsigned long long wait_ns = (unsigned long long)p.wait_timeout_ms * 1000000ull;
+  unsigned flags = 0;
+
+  if (tid == 0) {
+    for (int s = 0; s < NS; ++s) {
+      mbar_init(bar_full + s * 8, 1 + 32);  // the announcement, and every producer lane's scale copies
+      mbar_init(bar_empty + s * 8, kConsumerWarps);
+    }
+    mbar_init(bar_c, kConsumerWarps);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+  }
+  __syncthreads();
+  // launched as a programmatic dependent of the planner: everything above overlapped its tail
+  if (p.pdl & 2) pdl_wait();
+  const int n_work = p.header[kHdrNumUnits] * Hkv;
+
+  if (warp == kConsumerWarps) {
+    // =============================== producer warp ===============================
+    const int blocks_per_stage = TK >> pb_shift;
+    const uint32_t box_bytes = (uint32_t)pb * 2 * D;
+    const int scales_per_page = p.page_size >> sb_shift;
+    int s = 0;
+    uint32_t empty_parity = 1;  // a fresh barrier passes a wait on parity 1: all stages start empty
+    int k = 0;
+    int fills = 0;  // stages announced so far
+    int wid = 0;
+    if (lane == 0) wid = atomicAdd(&p.header[kHdrQueue], 1);
+    wid = __shfl_sync(0xffffffffu, wid, 0);
+    // page id of a key of a sequence; one that is out of range is reported and read as page 0
+    auto split_key = [&](int key, int& off) {
+      int pi;
+      if (p.page_shift >= 0) {
+        pi = key >> p.page_shift;
+        off = key & (p.page_size - 1);
+      } else {
+        pi = key / p.page_size;
+        off = key - pi * p.page_size;
+      }
+      return pi;
+    };
+    auto page_of = [&](const int32_t* tab, int pi) {
+      int page = __ldg(tab + pi);
+      if ((unsigned)page >= (unsigned)p.num_pages) {
+        flags |= EJK_RPA_ST_PAGE_ID;
+        page = 0;
+      }
+      return page;
+    };
+    bool alive = true;
+    while (alive) {
+      if (wid >= n_work) {
+        // end-of-stream marker for the consumers
+        if (!mbar_wait(bar_empty + s * 8, empty_parity, abort_flag, wait_ns)) break;
+        if (lane == 0) {
+          metas[s] = make_int2(-1, 0);
+          mbar_arrive(bar_full + s * 8);
+        }
+        cp_async_arrive(bar_full + s * 8);
+        ++fills;
+        break;
+      }
+      const int ui = wid / Hkv;
+      const int h = wid - ui * Hkv;
+      Unit u;
+      {
+        const int4* src = reinterpret_cast<const int4*>(p.units + ui);
+        const int4 a = __ldg(src), b = __ldg(src + 1), c3 = __ldg(src + 2);
+        u.seq = a.x; u.row0 = a.y; u.kv_begin = a.z; u.kv_end = a.w;
+        u.slot = b.x; u.q_start = b.y; u.q_len = b.z; u.kv_len = b.w;
+        u.merge_idx = c3.x; u.chunk_idx = c3.y; u.n_chunks = c3.z; u.pad = 0;
+      }
+      const int ring_slot = k % kRing;
+      int wid_next = 0;
+      if (lane == 0) wid_next = atomicAdd(&p.header[kHdrQueue], 1);  // consumed only at the next item
+      const int32_t* tab = p.block_tables + (size_t)u.seq * p.pages_per_seq;
+      bool first = true;
+      for (int pos = u.kv_begin; first || pos < u.kv_end; pos += TK) {
+        int nblk = (u.kv_end - pos + pb - 1) >> pb_shift;
+        if (nblk > blocks_per_stage) nblk = blocks_per_stage;
+        if (nblk < 0) nblk = 0;
+        // this lane's page, fetched before the wait so that its latency is hidden
+        int page = 0, off = 0;
+        if (lane < nblk) page = page_of(tab, split_key(pos + (lane << pb_shift), off));
+        if (!mbar_wait(bar_empty + s * 8, empty_parity, abort_flag, wait_ns)) {
+          alive = false;
+          break;
+        }
+        // test hook: the stage is never announced, the consumers' wait for it must run out
+        const bool withhold = (p.test_withhold & 1) && wid == 0 && first;
+        const uint32_t full = bar_full + s * 8;
+        if (!withhold) {
+          if (lane == 0 && nblk > 0)  // the bytes are expected before the first copy can report them; no arrival yet
+            asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;\n" ::"r"(full), "r"((uint32_t)nblk * box_bytes) : "memory");
+          __syncwarp();
+          if (lane < nblk) tma_load_5d(smem_base + s * C::STAGE_BYTES + lane * box_bytes, &tmap, full, 0, off, 0, 2 * h, page);
+          // scales of the blocks that the stage's keys lie in: K's, then V's
+          const int e0 = pos >> sb_shift;
+          const int last = (u.kv_end < pos + TK ? u.kv_end : pos + TK) - 1;
+          const int n_e = last >= pos ? (last >> sb_shift) - e0 + 1 : 0;
+          const uint32_t sdst = smem_base + C::OFF_SCALE + s * (2 * TK * 4);
+          for (int e = lane; e < n_e; e += 32) {
+            int eoff;
+            const int key = (e0 + e) << sb_shift;
+            const int pi = split_key(key > pos ? key : pos, eoff);
+            const long long at = (((long long)page_of(tab, pi) * Hkv + h) * 2) * scales_per_page + (eoff >> sb_shift);
+            cp_async4(sdst + e * 4, cache.scales + at);
+            cp_async4(sdst + (TK + e) * 4, cache.scales + at + scales_per_page);
+          }
+        }
+        if (first) {
+          // the item's descriptor and query tile travel with its first stage
+          if (lane == 0) {
+            ItemDesc d;
+            d.u = u;
+            d.h = h;
+            ring[ring_slot] = d;
+          }
+          constexpr int QCH = D / 8;  // 16-byte chunks of a row: 8, 16 or 32 neighbouring lanes hold one row
+          uint8_t* qdst = smem + C::OFF_Q + s * C::Q_BYTES;
+          float* qfac = reinterpret_cast<float*>(smem + C::OFF_QFAC + s * RT * 4);
+          const int rows_total = u.q_len * G;
+#pragma unroll 4
+          for (int cidx = lane; cidx < RT * QCH; cidx += 32) {
+            const int r = cidx / QCH, ch = cidx % QCH;
+            const int R = u.row0 + r;
+            uint4 v = make_uint4(0u, 0u, 0u, 0u);
+            if (R < rows_total) {
+              const int qt = R / G, g = R - qt * G;
+              v = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(p.q) +
+                                                       ((size_t)(u.q_start + qt) * p.Hq + h * G + g) * D * sizeof(T) + ch * 16));
+            }
+            if constexpr (!std::is_same<T, __half>::value) {
+              // to f16 by a power of two that takes the row's largest element to [2^14, 2^15): exact for every element
+              // above 2^-28 of it, absolute error 2^-39 of it below
+              uint32_t w[4] = {v.x, v.y, v.z, v.w};
+              uint32_t big = 0;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) big = max(big, max((w[i] << 16) & 0x7fffffffu, w[i] & 0x7fff0000u));
+#pragma unroll
+              for (int o = QCH / 2; o > 0; o >>= 1) big = max(big, __shfl_xor_sync(0xffffffffu, big, o));
+              int e = (int)(big >> 23);  // biased exponent of the row's largest element
+              e = e == 255 ? 127 + 14 : (e < 20 ? 20 : e);  // infinities and NaN stay what they are; 2^k stays finite
+              const float up = __uint_as_float((uint32_t)(254 + 14 - e) << 23);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const float2 a = unpack2<T>(w[i]);
+                w[i] = Mma<__half>::pack(a.x * up, a.y * up);
+              }
+              v = make_uint4(w[0], w[1], w[2], w[3]);
+              if (ch == 0) qfac[r] = __uint_as_float((uint32_t)(e - 14) << 23);
+            } else {
+              if (ch == 0) qfac[r] = 1.f;
+            }
+            *reinterpret_cast<uint4*>(qdst + r * C::Q_ROW_BYTES + ch * 16) = v;
+          }
+        }
+        __syncwarp();  // what the lanes wrote is ordered before the announcement
+        ++fills;
+        if (!withhold) {
+          if (lane == 0) {
+            metas[s] = make_int2(ring_slot, pos);
+            mbar_arrive(full);
+          }
+          cp_async_arrive(full);
+        }
+        first = false;
+        if (++s == NS) {
+          s = 0;
+          empty_parity ^= 1u;
+        }
+      }
+      ++k;
+      wid = __shfl_sync(0xffffffffu, wid_next, 0);
+    }
+    // Leave only after every bulk copy this warp issued has landed: wait (bounded) for the
+    // consumers to drain all stages, which implies all "full" phases completed.
+    for (int i = 0; i < NS; ++i) {
+      if (!mbar_wait(bar_empty + s * 8, empty_parity, abort_flag, wait_ns)) break;
+      if (++s == NS) {
+        s = 0;
+        empty_parity ^= 1u;
+      }
+    }
+    if (*abort_flag) {
+      // Giving up: the consumers no longer release stages, so wait (bounded, 2 ms per stage) for the
+      // copies themselves -- the "full" phase of each of the last NS announced stages -- before this
+      // CTA's shared memory can go to another CTA.
+      flags |= EJK_RPA_ST_TIMEOUT;
+      for (int i = 1; i <= NS && i <= fills; ++i) {
+        const int f = fills - i;
+        mbar_wait_quiet(bar_full + (f % NS) * 8, (uint32_t)((f / NS) & 1), 2000000ull);
+      }
+    }
+    asm volatile("cp.async.wait_all;\n" ::: "memory");
+  } else {
+    // =============================== consumer warps ===============================
+    // Shared-memory offsets of this lane's ldmatrix rows.  Token tl of the stage sits in box tl / pb at row tl % pb; a
+    // box is [K|V][DC columns][pb rows][RB bytes].  The swizzle XORs the 16-byte chunk with the row number, counted
+    // in 128-byte lines: row & 7 at 128-byte rows, (row >> 1) & 3 at 64-byte rows.
+    const uint32_t swz = (uint32_t)((C::RB == 128 ? (lane & 7) : ((lane & 7) >> 1))) << 4;
+    const uint32_t dc_stride = (uint32_t)pb * C::RB;
+    auto row_off = [&](int tl, int kv) {
+      const int j = tl >> pb_shift, tp = tl & (pb - 1);
+      return (uint32_t)((j * 2 + kv) * C::DC) * dc_stride + (uint32_t)tp * C::RB;
+    };
+    // K: two 16-token blocks, in each the matrices (tokens 0-7 | 8-15) x (16-byte chunk c | c + 1);
+    // V: four transposed matrices of one chunk, tokens 8j .. 8j+7
+    const uint32_t k_off0 = row_off(warp * TW + (lane & 7) + ((lane >> 3) & 1) * 8, 0);
+    const uint32_t k_off1 = row_off(warp * TW + 16 + (lane & 7) + ((lane >> 3) & 1) * 8, 0);
+    const uint32_t v_off = row_off(warp * TW + (lane & 7) + (lane >> 3) * 8, 1);
+    const int k_dhalf = lane >> 4;
+
+    uint32_t qf[NT][D / 32][4];  // B operands of Q.K^T: two f16 mmas per 32-byte chunk of K
+    float acc[NT][KT][4];
+    float m_run[NT][2], l_run[NT][2], q_fac[NT][2];
+    int pos_r[NT][2], lo_r[NT][2];
+    int pos_min = 0, lo_max = 0, lo_min = -1;
+    float v_norm = 1.f;  // power of two that the V scales are multiplied by
+    int s = 0;
+    uint32_t full_parity = 0, c_parity = 0;
+
+    auto consumer_sync = [&]() -> bool {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar_c);
+      const bool ok = mbar_wait(bar_c, c_parity, abort_flag, wait_ns);
+      c_parity ^= 1u;
+      return ok;
+    };
+
+    while (true) {
+      if (!mbar_wait(bar_full + s * 8, full_parity, abort_flag, wait_ns)) break;
+      const int2 meta = metas[s];
+      if (meta.x < 0) break;
+      const ItemDesc& it = ring[meta.x];
+      const Unit u = it.u;
+      const int h = it.h;
+      const int pos = meta.y;
+      const uint32_t sbase = smem_base + s * C::STAGE_BYTES;
+      const int rows_total = u.q_len * G;
+      int n_rows = rows_total - u.row0;
+      if (n_rows > RT) n_rows = RT;
+
+      if (pos == u.kv_begin) {
+        const uint8_t* qs = smem + C::OFF_Q + s * C::Q_BYTES;
+        const float* qfac = reinterpret_cast<const float*>(smem + C::OFF_QFAC + s * RT * 4);
+        const float to_log2 = p.cap != 0.f ? p.inv_cap_scale : p.scale_log2;
+        const int base = u.kv_len - u.q_len;
+        pos_min = base + u.row0 / G;
+        lo_max = (p.window > 0) ? (base + (u.row0 + n_rows - 1) / G - p.window) : -1;
+        lo_min = (p.window > 0) ? pos_min - p.window : -1;
+        v_norm = __uint_as_float((127u + 125u) << 23);  // no scale met yet: the largest power of two (see below)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          // elements 32kt + 4t .. +3 (first mma of the chunk) and 32kt + 16 + 4t .. +3 (second)
+          const uint8_t* qrow = qs + (nt * 8 + (lane >> 2)) * C::Q_ROW_BYTES + (lane & 3) * 8;
+#pragma unroll
+          for (int kt = 0; kt < D / 32; ++kt) {
+            const uint2 a = *reinterpret_cast<const uint2*>(qrow + kt * 64);
+            const uint2 b = *reinterpret_cast<const uint2*>(qrow + kt * 64 + 32);
+            qf[nt][kt][0] = a.x;
+            qf[nt][kt][1] = a.y;
+            qf[nt][kt][2] = b.x;
+            qf[nt][kt][3] = b.y;
+          }
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int r = nt * 8 + (lane & 3) * 2 + j;
+            const int R = u.row0 + r;
+            const int ps = (R < rows_total) ? base + R / G : -1;
+            pos_r[nt][j] = ps;
+            lo_r[nt][j] = (p.window > 0) ? ps - p.window : -1;
+            q_fac[nt][j] = qfac[r] * to_log2;
+            m_run[nt][j] = -INFINITY;
+            l_run[nt][j] = 0.f;
+          }
+#pragma unroll
+          for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[nt][kt][e] = 0.f;
+        }
+      }
+
+      const int key0 = pos + warp * TW;
+      if (key0 < u.kv_end) {
+        // ---- S^T[32 tokens x rows] = K . Q^T as two 16-token blocks
+        float sc[NT][2][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sc[nt][b][e] = 0.f;
+#pragma unroll
+        for (int kt = 0; kt < D / 32; ++kt) {
+          const int c16 = kt * 2;  // 16-byte chunk of the token's row; + k_dhalf at run time
+          const uint32_t coff = (uint32_t)(c16 / CH) * dc_stride + ((((uint32_t)(c16 % CH) | (uint32_t)k_dhalf) << 4) ^ swz);
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            // a[0] = (token g, bytes 4t..4t+3 of the chunk), a[1] = token g+8, a[2] / a[3] = the next chunk.  The low two
+            // bytes of a register become k slots 2t, 2t+1, the high two k slots 8+2t, 8+2t+1 of one f16 mma -- the
+            // query fragments were loaded in the same order
+            uint32_t a[4];
+            ldmatrix_x4(a, sbase + (b ? k_off1 : k_off0) + coff);
+            uint32_t lo[4], hi[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) Code::widen(a[i], lo[i], hi[i]);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              mma_f16(sc[nt][b], lo[0], lo[1], hi[0], hi[1], qf[nt][kt][0], qf[nt][kt][1]);
+              mma_f16(sc[nt][b], lo[2], lo[3], hi[2], hi[3], qf[nt][kt][2], qf[nt][kt][3]);
+            }
+          }
+        }
+        // ---- scales of this lane's four tokens, and the largest V scale of the warp's 32
+        const float* ks_s = reinterpret_cast<const float*>(smem + C::OFF_SCALE + s * (2 * TK * 4));
+        const float* vs_s = ks_s + TK;
+        const int e0 = pos >> sb_shift;
+        float ks[4], vs[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int key = key0 + (lane >> 2) + i * 8;
+          const int e = (key >> sb_shift) - e0;
+          ks[i] = ks_s[e];
+          // no row sees a key from kv_end on, or one that the window of the tile's first row has left behind
+          vs[i] = (key < u.kv_end && key > lo_min) ? vs_s[e] : 0.f;
+        }
+        {
+          float top = fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3]));
+          const uint32_t tb = __reduce_max_sync(0xffffffffu, __float_as_uint(top));  // positive floats order as integers
+          top = __uint_as_float(tb);
+          if (top * v_norm >= (float)(2 << kVBits)) {
+            // a larger scale than any before: take it to [2^6, 2^7) and the accumulators along
+            uint32_t e = tb >> 23;
+            e = e < 8u ? 8u : e;
+            const float v_new = __uint_as_float((254u + kVBits - e) << 23);
+            const float f = v_new * power_of_two_inverse(v_norm);  // 0 where the old terms are below anything that counts
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int mt = 0; mt < KT; ++mt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[nt][mt][i] *= f;
+            v_norm = v_new;
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) vs[i] *= v_norm;
+        }
+        const bool tail = key0 + TW > u.kv_end;  // tokens past the chunk end: stale or unowned bytes
+        const bool edge = tail || key0 <= lo_min;
+        const bool need_mask = tail || (key0 + TW - 1 > pos_min) || (key0 <= lo_max);
+        bool grow = false;
+        float mx[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+          for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int j = e & 1;
+              float x = sc[nt][b][e] * (q_fac[nt][j] * ks[b * 2 + (e >> 1)]);
+              if (p.cap != 0.f) x = p.cap_log2 * soft_cap_tanh(x);
+              if (need_mask) {
+                // a 128-token stage can straddle the end of a chunk (chunks are cut at multiples of 64): keys from
+                // kv_end on belong to the next chunk, or to nobody
+                const int key = key0 + b * 16 + (lane >> 2) + (e >> 1) * 8;
+                if (key > pos_r[nt][j] || key <= lo_r[nt][j] || key >= u.kv_end) x = -INFINITY;
+              }
+              sc[nt][b][e] = x;
+            }
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            float v = fmaxf(fmaxf(sc[nt][0][j], sc[nt][0][j + 2]), fmaxf(sc[nt][1][j], sc[nt][1][j + 2]));
+            v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
+            v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
+            v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
+            mx[nt][j] = v;
+            // lazy rescaling: keep the old reference maximum unless the new one is 2^8 larger
+            grow |= (v > m_run[nt][j] + kLazyRescale) || (m_run[nt][j] == -INFINITY && v > -INFINITY);
+          }
+        }
+        if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            float alpha[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const bool g = (mx[nt][j] > m_run[nt][j] + kLazyRescale) || (m_run[nt][j] == -INFINITY && mx[nt][j] > -INFINITY);
+              const float m_new = g ? mx[nt][j] : m_run[nt][j];
+              alpha[j] = g ? fast_exp2(m_run[nt][j] - m_new) : 1.f;  // exp2(-inf) = 0 on the first tile
+              m_run[nt][j] = m_new;
+              l_run[nt][j] *= alpha[j];
+            }
+#pragma unroll
+            for (int mt = 0; mt < KT; ++mt) {
+              acc[nt][mt][0] *= alpha[0];
+              acc[nt][mt][1] *= alpha[1];
+              acc[nt][mt][2] *= alpha[0];
+              acc[nt][mt][3] *= alpha[1];
+            }
+          }
+        }
+        // ---- probabilities; times the V scale to f16, transposed into the B fragments of P.V
+        uint32_t pbf[NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const float m_use = (m_run[nt][j] == -INFINITY) ? 0.f : m_run[nt][j];
+              const float p0 = fast_exp2(sc[nt][b][j] - m_use);
+              const float p1 = fast_exp2(sc[nt][b][j + 2] - m_use);
+              l_run[nt][j] += p0 + p1;
+              sc[nt][b][j] = p0 * vs[b * 2];
+              sc[nt][b][j + 2] = p1 * vs[b * 2 + 1];
+            }
+            pbf[nt][b * 2] = movmatrix_trans(Mma<__half>::pack(sc[nt][b][0], sc[nt][b][1]));
+            pbf[nt][b * 2 + 1] = movmatrix_trans(Mma<__half>::pack(sc[nt][b][2], sc[nt][b][3]));
+          }
+        }
+        // ---- V^T fragments: four transposed 8-token matrices of one 16-byte chunk; register j holds, for the two
+        // head-dim lanes 2g and 2g+1, tokens 8j + 2t (low half) and 8j + 2t + 1 (high half): rows g and g+8 of the mma
+        // stand for lanes 16mt + 2g and + 1.  The bytes of keys that no row sees are cleared, so that 0 * (stale
+        // NaN) cannot reach the accumulators.
+        uint32_t vmask[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
+        if (edge) {
+          const int t0 = key0 + (lane & 3) * 2;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int a = t0 + 8 * j;
+            vmask[j] = (a < u.kv_end && a > lo_min ? 0x0000ffffu : 0u) | (a + 1 < u.kv_end && a + 1 > lo_min ? 0xffff0000u : 0u);
+          }
+        }
+#pragma unroll
+        for (int mt = 0; mt < KT; ++mt) {
+          uint32_t r[4];
+          ldmatrix_x4_trans(r, sbase + v_off + (uint32_t)(mt / CH) * dc_stride + (((uint32_t)(mt % CH) << 4) ^ swz));
+          if (edge) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) r[j] &= vmask[j];
+          }
+          uint32_t even[4], odd[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) Code::widen_interleaved(r[j], even[j], odd[j]);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            mma_f16(acc[nt][mt], even[0], odd[0], even[1], odd[1], pbf[nt][0], pbf[nt][1]);
+            mma_f16(acc[nt][mt], even[2], odd[2], even[3], odd[3], pbf[nt][2], pbf[nt][3]);
+          }
+        }
+      }
+      // this warp is done with the stage's bytes (query fragments are in registers by now)
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar_empty + s * 8);
+
+      if (pos + TK >= u.kv_end) {
+        // ---- end of item: combine the four warps ----
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            float l = l_run[nt][j];
+            l += __shfl_xor_sync(0xffffffffu, l, 4);
+            l += __shfl_xor_sync(0xffffffffu, l, 8);
+            l += __shfl_xor_sync(0xffffffffu, l, 16);
+            if (lane < 4) {
+              const int r = nt * 8 + lane * 2 + j;
+              mbuf[warp * RT + r] = m_run[nt][j];
+              lbuf[warp * RT + r] = l;
+            }
+          }
+        if (!consumer_sync()) break;
+        // Every lane derives the rescale factors of its own rows from the four (m, l) pairs; the
+        // accumulators are then added into obuf in four rounds, warp w handling the d-slice
+        // (w + round) % 4, so each address receives its four contributions in a fixed order and
+        // the result does not depend on warp timing (no floating-point atomics).
+        // (v_back undoes the power of two that this warp took the V scales by)
+        const float v_back = power_of_two_inverse(v_norm);
+        float f_own[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int r = nt * 8 + (lane & 3) * 2 + j;
+            float mt = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < kConsumerWarps; ++w) mt = fmaxf(mt, mbuf[w * RT + r]);
+            const float mu = (mt == -INFINITY) ? 0.f : mt;
+            f_own[nt][j] = fast_exp2(m_run[nt][j] - mu) * v_back;
+          }
+        if (tid < RT) {
+          const int r = tid;
+          float mt = -INFINITY;
+#pragma unroll
+          for (int w = 0; w < kConsumerWarps; ++w) mt = fmaxf(mt, mbuf[w * RT + r]);
+          const float mu = (mt == -INFINITY) ? 0.f : mt;
+          float lt = 0.f;
+#pragma unroll
+          for (int w = 0; w < kConsumerWarps; ++w) lt += lbuf[w * RT + r] * fast_exp2(mbuf[w * RT + r] - mu);
+          float scl = 1.f;
+          if (u.slot < 0) {
+            float l_fin = lt;
+            if (p.num_sinks > 0 && r < n_rows) {
+              // attention sinks join the denominator only
+              const int R = u.row0 + r;
+              const int hq = h * G + (R % G);
+              const int srow = (p.sink_rows == p.Hq) ? hq : (p.sink_rows == Hkv ? h : 0);
+              const float* sk = p.sinks + (size_t)srow * p.num_sinks;
+              float sm = -INFINITY;
+              for (int i = 0; i < p.num_sinks; ++i) sm = fmaxf(sm, sk[i] * kLog2e);
+              const float m_fin = fmaxf(mt, sm);
+              const float mf = (m_fin == -INFINITY) ? 0.f : m_fin;
+              scl = fast_exp2(mt - mf);
+              l_fin = lt * scl;
+              for (int i = 0; i < p.num_sinks; ++i) l_fin += fast_exp2(sk[i] * kLog2e - mf);
+            }
+            scl = (l_fin > 0.f) ? scl / l_fin : 0.f;
+          }
+          row_scale[r] = scl;
+          row_m[r] = mt;
+          row_l[r] = lt;
+        }
+        bool alive_c = true;
+#pragma unroll
+        for (int round = 0; round < kConsumerWarps; ++round) {
+          const int slice = (warp + round) % kConsumerWarps;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            const int r0 = nt * 8 + (lane & 3) * 2;
+            const float f0 = f_own[nt][0], f1 = f_own[nt][1];
+#pragma unroll
+            for (int mi = 0; mi < KT / kConsumerWarps; ++mi) {
+              // compile-time accumulator index in every branch keeps acc[] in registers
+#pragma unroll
+              for (int sl = 0; sl < kConsumerWarps; ++sl) {
+                if (sl == slice) {
+                  const int mt = sl * (KT / kConsumerWarps) + mi;
+                  // accumulator rows g / g+8 of block mt are head-dim lanes 16mt + 2g / + 1 (see the V fragments)
+                  constexpr int HI = 1;
+                  const int d = mt * 16 + (lane >> 2) * 2;
+                  float* o0 = &obuf[r0 * D + d];
+                  float* o1 = &obuf[(r0 + 1) * D + d];
+                  if (round == 0) {
+                    o0[0] = acc[nt][mt][0] * f0;
+                    o0[HI] = acc[nt][mt][2] * f0;
+                    o1[0] = acc[nt][mt][1] * f1;
+                    o1[HI] = acc[nt][mt][3] * f1;
+                  } else {
+                    o0[0] += acc[nt][mt][0] * f0;
+                    o0[HI] += acc[nt][mt][2] * f0;
+                    o1[0] += acc[nt][mt][1] * f1;
+                    o1[HI] += acc[nt][mt][3] * f1;
+                  }
+                }
+              }
+            }
+          }
+          if (!consumer_sync()) {
+            alive_c = false;
+            break;
+          }
+        }
+        if (!alive_c) break;
+        constexpr int kCT = kConsumerWarps * 32;
+        if (u.slot < 0) {
+          T* out = reinterpret_cast<T*>(p.out);
+          for (int i = tid; i < n_rows * (D / 2); i += kCT) {
+            const int r = i / (D / 2), d = (i % (D / 2)) * 2;
+            const int R = u.row0 + r;
+            const int qt = R / G, g = R - qt * G;
+            const float scl = row_scale[r];
+            const float2 v = *reinterpret_cast<float2*>(&obuf[r * D + d]);
+            *reinterpret_cast<uint32_t*>(out + ((size_t)(u.q_start + qt) * p.Hq + h * G + g) * D + d) =
+                  Mma<T>::pack(v.x * scl, v.y * scl);
+          }
+        } else {
+          float* po = p.part_o + ((size_t)u.slot * Hkv + h) * RT * D;
+          float2* pml = p.part_ml + ((size_t)u.slot * Hkv + h) * RT;
+          for (int i = tid; i < n_rows * (D / 4); i += kCT) {
+            const int r = i / (D / 4), d = (i % (D / 4)) * 4;
+            const float4 v = *reinterpret_cast<float4*>(&obuf[r * D + d]);
+            *reinterpret_cast<float4*>(po + r * D + d) = v;
+          }
+          if (tid < n_rows) pml[tid] = make_float2(row_m[tid], row_l[tid]);
+          if (p.fused_merge) {
+            // Last-arriver merge: publish this chunk's partial, take a ticket for (tile, kv head); the
+            // chunk that draws the last ticket combines all of them, in chunk order, so the result
+            // does not depend on which chunk finished last.  No CTA ever waits for another.
+            __threadfence();
+            if (!consumer_sync()) break;
+            if (tid == 0) {
+              const int old = atomicAdd(&p.tickets[(size_t)u.merge_idx * Hkv + h], 1);
+              row_l[0] = (old == u.n_chunks - 1) ? 1.f : 0.f;  // row_l/row_m were consumed above
+            }
+            if (!consumer_sync()) break;
+            const bool last = row_l[0] != 0.f;
+            if (last) {
+              __threadfence();
+              constexpr int VPL = D / 32;
+              const int slot0 = u.slot - u.chunk_idx;
+              T* out = reinterpret_cast<T*>(p.out);
+              for (int r = warp; r < n_rows; r += kConsumerWarps) {
+                float m_tot = -INFINITY;
+                for (int c = lane; c < u.n_chunks; c += 32)
+                  m_tot = fmaxf(m_tot, __ldcg(&p.part_ml[((size_t)(slot0 + c) * Hkv + h) * RT + r]).x);
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) m_tot = fmaxf(m_tot, __shfl_xor_sync(0xffffffffu, m_tot, o));
+                const float mu = (m_tot == -INFINITY) ? 0.f : m_tot;
+                float accm[VPL];
+#pragma unroll
+                for (int i = 0; i < VPL; ++i) accm[i] = 0.f;
+                float l_tot = 0.f;
+                // kMergeInFlight chunks' loads in flight at a time (each is an L2 round trip); the sums still run in
+                // chunk order
+                for (int c0 = 0; c0 < u.n_chunks; c0 += kMergeInFlight) {
+                  float2 ml[kMergeInFlight];
+                  float vv[kMergeInFlight][VPL];
+#pragma unroll
+                  for (int j = 0; j < kMergeInFlight; ++j) {
+                    const int c = min(c0 + j, u.n_chunks - 1);
+                    const size_t base = ((size_t)(slot0 + c) * Hkv + h) * RT + r;
+                    ml[j] = __ldcg(&p.part_ml[base]);
+                    const float* src = p.part_o + base * D + lane * VPL;
+                    if constexpr (VPL == 2) {
+                      const float2 v = __ldcg(reinterpret_cast<const float2*>(src));
+                      vv[j][0] = v.x;
+                      vv[j][1] = v.y;
+                    } else {
+#pragma unroll
+                      for (int i = 0; i < VPL; i += 4) {
+                        const float4 v = __ldcg(reinterpret_cast<const float4*>(src + i));
+                        vv[j][i] = v.x;
+                        vv[j][i + 1] = v.y;
+                        vv[j][i + 2] = v.z;
+                        vv[j][i + 3] = v.w;
+                      }
+                    }
+                  }
+#pragma unroll
+                  for (int j = 0; j < kMergeInFlight; ++j) {
+                    if (c0 + j < u.n_chunks) {
+                      const float f = fast_exp2(ml[j].x - mu);
+                      l_tot += ml[j].y * f;
+#pragma unroll
+                      for (int i = 0; i < VPL; ++i) accm[i] += vv[j][i] * f;
+                    }
+                  }
+                }
+                const int R = u.row0 + r;
+                const int qt = R / G, g = R - qt * G;
+                const int hq = h * G + g;
+                float scl = 1.f, l_fin = l_tot;
+                if (p.num_sinks > 0) {
+                  const int srow = (p.sink_rows == p.Hq) ? hq : (p.sink_rows == Hkv ? h : 0);
+                  const float* sk = p.sinks + (size_t)srow * p.num_sinks;
+                  float sm = -INFINITY;
+                  for (int i = 0; i < p.num_sinks; ++i) sm = fmaxf(sm, sk[i] * kLog2e);
+                  const float m_fin = fmaxf(m_tot, sm);
+                  const float mf = (m_fin == -INFINITY) ? 0.f : m_fin;
+                  scl = fast_exp2(m_tot - mf);
+                  l_fin = l_tot * scl;
+                  for (int i = 0; i < p.num_sinks; ++i) l_fin += fast_exp2(sk[i] * kLog2e - mf);
+                }
+                scl = (l_fin > 0.f) ? scl / l_fin : 0.f;
+                T* dst = out + ((size_t)(u.q_start + qt) * p.Hq + hq) * D + lane * VPL;
+                {
+#pragma unroll
+                  for (int i = 0; i < VPL; i += 2)
+                    *reinterpret_cast<uint32_t*>(dst + i) = Mma<T>::pack(accm[i] * scl, accm[i + 1] * scl);
+                }
+              }
+            }
+          }
+        }
+        // The next item's writes to mbuf/lbuf come before its first consumer_sync, but they only
+        // race with readers of mbuf/lbuf, and those finished before the first combine step's sync above; its
+        // writes to obuf/row_* come after its first consumer_sync, which every warp reaches only
+        // after finishing the loops above.
+      }
+      if (++s == NS) {
+        s = 0;
+        full_parity ^= 1u;
+      }
+    }
+    if (*abort_flag) flags |= EJK_RPA_ST_TIMEOUT;
+  }
+  if (flags && p.status) atomicOr(reinterpret_cast<unsigned*>(p.status), flags);
+  zero_tail_rows(p.out, p.header[kHdrTailStart], p.T, (size_t)p.Hq * D * sizeof(T));
+  // In a mixed batch this grid is a programmatic dependent of the prefill-tile grid and never waited for it
+  // (the two write different rows).  Whatever follows in the stream, though, is only ordered after THIS grid:
+  // one thread per CTA now waits for the prefill grid, so this grid cannot complete before it, and a later
+  // kernel (a reader of `out`, the next call's planner) is ordered after both.  All prefill CTAs are resident
+  // before this grid starts (it is released when each of them has seen the plan), so the wait cannot starve them.
+  if ((p.pdl & 1) && tid == 0) pdl_wait();
+}
+
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                              const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                              CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeFn encode_fn() {
+  static EncodeFn fn = nullptr;
+  if (!fn) {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      return nullptr;
+    fn = reinterpret_cast<EncodeFn>(ptr);
+  }
+  return fn;
+}
+
+template <typename T, typename Code, int D, int NT, int NS>
+cudaError_t launch_one(const Params& p, const Q8Cache& c, const CUtensorMap& map, int n_sm, cudaStream_t stream, bool pdl) {
+  using C = Cfg<D, NT, NS>;
+  auto kern = q8_splitkv_kernel<T, Code, D, NT, NS>;
+  static std::atomic<bool> configured[64];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= 64 || !configured[dev].load(std::memory_order_acquire)) {
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES);
+    if (e != cudaSuccess) return e;
+    if (dev >= 0 && dev < 64) configured[dev].store(true, std::memory_order_release);
+  }
+  return launch_kernel(kern, dim3(n_sm * C::CTAS), dim3(kThreads), C::SMEM_BYTES, stream, pdl, map, p, c);
+}
+
+template <typename T, typename Code>
+cudaError_t dispatch(const Params& p, const Q8Cache& c, const CUtensorMap& map, int n_sm, cudaStream_t stream, bool pdl) {
+  const bool wide = p.rows_per_tile == 16;
+  switch (p.D) {
+    case 64:
+      return wide ? launch_one<T, Code, 64, 2, 5>(p, c, map, n_sm, stream, pdl) : launch_one<T, Code, 64, 1, 5>(p, c, map, n_sm, stream, pdl);
+    case 128:
+      return wide ? launch_one<T, Code, 128, 2, 5>(p, c, map, n_sm, stream, pdl) : launch_one<T, Code, 128, 1, 3>(p, c, map, n_sm, stream, pdl);
+    case 256:
+      return wide ? launch_one<T, Code, 256, 2, 2>(p, c, map, n_sm, stream, pdl) : launch_one<T, Code, 256, 1, 3>(p, c, map, n_sm, stream, pdl);
+  }
+  return cudaErrorInvalidValue;
+}
+
+}  // namespace
+
+bool q8_tma_supported(int page_size) {
+  // boxes are whole 8-token groups of one page: the period of the swizzle
+  return page_size >= 8 && page_size % 8 == 0 && encode_fn() != nullptr;
+}
+
+// kv_pages as a tensor map, innermost first: one swizzle span of bytes | token in page | column of head_dim | head and K or
+// V | page.  One box is `box_tokens` tokens of one head, K and V.
+cudaError_t q8_tensor_map(CUtensorMap* map, const Q8Cache& c, int box_tokens) {
+  EncodeFn enc = encode_fn();
+  if (!enc) return cudaErrorNotSupported;
+  const cuuint64_t D = c.D, rb = c.D < 128 ? c.D : 128, page = c.page_size, planes = 2ull * c.Hkv;
+  cuuint64_t dims[5] = {rb, page, D / rb, planes, (cuuint64_t)c.num_pages};
+  cuuint64_t strides[4] = {D, rb, page * D, planes * page * D};
+  cuuint32_t box[5] = {(cuuint32_t)rb, (cuuint32_t)box_tokens, (cuuint32_t)(D / rb), 2, 1};
+  cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+  const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 5, c.pages, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         rb == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
+cudaError_t launch_q8_splitkv(const Params& p, const Q8Cache& c, int dtype, int code, int n_sm, cudaStream_t stream, bool pdl) {
+  CUtensorMap map;
+  if (cudaError_t e = q8_tensor_map(&map, c, p.tma_block_tokens); e != cudaSuccess) return e;
+  if (code == EJK_Q8_I8)
+    return dtype == EJK_RPA_BF16 ? dispatch<__nv_bfloat16, CodeI8>(p, c, map, n_sm, stream, pdl)
+                                 : dispatch<__half, CodeI8>(p, c, map, n_sm, stream, pdl);
+  return dtype == EJK_RPA_BF16 ? dispatch<__nv_bfloat16, CodeE4M3>(p, c, map, n_sm, stream, pdl)
+                               : dispatch<__half, CodeE4M3>(p, c, map, n_sm, stream, pdl);
+}
+
+}  // namespace ejk

@@ -1,5 +1,6 @@
 // The 8-bit cache: parameters of its kernels and the conversions of its codes.
 #pragma once
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <stdint.h>
@@ -18,7 +19,27 @@ struct Q8Cache {
   int32_t block_shift;  // log2 of the tokens that share a scale
 };
 
+// Codes to f16, exactly, four at a time.  widen: bytes 0, 1 and 2, 3 of `w`; widen_interleaved: bytes 0, 2 and 1, 3.
+__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
+  uint32_t r;
+  asm("prmt.b32 %0, %1, %2, %3;\n" : "=r"(r) : "r"(a), "r"(b), "r"(sel));
+  return r;
+}
+
 struct CodeE4M3 {
+  static __device__ __forceinline__ uint32_t widen2(uint32_t two) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;\n" : "=r"(r) : "h"((uint16_t)two));
+    return r;
+  }
+  static __device__ __forceinline__ void widen(uint32_t w, uint32_t& lo, uint32_t& hi) {
+    lo = widen2(w);
+    hi = widen2(w >> 16);
+  }
+  static __device__ __forceinline__ void widen_interleaved(uint32_t w, uint32_t& even, uint32_t& odd) {
+    widen(prmt(w, w, 0x3120u), even, odd);
+  }
+
   static constexpr int kId = EJK_RPA_E4M3;
   static constexpr float kMax = 448.f;
   static __device__ __forceinline__ float decode(uint8_t c) {
@@ -38,6 +59,23 @@ struct CodeE4M3 {
   }
 };
 struct CodeI8 {
+  // byte + 128 under the exponent of 1024 is the f16 1152 + code; the difference is exact
+  static __device__ __forceinline__ uint32_t less_1152(uint32_t w) {
+    const uint32_t b = 0x64806480u;
+    const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&w), *reinterpret_cast<const __half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&d);
+  }
+  static __device__ __forceinline__ void widen(uint32_t w, uint32_t& lo, uint32_t& hi) {
+    w ^= 0x80808080u;
+    lo = less_1152(prmt(w, 0x64646464u, 0x4140u));
+    hi = less_1152(prmt(w, 0x64646464u, 0x4342u));
+  }
+  static __device__ __forceinline__ void widen_interleaved(uint32_t w, uint32_t& even, uint32_t& odd) {
+    w ^= 0x80808080u;
+    even = less_1152(prmt(w, 0x64646464u, 0x4240u));
+    odd = less_1152(prmt(w, 0x64646464u, 0x4341u));
+  }
+
   static constexpr int kId = EJK_Q8_I8;
   static constexpr float kMax = 127.f;
   static __device__ __forceinline__ float decode(uint8_t c) { return (float)(int8_t)c; }
@@ -78,6 +116,10 @@ void set_last_launches(int n);
 
 // launchers
 cudaError_t launch_q8_gather(const Params& p, const Q8Cache& c, int dtype, int code, cudaStream_t stream);
+// the pipelined kernel: page sizes that are multiples of 8
+bool q8_tma_supported(int page_size);
+cudaError_t q8_tensor_map(CUtensorMap* map, const Q8Cache& c, int box_tokens);
+cudaError_t launch_q8_splitkv(const Params& p, const Q8Cache& c, int dtype, int code, int n_sm, cudaStream_t stream, bool pdl);
 cudaError_t launch_q8_write(const void* keys, const void* values, long long key_stride, long long value_stride,
                             const Q8Cache& c, const int32_t* slots, int32_t* status, int rows, int dtype, int code,
                             cudaStream_t stream);
