@@ -62,7 +62,10 @@ extern "C" {
 size_t ejk_q8_workspace_bytes(const ejk_q8_shape* shape) {
   if (!shape || check_attention(*shape) != 0) return 0;
   const int n_sm = sm100_sm_count();
-  return n_sm ? workspace_layout(as_rpa(*shape), n_sm).total : 0;
+  if (!n_sm) return 0;
+  const WorkspaceLayout L = workspace_layout(as_rpa(*shape), n_sm);
+  // shapes that can hold a multi-token sequence also get room for the parts of tensor-tile items cut along KV
+  return shape->total_tokens > shape->max_num_seqs && q8_prefill_supported(shape->head_dim) ? L.total_split : L.total;
 }
 
 int ejk_q8_attention_launch(const void* queries, const void* kv_pages, const float* kv_scales,
@@ -168,14 +171,37 @@ int ejk_q8_attention_launch(const void* queries, const void* kv_pages, const flo
     p.fused_merge = (opt.fused_merge == 2 || (opt.fused_merge == 1 && few)) ? 1 : 0;
   }
   p.prefill_item_rows = prefill_rows_per_item(s.head_dim);
+  // Batches that can hold a sequence with many query rows also get the tensor-tile kernel; whether one qualifies is
+  // decided by the planner on the device.
+  int prefill_rows = opt.prefill_rows;
+  if (a.num_queries_per_block > 0) {  // per-call hint: query tokens from which on a sequence is served by tensor tiles
+    const long long r = (long long)a.num_queries_per_block * p.G;
+    prefill_rows = r > 0x40000000ll ? 0x40000000 : (int)r;
+  }
+  const bool use_prefill = prefill_rows > 0 && q8_prefill_supported(s.head_dim) &&
+                           (long long)s.total_tokens * p.G >= prefill_rows && s.total_tokens > s.max_num_seqs;
+  p.prefill_min_rows = use_prefill ? prefill_rows : 0;
+  p.prefill_share = opt.prefill_share;
+  if (use_prefill && opt.prefill_split && workspace_bytes >= L.total_split) {
+    p.pprefix = reinterpret_cast<int32_t*>(ws + L.pprefix_off);
+    p.ptickets = reinterpret_cast<int32_t*>(ws + L.ptickets_off);
+    p.ppart_ml = reinterpret_cast<float2*>(ws + L.ppart_ml_off);
+    p.ppart_o = reinterpret_cast<float*>(ws + L.ppart_o_off);
+    p.prefill_split = opt.prefill_split;
+  }
   // Kernels of one call are launched as programmatic dependents: each waits on the device for what it needs of the one
   // before, the planner for whatever precedes the call.
   const bool pdl = opt.overlap != 0;
-  p.pdl = pdl ? 2 : 0;
+  p.pdl = pdl ? (use_prefill ? 1 : 2) : 0;
   int launches = 0;
   cudaError_t e = launch_plan(p, st, pdl);
   if (e != cudaSuccess) return static_cast<int>(e);
   ++launches;
+  if (use_prefill) {
+    e = launch_q8_prefill(p, c, s.dtype, s.code_dtype, n_sm, st, pdl);
+    if (e != cudaSuccess) return static_cast<int>(e);
+    ++launches;
+  }
   e = launch_q8_splitkv(p, c, s.dtype, s.code_dtype, n_sm, st, pdl);
   if (e != cudaSuccess) return static_cast<int>(e);
   ++launches;

@@ -120,6 +120,9 @@ cudaError_t launch_q8_gather(const Params& p, const Q8Cache& c, int dtype, int c
 bool q8_tma_supported(int page_size);
 cudaError_t q8_tensor_map(CUtensorMap* map, const Q8Cache& c, int box_tokens);
 cudaError_t launch_q8_splitkv(const Params& p, const Q8Cache& c, int dtype, int code, int n_sm, cudaStream_t stream, bool pdl);
+// tcgen05 tiles for sequences with many query rows (head_dim 64 and 128)
+bool q8_prefill_supported(int head_dim);
+cudaError_t launch_q8_prefill(const Params& p, const Q8Cache& c, int dtype, int code, int n_sm, cudaStream_t stream, bool pdl);
 cudaError_t launch_q8_write(const void* keys, const void* values, long long key_stride, long long value_stride,
                             const Q8Cache& c, const int32_t* slots, int32_t* status, int rows, int dtype, int code,
                             cudaStream_t stream);
