@@ -572,6 +572,7 @@ q8_prefill_kernel(const Params p, const Q8Cache cache) {
     // swizzled stage, both without bank conflicts
     constexpr int CPT = D / 8;            // 8-code chunks per token
     constexpr int TSTEP = 128 / CPT;      // tokens per step of the four warps
+    static_assert(kBN % (2 * TSTEP) == 0, "two tokens per step and thread");
     const int ch = ctid % CPT, t0 = ctid / CPT;
     const float to_log2 = p.cap != 0.f ? p.inv_cap_scale : p.scale_log2;
     float v_norm = 1.f;
@@ -581,8 +582,8 @@ q8_prefill_kernel(const Params p, const Q8Cache cache) {
       const int rs = gi % NR, st = gi % NS;
       if (!mbar_wait(bar_raw_full(rs), (gi / NR) & 1, abort_flag, wait_ns)) break;
       const int2 meta = raw_metas[rs];
-      if (!mbar_wait(bar_kv_empty(st), ((gi / NS) & 1) ^ 1, abort_flag, wait_ns)) break;
       if (meta.x < 0) {  // the end marker goes on
+        if (!mbar_wait(bar_kv_empty(st), ((gi / NS) & 1) ^ 1, abort_flag, wait_ns)) break;
         if (ctid == 0) metas[st] = meta;
         __syncwarp();
         if (lane == 0) {
@@ -602,20 +603,19 @@ q8_prefill_kernel(const Params p, const Q8Cache cache) {
         v_norm = __uint_as_float((127u + 125u) << 23);  // no scale met yet: the largest power of two
       }
       // the largest V scale of the stage's keys that some row sees; every warp computes the same
-      {
-        uint32_t tb = 0;
+      uint32_t tb = 0;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int key = pos + lane + 32 * i;
-          if (key < kv_end && key > lo_min) tb = max(tb, __float_as_uint(vs_s[(key >> sb_shift) - e0]));
-        }
-        tb = __reduce_max_sync(0xffffffffu, tb);  // positive floats order as integers
-        if (__uint_as_float(tb) * v_norm >= (float)(2 << kVBits)) {
-          uint32_t e = tb >> 23;
-          e = e < 8u ? 8u : e;
-          v_norm = __uint_as_float((254u + kVBits - e) << 23);
-        }
+      for (int i = 0; i < kBN / 32; ++i) {
+        const int key = pos + lane + 32 * i;
+        if (key < kv_end && key > lo_min) tb = max(tb, __float_as_uint(vs_s[(key >> sb_shift) - e0]));
       }
+      tb = __reduce_max_sync(0xffffffffu, tb);  // positive floats order as integers
+      if (__uint_as_float(tb) * v_norm >= (float)(2 << kVBits)) {
+        uint32_t e = tb >> 23;
+        e = e < 8u ? 8u : e;
+        v_norm = __uint_as_float((254u + kVBits - e) << 23);
+      }
+      if (!mbar_wait(bar_kv_empty(st), ((gi / NS) & 1) ^ 1, abort_flag, wait_ns)) break;
       if (ctid < kBN) {
         const int key = pos + ctid;
         reinterpret_cast<float*>(smem + C::OFF_KSCALE + st * (kBN * 4))[ctid] = key < kv_end ? ks_s[(key >> sb_shift) - e0] * to_log2 : 0.f;
@@ -626,24 +626,36 @@ q8_prefill_kernel(const Params p, const Q8Cache cache) {
       }
       const uint8_t* raw = smem + C::OFF_RAW + rs * C::RAW_BYTES + ch * 8;
       uint8_t* out = smem + C::OFF_KV + st * C::STAGE_BYTES + (ch >> 3) * 1024;
+      // a short loop on purpose: the roles of this kernel share an instruction cache that their unrolled bodies overflow
+      // (all of a stage unrolled: 2.57 ms where this takes %UNROLL%)
+#pragma unroll 1
+      for (int t = t0; t < kBN; t += 2 * TSTEP) {
+        uint2 kc[2], vc[2];
+        float f[2];
 #pragma unroll
-      for (int t = t0; t < kBN; t += TSTEP) {
-        const uint32_t at = (uint32_t)(t >> 3) * C::GROUP_BYTES + (uint32_t)(t & 7) * 128 + (uint32_t)(((ch & 7) ^ (t & 7)) << 4);
-        const uint2 k = *reinterpret_cast<const uint2*>(raw + t * D);
-        uint32_t w[4];
-        Code::widen(k.x, w[0], w[1]);
-        Code::widen(k.y, w[2], w[3]);
-        *reinterpret_cast<uint4*>(out + at) = make_uint4(from_f16x2<T>(w[0]), from_f16x2<T>(w[1]), from_f16x2<T>(w[2]), from_f16x2<T>(w[3]));
-        const int key = pos + t;
-        uint4 v = make_uint4(0u, 0u, 0u, 0u);  // keys that no row sees: stale or unowned bytes, possibly NaN
-        if (key < kv_end && key > lo_min) {
-          const uint2 c = *reinterpret_cast<const uint2*>(raw + (kBN + t) * D);
-          const __half2 f = __float2half2_rn(vs_s[(key >> sb_shift) - e0] * v_norm);
-          Code::widen(c.x, w[0], w[1]);
-          Code::widen(c.y, w[2], w[3]);
-          v = make_uint4(mul_f16x2(w[0], f), mul_f16x2(w[1], f), mul_f16x2(w[2], f), mul_f16x2(w[3], f));
+        for (int i = 0; i < 2; ++i) {
+          kc[i] = *reinterpret_cast<const uint2*>(raw + (t + i * TSTEP) * D);
+          vc[i] = *reinterpret_cast<const uint2*>(raw + (kBN + t + i * TSTEP) * D);
+          const int key = pos + t + i * TSTEP;
+          f[i] = vs_s[(key >> sb_shift) - e0] * v_norm;
+          if (key >= kv_end || key <= lo_min) {  // V of a key that no row sees is zero: those are stale bytes, possibly NaN
+            vc[i] = make_uint2(0u, 0u);
+            f[i] = 0.f;
+          }
         }
-        *reinterpret_cast<uint4*>(out + C::V_OFF + at) = v;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int tt = t + i * TSTEP;
+          const uint32_t at = (uint32_t)(tt >> 3) * C::GROUP_BYTES + (uint32_t)(tt & 7) * 128 + (uint32_t)(((ch & 7) ^ (tt & 7)) << 4);
+          uint32_t w[4];
+          Code::widen(kc[i].x, w[0], w[1]);
+          Code::widen(kc[i].y, w[2], w[3]);
+          *reinterpret_cast<uint4*>(out + at) = make_uint4(from_f16x2<T>(w[0]), from_f16x2<T>(w[1]), from_f16x2<T>(w[2]), from_f16x2<T>(w[3]));
+          const __half2 f2 = __float2half2_rn(f[i]);
+          Code::widen(vc[i].x, w[0], w[1]);
+          Code::widen(vc[i].y, w[2], w[3]);
+          *reinterpret_cast<uint4*>(out + C::V_OFF + at) = make_uint4(mul_f16x2(w[0], f2), mul_f16x2(w[1], f2), mul_f16x2(w[2], f2), mul_f16x2(w[3], f2));
+        }
       }
       fence_async_smem();  // the MMAs read the stage through the async proxy
       __syncwarp();
@@ -788,11 +800,11 @@ q8_prefill_kernel(const Params p, const Q8Cache cache) {
             sr[i + 2] = __float_as_uint(__uint_as_float(sr[i + 2]) * f.z);
             sr[i + 3] = __float_as_uint(__uint_as_float(sr[i + 3]) * f.w);
           }
-          if (p.cap != 0.f) {
+          if (__builtin_expect(p.cap != 0.f, 0)) {
 #pragma unroll
             for (int i = 0; i < HB; ++i) sr[i] = __float_as_uint(p.cap_log2 * soft_cap_tanh(__uint_as_float(sr[i])));
           }
-          if (!full_vis) {
+          if (__builtin_expect(!full_vis, 0)) {
             const int hi_i = pos_row - pos;  // last visible column of the stage
             const int lo_i = lo_row - pos;   // columns up to here are left of the window
 #pragma unroll
