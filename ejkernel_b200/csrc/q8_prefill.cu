@@ -7,11 +7,11 @@
 //
 //   producer warp --raw stage (codes: bulk copies; scales: 4-byte cp.async)--> four converter warps --16-bit stage--> MMAs
 //
-//   * the converters write K as the queries' type (a code has at most 8 significant bits: exact in bf16 and f16) and V as
-//     f16, both in the swizzled layout that the tensor cores read.  An 8-bit MMA would take the codes as they are, but
-//     would need q and P in 8 bits too.
-//   * k_scale goes into the logits, a multiplication per element by a factor that the row threads read from shared memory
-//     (64 per stage, the same for all rows).
+//   * the converters write K and V as f16 (K exactly) in the swizzled layout that the tensor cores read.  An 8-bit MMA would
+//     take the codes as they are, but would need q and P in 8 bits too.
+//   * bf16 queries go to f16 by a power of two per row (their largest element to [2^14, 2^15)), undone on the logits.
+//   * k_scale goes into the logits: where blocks have 8 tokens or more (and neither a soft cap nor a negative scale
+//     interferes) as the multiplier of the exponent's FMA, one factor per 8 columns; otherwise one per column.
 //   * v_scale goes into V, where it costs the softmax threads, which bound the kernel, nothing: the converters multiply by
 //     v_scale / v_ref, v_ref a power of two that keeps the products within f16: the largest v_scale met so far is taken to
 //     [2^6, 2^7), and a power of two times a code is exact down to 2^-24.  When a larger scale comes, v_ref grows and the
@@ -19,7 +19,7 @@
 //   * P is f16.  Its reference sits 2^7 below the maximum it was chosen for, which puts the weights between 2^15 and 2^-24:
 //     what is below 2^-31 of the largest weight is lost.
 //   * registers: 16 warps have 128 registers a thread; the issuing warps and the converters give theirs to the softmax
-//     warps (setmaxnreg: 80 + 96 + 2 * 168 = 4 * 128).
+//     warps (setmaxnreg: 64 + 72 + 2 * 184 <= 4 * 128).
 //
 // Warp roles (512 threads with two tiles, 384 with one; one CTA per SM, persistent over the planner's prefill queue):
 //   warp 0 producer, warp 1 S of tile 0 (and the TMEM allocation), warp 2 S of tile 1, warp 3 P.V of all tiles,
@@ -65,7 +65,7 @@ struct CfgP {
   static constexpr int CV_WARPS = 4;                  // converter warps
   static constexpr int THREADS = 32 * (4 + CV_WARPS + SM_WARPS * NT);
   static constexpr int REGS = 65536 / THREADS / 8 * 8;  // per thread at launch
-  static constexpr int REGS_ISSUE = 80, REGS_CONVERT = 96, REGS_SOFTMAX = 168;
+  static constexpr int REGS_ISSUE = 64, REGS_CONVERT = 72, REGS_SOFTMAX = 184;
   static_assert(REGS_ISSUE + REGS_CONVERT + NT * REGS_SOFTMAX <= (2 + NT) * REGS, "setmaxnreg.inc draws on the block's own registers");
   static constexpr int RAW_BYTES = BN * 2 * D;        // a stage of codes: [K|V][BN][D]
   static constexpr int STAGE_BYTES = BN * 2 * D * 2;  // a stage of 16-bit values
@@ -122,22 +122,13 @@ template <int N>
 __device__ __forceinline__ void take_registers() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(N));
 }
-// two f16 as two values of the queries' type
-template <typename T>
-__device__ __forceinline__ uint32_t from_f16x2(uint32_t w) {
-  if constexpr (std::is_same<T, __half>::value) {
-    return w;
-  } else {
-    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
-    return Mma<T>::pack(f.x, f.y);  // exact: a code has at most 8 significant bits
-  }
-}
 __device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, __half2 b) {
   const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), b);
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 
-template <typename T, typename Code, int D>
+// PLAIN: scale blocks of 8 tokens or more, no soft cap, a positive scale
+template <typename T, typename Code, int D, bool PLAIN>
 __global__ void __launch_bounds__(CfgP<D>::THREADS, 1)
 q8_prefill_kernel(const Params p, const Q8Cache cache) {
   using C = CfgP<D>;
@@ -450,7 +441,7 @@ q8_prefill_kernel(const Params p, const Q8Cache cache) {
     if (lane == 0 && (warp == 3 || warp - 1 < NT)) {
       const bool is_s = warp < 3;
       const int x = is_s ? warp - 1 : 0;
-      constexpr uint32_t idesc_s = instr_desc<T>(kBN, false);
+      constexpr uint32_t idesc_s = instr_desc<__half>(kBN, false);
       constexpr uint32_t idesc_pv = instr_desc<__half>(D, true);
       // hi word of a descriptor: stride byte offset >> 4, version 1 (bit 46), SWIZZLE_128B (bits 61-63)
       constexpr uint64_t kHiAtom1024 = ((uint64_t)((1024u >> 4) | (1u << 14) | (2u << 29))) << 32;
@@ -568,12 +559,15 @@ q8_prefill_kernel(const Params p, const Q8Cache cache) {
     // =============================== converters ===============================
     const int ctid = tid - 128;  // 0 .. 127
     const int sb_shift = cache.block_shift;
-    // eight codes of a token per thread and step: a warp reads 256 consecutive bytes and writes whole 128-byte rows of the
-    // swizzled stage, both without bank conflicts
-    constexpr int CPT = D / 8;            // 8-code chunks per token
+    // Sixteen codes of a token per thread and step: a quarter warp reads 128 consecutive bytes, and writes the two 16-byte
+    // halves of its 32 bytes in an order that keeps its eight stores on different banks.
+    constexpr int CPT = D / 16;           // 16-code chunks per token
     constexpr int TSTEP = 128 / CPT;      // tokens per step of the four warps
-    static_assert(kBN % (2 * TSTEP) == 0, "two tokens per step and thread");
+    static_assert(kBN % TSTEP == 0, "whole steps");
     const int ch = ctid % CPT, t0 = ctid / CPT;
+    const int half_first = D == 128 ? (ch >> 2) & 1 : 0;
+    const uint32_t c_first = (uint32_t)((2 * ch + half_first) & 7), c_second = c_first ^ 1u;
+    const bool coarse = PLAIN || sb_shift >= 3;    // one factor per 8 tokens is enough
     const float to_log2 = p.cap != 0.f ? p.inv_cap_scale : p.scale_log2;
     float v_norm = 1.f;
     int lo_min = -1, kv_end = 0;
@@ -616,46 +610,48 @@ q8_prefill_kernel(const Params p, const Q8Cache cache) {
         v_norm = __uint_as_float((254u + kVBits - e) << 23);
       }
       if (!mbar_wait(bar_kv_empty(st), ((gi / NS) & 1) ^ 1, abort_flag, wait_ns)) break;
-      if (ctid < kBN) {
-        const int key = pos + ctid;
-        reinterpret_cast<float*>(smem + C::OFF_KSCALE + st * (kBN * 4))[ctid] = key < kv_end ? ks_s[(key >> sb_shift) - e0] * to_log2 : 0.f;
+      // each token's factor on its logits; where blocks have 8 tokens or more, one per 8 tokens.  Never 0: masked logits are
+      // -inf, and their product with it has to stay that
+      if (ctid < (coarse ? kBN / 8 : kBN)) {
+        const int key = pos + (coarse ? ctid * 8 : ctid);
+        reinterpret_cast<float*>(smem + C::OFF_KSCALE + st * (kBN * 4))[ctid] = key < kv_end ? ks_s[(key >> sb_shift) - e0] * to_log2 : 1.f;
       }
       if (ctid == 0) {
         metas[st] = meta;
         vrefs[st] = v_norm;
       }
-      const uint8_t* raw = smem + C::OFF_RAW + rs * C::RAW_BYTES + ch * 8;
-      uint8_t* out = smem + C::OFF_KV + st * C::STAGE_BYTES + (ch >> 3) * 1024;
+      const uint8_t* raw = smem + C::OFF_RAW + rs * C::RAW_BYTES + ch * 16;
+      uint8_t* out = smem + C::OFF_KV + st * C::STAGE_BYTES + (ch >> 2) * 1024;
       // a short loop on purpose: the roles of this kernel share an instruction cache that their unrolled bodies overflow
-      // (all of a stage unrolled: 2.57 ms where this takes %UNROLL%)
 #pragma unroll 1
-      for (int t = t0; t < kBN; t += 2 * TSTEP) {
-        uint2 kc[2], vc[2];
-        float f[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          kc[i] = *reinterpret_cast<const uint2*>(raw + (t + i * TSTEP) * D);
-          vc[i] = *reinterpret_cast<const uint2*>(raw + (kBN + t + i * TSTEP) * D);
-          const int key = pos + t + i * TSTEP;
-          f[i] = vs_s[(key >> sb_shift) - e0] * v_norm;
-          if (key >= kv_end || key <= lo_min) {  // V of a key that no row sees is zero: those are stale bytes, possibly NaN
-            vc[i] = make_uint2(0u, 0u);
-            f[i] = 0.f;
-          }
+      for (int t = t0; t < kBN; t += TSTEP) {
+        const uint4 kc = *reinterpret_cast<const uint4*>(raw + t * D);
+        uint4 vc = *reinterpret_cast<const uint4*>(raw + (kBN + t) * D);
+        const int key = pos + t;
+        float f = vs_s[(key >> sb_shift) - e0] * v_norm;
+        if (key >= kv_end || key <= lo_min) {  // V of a key that no row sees is zero: those are stale bytes, possibly NaN
+          vc = make_uint4(0u, 0u, 0u, 0u);
+          f = 0.f;
         }
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int tt = t + i * TSTEP;
-          const uint32_t at = (uint32_t)(tt >> 3) * C::GROUP_BYTES + (uint32_t)(tt & 7) * 128 + (uint32_t)(((ch & 7) ^ (tt & 7)) << 4);
-          uint32_t w[4];
-          Code::widen(kc[i].x, w[0], w[1]);
-          Code::widen(kc[i].y, w[2], w[3]);
-          *reinterpret_cast<uint4*>(out + at) = make_uint4(from_f16x2<T>(w[0]), from_f16x2<T>(w[1]), from_f16x2<T>(w[2]), from_f16x2<T>(w[3]));
-          const __half2 f2 = __float2half2_rn(f[i]);
-          Code::widen(vc[i].x, w[0], w[1]);
-          Code::widen(vc[i].y, w[2], w[3]);
-          *reinterpret_cast<uint4*>(out + C::V_OFF + at) = make_uint4(mul_f16x2(w[0], f2), mul_f16x2(w[1], f2), mul_f16x2(w[2], f2), mul_f16x2(w[3], f2));
-        }
+        uint8_t* row = out + (uint32_t)(t >> 3) * C::GROUP_BYTES + (uint32_t)(t & 7) * 128;
+        uint8_t* at0 = row + ((c_first ^ (uint32_t)(t & 7)) << 4);
+        uint8_t* at1 = row + ((c_second ^ (uint32_t)(t & 7)) << 4);
+        const uint32_t k0 = half_first ? kc.z : kc.x, k1 = half_first ? kc.w : kc.y, k2 = half_first ? kc.x : kc.z, k3 = half_first ? kc.y : kc.w;
+        uint32_t w[4];
+        Code::widen(k0, w[0], w[1]);
+        Code::widen(k1, w[2], w[3]);
+        *reinterpret_cast<uint4*>(at0) = make_uint4(w[0], w[1], w[2], w[3]);
+        Code::widen(k2, w[0], w[1]);
+        Code::widen(k3, w[2], w[3]);
+        *reinterpret_cast<uint4*>(at1) = make_uint4(w[0], w[1], w[2], w[3]);
+        const __half2 f2 = __float2half2_rn(f);
+        const uint32_t v0 = half_first ? vc.z : vc.x, v1 = half_first ? vc.w : vc.y, v2 = half_first ? vc.x : vc.z, v3 = half_first ? vc.y : vc.w;
+        Code::widen(v0, w[0], w[1]);
+        Code::widen(v1, w[2], w[3]);
+        *reinterpret_cast<uint4*>(at0 + C::V_OFF) = make_uint4(mul_f16x2(w[0], f2), mul_f16x2(w[1], f2), mul_f16x2(w[2], f2), mul_f16x2(w[3], f2));
+        Code::widen(v2, w[0], w[1]);
+        Code::widen(v3, w[2], w[3]);
+        *reinterpret_cast<uint4*>(at1 + C::V_OFF) = make_uint4(mul_f16x2(w[0], f2), mul_f16x2(w[1], f2), mul_f16x2(w[2], f2), mul_f16x2(w[3], f2));
       }
       fence_async_smem();  // the MMAs read the stage through the async proxy
       __syncwarp();
@@ -672,6 +668,7 @@ q8_prefill_kernel(const Params p, const Q8Cache cache) {
     // warp may touch are fixed by warp % 4), so row maxima and sums need no shuffles.
     constexpr int HB = kBN;
     const int sw = warp - 8;
+    [[maybe_unused]] const bool coarse = PLAIN || cache.block_shift >= 3;
     const int x = sw / C::SM_WARPS;                       // which tile of the CTA
     const int row = (warp & 3) * 32 + lane;               // TMEM lane == row within the tile
     const uint32_t lane_addr = (uint32_t)((warp & 3) * 32) << 16;
@@ -683,25 +680,46 @@ q8_prefill_kernel(const Params p, const Q8Cache cache) {
     int k = 0;    // item counter (all roles see the same item sequence)
     int pc = 0;   // stages in which both tiles took part (the tiles take turns at the exponentials)
     bool alive = true;
-    // The query row of an item (K-major, 128B swizzle) goes from global to shared memory with cp.async,
-    // no registers in between, so that the row of the NEXT item can be fetched under the last stage of
-    // the current one: the tile's query buffer is free as soon as the item's last S has completed, and
-    // with the row in place the S issuer starts the next item while this thread is still in the epilogue.
-    const uint32_t q_row_smem = sb + C::OFF_Q + x * C::Q_BYTES + (uint32_t)row * 128;
-    auto q_issue = [&](const Unit& uu, int hh) {
+    // The query row of an item goes to shared memory as f16 (K-major, 128B swizzle); a bf16 row by a power of two that takes
+    // its largest element to [2^14, 2^15): exact for every element above 2^-28 of it, absolute error 2^-39 of it below.  The
+    // row of the NEXT item is fetched under the last stage of the current one: the tile's query buffer is free as soon as
+    // the item's last S has completed, and with the row in place the S issuer starts the next item while this thread is
+    // still in the epilogue.
+    uint8_t* q_row = smem + C::OFF_Q + x * C::Q_BYTES + (uint32_t)row * 128;
+    float q_fac = 1.f, q_fac_next = 1.f;  // 2^-k of the row
+    auto q_fetch = [&](const Unit& uu, int hh) {
       const int R = uu.row0 + x * kBM + row;
       const bool ok = R < uu.q_len * G;
       const int qt = R / G, g = R - qt * G;
-      const uint8_t* src = reinterpret_cast<const uint8_t*>(p.q);
-      if (ok) src += ((size_t)(uu.q_start + qt) * p.Hq + hh * G + g) * D * sizeof(T);
+      const uint4* src = reinterpret_cast<const uint4*>(p.q);
+      if (ok) src += ((size_t)(uu.q_start + qt) * p.Hq + hh * G + g) * (D / 8);
+      int e = 127 + 14;
+      if constexpr (!std::is_same<T, __half>::value) {
+        uint32_t big = 0;
+#pragma unroll 4
+        for (int c = 0; c < D / 8; ++c) {
+          const uint4 v = ok ? __ldg(src + c) : make_uint4(0u, 0u, 0u, 0u);
+          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-      for (int c = 0; c < D / 8; ++c)
-        cp_async16(q_row_smem + (uint32_t)(c >> 3) * (kBM * 128) + (uint32_t)(((c & 7) ^ (row & 7)) << 4),
-                   ok ? src + c * 16 : src, ok ? 16 : 0);  // rows past the item's end are zero-filled
-      cp_async_commit();
-    };
-    auto q_finish = [&]() {
-      cp_async_wait<0>();
+          for (int i = 0; i < 4; ++i) big = max(big, max((w[i] << 16) & 0x7fffffffu, w[i] & 0x7fff0000u));
+        }
+        e = (int)(big >> 23);  // biased exponent of the row's largest element
+        e = e == 255 ? 127 + 14 : (e < 20 ? 20 : e);  // infinities and NaN stay what they are; 2^k stays finite
+      }
+      const float up = __uint_as_float((uint32_t)(254 + 14 - e) << 23);
+#pragma unroll 4
+      for (int c = 0; c < D / 8; ++c) {  // rows past the item's end are zero
+        uint4 v = ok ? __ldg(src + c) : make_uint4(0u, 0u, 0u, 0u);
+        if constexpr (!std::is_same<T, __half>::value) {
+          uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            w[i] = Mma<__half>::pack(__uint_as_float(w[i] << 16) * up, __uint_as_float(w[i] & 0xffff0000u) * up);
+          v = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        *reinterpret_cast<uint4*>(q_row + (uint32_t)(c >> 3) * (kBM * 128) + (uint32_t)(((c & 7) ^ (row & 7)) << 4)) = v;
+      }
+      q_fac_next = __uint_as_float((uint32_t)(e - 14) << 23);
       fence_async_smem();  // the MMA reads the tile through the async proxy
       __syncwarp();
       if (lane == 0) mbar_arrive(bar_q_full(x));
@@ -762,10 +780,10 @@ q8_prefill_kernel(const Params p, const Q8Cache cache) {
       if (!q_ready) {
         // all S MMAs of this tile's previous item completed before its last s_full fired, which
         // this thread waited for, so the query tile may be overwritten
-        q_issue(u, h);
-        q_finish();
+        q_fetch(u, h);
       }
       q_ready = false;
+      q_fac = q_fac_next;
       for (int js = 0; js < n_stages; ++js, ++gi, ++ti) {
         const int st = gi % NS;
         const int pos = u.kv_begin + js * kBN;  // first key of the stage
@@ -784,39 +802,62 @@ q8_prefill_kernel(const Params p, const Q8Cache cache) {
         __syncwarp();
         if (lane == 0) mbar_arrive(bar_s_free(x));
 
-        // ---- logits in the log2 domain: the token's factor (k_scale * scale * log2 e), soft cap, masks
+        // ---- logits in the log2 domain: raw dot products times the token's factor (k_scale * scale * log2 e) and the row's.
+        // Common case: the products stay in the registers, a factor per 8 columns goes into the exponent's FMA and only the
+        // groups' maxima are multiplied; a soft cap, finer scales or a scale that is not positive materialise the logits.
         if (!mbar_wait(bar_kv_full(st), (gi / NS) & 1, abort_flag, wait_ns)) { alive = false; break; }  // long complete: orders the reads
         const float v_new = vrefs[st];
-        const float4* kf = reinterpret_cast<const float4*>(smem + C::OFF_KSCALE + st * (kBN * 4));
+        const float* kf = reinterpret_cast<const float*>(smem + C::OFF_KSCALE + st * (kBN * 4));
+        const float4* kf4 = reinterpret_cast<const float4*>(kf);
         const bool full_vis = (pos + HB - 1 <= pos_row) && (pos > lo_row);
-        float mx;
-        {
-          float ext[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        float ef[HB / 8];
 #pragma unroll
-          for (int i = 0; i < HB; i += 4) {
-            const float4 f = kf[i >> 2];
-            sr[i] = __float_as_uint(__uint_as_float(sr[i]) * f.x);
-            sr[i + 1] = __float_as_uint(__uint_as_float(sr[i + 1]) * f.y);
-            sr[i + 2] = __float_as_uint(__uint_as_float(sr[i + 2]) * f.z);
-            sr[i + 3] = __float_as_uint(__uint_as_float(sr[i + 3]) * f.w);
+        for (int i = 0; i < HB / 8; ++i) ef[i] = 1.f;
+        if constexpr (PLAIN) {
+#pragma unroll
+          for (int i = 0; i < HB / 8; i += 4) {
+            const float4 f = kf4[i >> 2];
+            // not below the smallest normal number: a masked logit, -inf, times 0 would be NaN
+            ef[i] = fmaxf(f.x * q_fac, 1.17549435e-38f);
+            ef[i + 1] = fmaxf(f.y * q_fac, 1.17549435e-38f);
+            ef[i + 2] = fmaxf(f.z * q_fac, 1.17549435e-38f);
+            ef[i + 3] = fmaxf(f.w * q_fac, 1.17549435e-38f);
           }
-          if (__builtin_expect(p.cap != 0.f, 0)) {
+        }
+        if constexpr (!PLAIN) {
+          if (coarse) {
+#pragma unroll
+            for (int i = 0; i < HB; ++i) sr[i] = __float_as_uint(__uint_as_float(sr[i]) * (kf[i >> 3] * q_fac));
+          } else {
+#pragma unroll
+            for (int i = 0; i < HB; i += 4) {
+              const float4 f = kf4[i >> 2];
+              sr[i] = __float_as_uint(__uint_as_float(sr[i]) * (f.x * q_fac));
+              sr[i + 1] = __float_as_uint(__uint_as_float(sr[i + 1]) * (f.y * q_fac));
+              sr[i + 2] = __float_as_uint(__uint_as_float(sr[i + 2]) * (f.z * q_fac));
+              sr[i + 3] = __float_as_uint(__uint_as_float(sr[i + 3]) * (f.w * q_fac));
+            }
+          }
+          if (p.cap != 0.f) {
 #pragma unroll
             for (int i = 0; i < HB; ++i) sr[i] = __float_as_uint(p.cap_log2 * soft_cap_tanh(__uint_as_float(sr[i])));
           }
-          if (__builtin_expect(!full_vis, 0)) {
-            const int hi_i = pos_row - pos;  // last visible column of the stage
-            const int lo_i = lo_row - pos;   // columns up to here are left of the window
+        }
+        if (__builtin_expect(!full_vis, 0)) {
+          const int hi_i = pos_row - pos;  // last visible column of the stage
+          const int lo_i = lo_row - pos;   // columns up to here are left of the window
 #pragma unroll
-            for (int i = 0; i < HB; ++i)
-              if (i > hi_i || i <= lo_i) sr[i] = __float_as_uint(-INFINITY);
-          }
+          for (int i = 0; i < HB; ++i)
+            if (i > hi_i || i <= lo_i) sr[i] = __float_as_uint(-INFINITY);
+        }
+        float mx = -INFINITY;
 #pragma unroll
-          for (int i = 0; i < HB; i += 8)
-#pragma unroll
-            for (int a = 0; a < 4; ++a)
-              ext[a] = fmax3(ext[a], __uint_as_float(sr[i + 2 * a]), __uint_as_float(sr[i + 2 * a + 1]));
-          mx = fmaxf(fmaxf(ext[0], ext[1]), fmaxf(ext[2], ext[3]));
+        for (int i = 0; i < HB; i += 8) {
+          float a = fmaxf(__uint_as_float(sr[i]), __uint_as_float(sr[i + 1]));
+          float b = fmaxf(__uint_as_float(sr[i + 2]), __uint_as_float(sr[i + 3]));
+          a = fmax3(a, __uint_as_float(sr[i + 4]), __uint_as_float(sr[i + 5]));
+          b = fmax3(b, __uint_as_float(sr[i + 6]), __uint_as_float(sr[i + 7]));
+          mx = fmaxf(mx, fmaxf(a, b) * ef[i >> 3]);
         }
         // P_x has two buffers: this stage's goes where the stage before the previous one's was, whose
         // P.V must have read it (it has, normally long ago)
@@ -868,8 +909,8 @@ q8_prefill_kernel(const Params p, const Q8Cache cache) {
           uint32_t pk[16];
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
-            const float p0 = fast_exp2(__uint_as_float(sr[c + 2 * j]) - m_use);
-            const float p1 = fast_exp2(__uint_as_float(sr[c + 2 * j + 1]) - m_use);
+            const float p0 = fast_exp2(fmaf(__uint_as_float(sr[c + 2 * j]), ef[(c + 2 * j) >> 3], -m_use));
+            const float p1 = fast_exp2(fmaf(__uint_as_float(sr[c + 2 * j + 1]), ef[(c + 2 * j) >> 3], -m_use));
             lsum4[j & 3] += p0 + p1;
             pk[j] = Mma<__half>::pack(p0, p1);
           }
@@ -887,24 +928,22 @@ q8_prefill_kernel(const Params p, const Q8Cache cache) {
         if (lane == 0) mbar_arrive(bar_p_full(x, ti & 1));
 
         if (pos + kBN >= u.kv_end) {
-          // ---- last stage of the piece.  All S of the item completed long ago, so the tile's query
-          // buffer is free: fetch the next item's query row (if the producer has published that item
-          // already; it normally has, it runs stages ahead) under the wait for the last P.V ...
+          // ---- last stage of the piece.  All S of the item completed long ago, so the tile's query buffer is free: fetch
+          // the next item's query row (if the producer has published that item already; it normally has, it runs stages
+          // ahead), then wait for the last P.V, normalise and store, or (a part of a split item) publish the unnormalised
+          // part and, if it is the last to arrive, combine ----
           bool q_pending = *items_pub > k;
           q_pending = __all_sync(0xffffffffu, q_pending);
           if (q_pending) {
             __threadfence_block();
             const Unit un = ring[k % kRingP].u;
             q_pending = un.seq >= 0 && (x == 0 || un.q_len * G > un.row0 + kBM);
-            if (q_pending) q_issue(un, ring[k % kRingP].h);
+            if (q_pending) {
+              q_fetch(un, ring[k % kRingP].h);
+              q_ready = true;
+            }
           }
-          // ---- ... wait for the P.V, then normalise and store, or (a part of a split item) publish the
-          // unnormalised part and, if it is the last to arrive, combine ----
           if (!mbar_wait(bar_pv_done(x, ti & 1), (ti >> 1) & 1, abort_flag, wait_ns)) { alive = false; break; }
-          if (q_pending) {  // the next item's first S runs while this one's epilogue does
-            q_finish();
-            q_ready = true;
-          }
           tc_fence_after();
           const float v_back = power_of_two_inverse(v_norm);  // O is in units of v_ref
           if (u.n_chunks > 1) {
@@ -1035,7 +1074,6 @@ q8_prefill_kernel(const Params p, const Q8Cache cache) {
       }
     }
   }
-  cp_async_wait<0>();  // a query row fetched ahead when a wait ran out
   if (*abort_flag) flags |= EJK_RPA_ST_TIMEOUT;
   // every role has left its loop (all waits are bounded), so the TMEM can go back
   tc_fence_before();
@@ -1047,10 +1085,10 @@ q8_prefill_kernel(const Params p, const Q8Cache cache) {
   if (flags && p.status) atomicOr(reinterpret_cast<unsigned*>(p.status), flags);
 }
 
-template <typename T, typename Code, int D>
+template <typename T, typename Code, int D, bool PLAIN>
 cudaError_t launch_one(const Params& p, const Q8Cache& c, int n_sm, cudaStream_t stream, bool pdl) {
   using C = CfgP<D>;
-  auto kern = q8_prefill_kernel<T, Code, D>;
+  auto kern = q8_prefill_kernel<T, Code, D, PLAIN>;
   static std::atomic<bool> configured[64];
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -1070,9 +1108,10 @@ cudaError_t launch_one(const Params& p, const Q8Cache& c, int n_sm, cudaStream_t
 
 template <typename T, typename Code>
 cudaError_t dispatch(const Params& p, const Q8Cache& c, int n_sm, cudaStream_t stream, bool pdl) {
+  const bool plain = c.block_shift >= 3 && p.cap == 0.f && p.scale_log2 > 0.f;
   switch (p.D) {
-    case 64: return launch_one<T, Code, 64>(p, c, n_sm, stream, pdl);
-    case 128: return launch_one<T, Code, 128>(p, c, n_sm, stream, pdl);
+    case 64: return plain ? launch_one<T, Code, 64, true>(p, c, n_sm, stream, pdl) : launch_one<T, Code, 64, false>(p, c, n_sm, stream, pdl);
+    case 128: return plain ? launch_one<T, Code, 128, true>(p, c, n_sm, stream, pdl) : launch_one<T, Code, 128, false>(p, c, n_sm, stream, pdl);
   }
   return cudaErrorInvalidValue;
 }
