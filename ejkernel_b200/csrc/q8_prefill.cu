@@ -122,6 +122,27 @@ template <int N>
 __device__ __forceinline__ void take_registers() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(N));
 }
+// two float32 in one instruction
+__device__ __forceinline__ uint64_t pack_f32x2(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};\n" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 unpack_f32x2(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;\n" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 __device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, __half2 b) {
   const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), b);
   return *reinterpret_cast<const uint32_t*>(&r);
@@ -179,7 +200,7 @@ q8_prefill_kernel(const Params p, const Q8Cache cache) {
       mbar_init(bar_raw_empty(s), C::CV_WARPS);
     }
     for (int x = 0; x < NT; ++x) {
-      mbar_init(bar_s_full(x), 1);
+      mbar_init(bar_s_full(x), 2);  // the commit, and the issuer's own arrival: it has seen the stage (see there)
       mbar_init(bar_s_free(x), C::SM_WARPS);  // one arrival per softmax warp
       for (int b = 0; b < 2; ++b) {
         mbar_init(bar_p_full(x, b), C::SM_WARPS);
@@ -537,6 +558,9 @@ q8_prefill_kernel(const Params p, const Q8Cache cache) {
           if (first && !mbar_wait_thread(bar_q_full(x), (items - 1) & 1, abort_flag, wait_ns)) break;
           if (t > 0 && !mbar_wait_thread(bar_s_free(x), (t - 1) & 1, abort_flag, wait_ns)) break;
           tc_fence_after();
+          // the softmax warps read the stage's factors after waiting for S alone: this arrival, after the wait for the
+          // stage, orders those reads behind the converters' writes
+          mbar_arrive(bar_s_full(x));
           const uint64_t kd = k_desc0 + (uint64_t)((st * C::STAGE_BYTES) >> 4);
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
@@ -805,7 +829,6 @@ q8_prefill_kernel(const Params p, const Q8Cache cache) {
         // ---- logits in the log2 domain: raw dot products times the token's factor (k_scale * scale * log2 e) and the row's.
         // Common case: the products stay in the registers, a factor per 8 columns goes into the exponent's FMA and only the
         // groups' maxima are multiplied; a soft cap, finer scales or a scale that is not positive materialise the logits.
-        if (!mbar_wait(bar_kv_full(st), (gi / NS) & 1, abort_flag, wait_ns)) { alive = false; break; }  // long complete: orders the reads
         const float v_new = vrefs[st];
         const float* kf = reinterpret_cast<const float*>(smem + C::OFF_KSCALE + st * (kBN * 4));
         const float4* kf4 = reinterpret_cast<const float4*>(kf);
@@ -903,20 +926,25 @@ q8_prefill_kernel(const Params p, const Q8Cache cache) {
         }
         const float m_use = (m_run == -INFINITY) ? 0.f : m_run;
         // probabilities, packed as 16-bit pairs, into the tile's P buffer of this stage
-        float lsum4[4] = {0.f, 0.f, 0.f, 0.f};
+        // (pairs of columns in one instruction where there is one: this loop's length bounds the kernel)
+        const uint64_t neg_m = pack_f32x2(-m_use, -m_use);
+        uint64_t lsum[2] = {0ull, 0ull};
 #pragma unroll
         for (int c = 0; c < HB; c += 32) {
           uint32_t pk[16];
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
-            const float p0 = fast_exp2(fmaf(__uint_as_float(sr[c + 2 * j]), ef[(c + 2 * j) >> 3], -m_use));
-            const float p1 = fast_exp2(fmaf(__uint_as_float(sr[c + 2 * j + 1]), ef[(c + 2 * j) >> 3], -m_use));
-            lsum4[j & 3] += p0 + p1;
+            const float f = ef[(c + 2 * j) >> 3];
+            const uint64_t y = fma_f32x2(pack_f32x2(__uint_as_float(sr[c + 2 * j]), __uint_as_float(sr[c + 2 * j + 1])), pack_f32x2(f, f), neg_m);
+            const float2 e = unpack_f32x2(y);
+            const float p0 = fast_exp2(e.x), p1 = fast_exp2(e.y);
+            lsum[j & 1] = add_f32x2(lsum[j & 1], pack_f32x2(p0, p1));
             pk[j] = Mma<__half>::pack(p0, p1);
           }
           tc_st16(tm_p + (c >> 1), pk);
         }
-        l_run += (lsum4[0] + lsum4[1]) + (lsum4[2] + lsum4[3]);
+        const float2 lsum_pair = unpack_f32x2(add_f32x2(lsum[0], lsum[1]));
+        l_run += lsum_pair.x + lsum_pair.y;
         if (two) {
           __syncwarp();
           if (lane == 0) mbar_arrive(bar_turn(x));
