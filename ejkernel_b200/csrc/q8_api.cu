@@ -149,6 +149,7 @@ int ejk_q8_attention_launch(const void* queries, const void* kv_pages, const flo
   p.max_punits = L.max_punits;
   p.target_units = L.target_units;
   p.target_units_max = L.target_units_max;
+  p.even_units = 2 * n_sm / s.num_kv_heads;
   p.min_chunk = opt.min_chunk;
   if (a.num_kv_pages_per_block > 0) {  // per-call hint: the smallest KV chunk, in pages
     long long chunk = (long long)a.num_kv_pages_per_block * s.page_size;

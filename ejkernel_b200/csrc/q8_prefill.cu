@@ -2,8 +2,10 @@
 //
 //     S[128 x 64] = Q[128 x D] . Kc^T,   P = 2^(S * k_scale * scale * log2 e - m),   O += P . (Vc * v_scale / v_ref)
 //
-// The tiles, barriers, turns, KV split and epilogue are those of rpa_prefill_sm100.cu (two 128-row tiles per CTA, 64-token
-// stages, S and P.V issued by single threads, one softmax thread per row).  What the codes add is a pipeline in front:
+// The tiles, barriers, KV split and epilogue are those of rpa_prefill_sm100.cu (two 128-row tiles per CTA, 64-token
+// stages, S and P.V issued by single threads, one softmax thread per row).  (The turns that the tiles of
+// that kernel take at the exponentials cost more than they give here: 1.49 ms with, 1.39 without, 4 x 2048 rows over 8192 keys.)
+// What the codes add is a pipeline in front:
 //
 //   producer warp --raw stage (codes: bulk copies; scales: 4-byte cp.async)--> four converter warps --16-bit stage--> MMAs
 //
@@ -86,8 +88,8 @@ struct CfgP {
   static constexpr int OFF_VREF = OFF_META + NS * 8;                 // per 16-bit stage: 1 / v_ref
   static constexpr int OFF_BAR = (OFF_VREF + NS * 4 + 7) / 8 * 8;
   // barriers: kv_full[NS] kv_empty[NS] raw_full[NR] raw_empty[NR], then per tile: s_full s_free p_full[2] pv_done[2]
-  // q_full o_free turn
-  static constexpr int BAR_PER_TILE = 9;
+  // q_full o_free
+  static constexpr int BAR_PER_TILE = 8;
   static constexpr int N_BAR = 2 * NS + 2 * NR + NT * BAR_PER_TILE;
   static constexpr int OFF_TMEM = OFF_BAR + N_BAR * 8;
   // abort flag, the published-items counter, per tile the count of items its softmax warps have skipped
@@ -181,7 +183,6 @@ q8_prefill_kernel(const Params p, const Q8Cache cache) {
   auto bar_pv_done = [&](int x, int b) { return tile_bar(x, 4 + b); };  // P_x.V(t) complete (commit): buffer t&1 is free
   auto bar_q_full = [&](int x) { return tile_bar(x, 6); };
   auto bar_o_free = [&](int x) { return tile_bar(x, 7); };
-  auto bar_turn = [&](int x) { return tile_bar(x, 8); };      // tile x has issued the exponentials of a stage
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int Hkv = p.Hkv, G = p.G;
@@ -209,7 +210,6 @@ q8_prefill_kernel(const Params p, const Q8Cache cache) {
       mbar_init(bar_q_full(x), C::SM_WARPS);
       mbar_init(bar_o_free(x), C::SM_WARPS);
       skipped[x] = 0;
-      mbar_init(bar_turn(x), C::SM_WARPS);
     }
     *abort_flag = 0;
     *items_pub = 0;
@@ -702,7 +702,6 @@ q8_prefill_kernel(const Params p, const Q8Cache cache) {
     int gi = 0;   // KV stage counter (all roles see the same stage sequence)
     int ti = 0;   // stages this tile took part in
     int k = 0;    // item counter (all roles see the same item sequence)
-    int pc = 0;   // stages in which both tiles took part (the tiles take turns at the exponentials)
     bool alive = true;
     // The query row of an item goes to shared memory as f16 (K-major, 128B swizzle); a bf16 row by a power of two that takes
     // its largest element to [2^14, 2^15): exact for every element above 2^-28 of it, absolute error 2^-39 of it below.  The
@@ -915,15 +914,6 @@ q8_prefill_kernel(const Params p, const Q8Cache cache) {
             }
           }
         }
-        // The MUFU unit gives 4 exponentials per cycle and scheduler, and both tiles' warps sit on the
-        // same schedulers: when both tiles are at work they take turns at the exponentials (tile 0
-        // first), so that one tile's waits and TMEM traffic overlap the other's MUFU phase instead of
-        // both phases running in lockstep at half speed.
-        if (two) {
-          const bool my_turn_ok = (x == 0) ? (pc == 0 || mbar_wait(bar_turn(1), (pc - 1) & 1, abort_flag, wait_ns))
-                                           : mbar_wait(bar_turn(0), pc & 1, abort_flag, wait_ns);
-          if (!my_turn_ok) { alive = false; break; }
-        }
         const float m_use = (m_run == -INFINITY) ? 0.f : m_run;
         // probabilities, packed as 16-bit pairs, into the tile's P buffer of this stage
         // (pairs of columns in one instruction where there is one: this loop's length bounds the kernel)
@@ -945,11 +935,6 @@ q8_prefill_kernel(const Params p, const Q8Cache cache) {
         }
         const float2 lsum_pair = unpack_f32x2(add_f32x2(lsum[0], lsum[1]));
         l_run += lsum_pair.x + lsum_pair.y;
-        if (two) {
-          __syncwarp();
-          if (lane == 0) mbar_arrive(bar_turn(x));
-          ++pc;
-        }
         tc_wait_st();
         tc_fence_before();
         __syncwarp();
