@@ -44,14 +44,34 @@ _MAX_STREAMS = 16
 _checked = jaxtyping.jaxtyped(typechecker=beartype)
 
 
-def _describe(t):
-    return (t.shape, t.dtype, t.stride(), t.device) if isinstance(t, torch.Tensor) else t
+_capturing = torch._C._cuda_isCurrentStreamCapturing
+_raw_stream = torch._C._cuda_getCurrentRawStream  # the current stream's handle, without a Stream object around it
+_current_device = torch._C._cuda_getDevice
+
+
+class _on:
+    """``torch.cuda.device`` that costs nothing on the device that is current already."""
+
+    __slots__ = ("index", "back")
+
+    def __init__(self, index: int):
+        self.index = index
+
+    def __enter__(self):
+        self.back = _current_device()
+        if self.back != self.index:
+            torch.cuda.set_device(self.index)
+
+    def __exit__(self, *_):
+        if self.back != self.index:
+            torch.cuda.set_device(self.back)
 
 
 def _remember(key, plan):
-    if len(_plans) >= _MAX_REMEMBERED:
-        _plans.clear()
-    _plans[key] = plan
+    if key is not None:
+        if len(_plans) >= _MAX_REMEMBERED:
+            _plans.clear()
+        _plans[key] = plan
     return plan
 
 
@@ -91,14 +111,15 @@ def _check_cache(kv_pages, kv_scales) -> int:
 
 
 def _status_word(device: torch.device):
+    """Address of the device's status word, or None."""
     word = _status.get(device.index)
     if word is None:
-        if torch.cuda.is_current_stream_capturing():
+        if _capturing():
             return None  # a word made here would be the graph's, and zeroed by every replay
         word = torch.zeros(1, dtype=torch.int32, device=device)
         torch.cuda.current_stream(device).synchronize()  # once: other streams may use it from now on
         _status[device.index] = word
-    return word
+    return word.data_ptr()
 
 
 def read_status(device: torch.device | str | int | None = None, clear: bool = True) -> int:
@@ -116,27 +137,34 @@ def read_status(device: torch.device | str | int | None = None, clear: bool = Tr
     return value
 
 
-def _after(status, what: str) -> None:
+def _after(device: torch.device, what: str) -> None:
     """Opt-in (``EJKERNEL_B200_CHECK_STATUS=1``): read the status word after the call and raise when an output is invalid."""
-    if status is None or os.environ.get("EJKERNEL_B200_CHECK_STATUS", "0") in ("", "0"):
+    if os.environ.get("EJKERNEL_B200_CHECK_STATUS", "0") in ("", "0") or device.index not in _status or _capturing():
         return
-    word = int(status.item())
+    word = int(_status[device.index].item())
     if word & (_cabi.ST_TIMEOUT | _cabi.ST_INTERNAL):
-        status.zero_()
+        _status[device.index].zero_()
         raise _cabi.RpaLibraryError(f"{what}: status word {word:#x}: " + "; ".join(_cabi.decode_status(word)))
 
 
 def _workspace(nbytes: int, device: torch.device, stream: int) -> torch.Tensor:
-    if torch.cuda.is_current_stream_capturing():
+    if _capturing():
         return torch.empty(nbytes, dtype=torch.uint8, device=device)
     key = (device.index, stream)
     ws = _scratch.pop(key, None)
-    if ws is None or ws.numel() < nbytes:
+    if ws is None or ws.shape[0] < nbytes:
         ws = torch.empty(1 << max(16, (nbytes - 1).bit_length()), dtype=torch.uint8, device=device)
     _scratch[key] = ws  # the most recently used stands last
     if len(_scratch) > _MAX_STREAMS:
         del _scratch[next(iter(_scratch))]
     return ws
+
+
+def _count(num_seqs, device: torch.device) -> torch.Tensor:
+    """The number of sequences as an int32 on the device."""
+    if isinstance(num_seqs, torch.Tensor) and num_seqs.dtype is torch.int32 and num_seqs.device == device and num_seqs.numel() == 1:
+        return num_seqs
+    return _num_seqs_tensor(num_seqs, device)
 
 
 # ---------------------------------------------------------------------------------------- attention
@@ -200,7 +228,7 @@ def _plan_attention(
             nbytes = int(_cabi.load().ejk_q8_workspace_bytes(ctypes.byref(shape)))
         if nbytes == 0:
             raise ValueError("ejk_q8_workspace_bytes rejected the shape")
-    return shape, attrs, nbytes
+    return shape, attrs, nbytes, ctypes.byref(shape), ctypes.byref(attrs)
 
 
 @serving_registry.register("quantized_ragged_page_attention", Platform.CUDA, Backend.GPU)
@@ -225,34 +253,42 @@ def quantized_ragged_page_attention(
     Products run on the codes as 16-bit floats (exact) and accumulate in float32; ``softmax_scale`` defaults to
     ``head_dim ** -0.5``.  Returns a tensor of the shape and dtype of ``queries``.
     """
-    key = ("attention", _describe(queries), _describe(kv_pages), _describe(kv_scales), _describe(context_lens),
-           _describe(block_tables), _describe(query_start_loc), _describe(softmax_aux), softmax_scale, logits_soft_cap,
-           sliding_window, num_kv_pages_per_block, num_queries_per_block, _cabi.get_option_cached("waves"))
-    plan = _plans.get(key)
+    try:
+        key = (queries.shape, queries.dtype, queries.is_contiguous(), queries.get_device(),
+               kv_pages.shape, kv_pages.dtype, kv_pages.is_contiguous(), kv_pages.get_device(),
+               kv_scales.shape, kv_scales.dtype, kv_scales.is_contiguous(), kv_scales.get_device(),
+               context_lens.shape, context_lens.dtype, context_lens.is_contiguous(), context_lens.get_device(),
+               block_tables.shape, block_tables.dtype, block_tables.is_contiguous(), block_tables.get_device(),
+               query_start_loc.shape, query_start_loc.dtype, query_start_loc.is_contiguous(), query_start_loc.get_device(),
+               None if softmax_aux is None else (softmax_aux.shape, softmax_aux.dtype, softmax_aux.get_device()),
+               softmax_scale, logits_soft_cap, sliding_window, num_kv_pages_per_block, num_queries_per_block,
+               _cabi.get_option_cached("waves"))
+        plan = _plans.get(key)
+    except (AttributeError, TypeError):  # not tensors, not hashable: the full check says what is wrong
+        key = plan = None
     if plan is None:
-        plan = _remember(key, _plan_attention(queries, kv_pages, kv_scales, context_lens, block_tables, query_start_loc, softmax_aux,
-                                              softmax_scale, logits_soft_cap, sliding_window, num_kv_pages_per_block,
-                                              num_queries_per_block))
-    shape, attrs, nbytes = plan
+        plan = _plan_attention(queries, kv_pages, kv_scales, context_lens, block_tables, query_start_loc, softmax_aux,
+                               softmax_scale, logits_soft_cap, sliding_window, num_kv_pages_per_block, num_queries_per_block)
+        _remember(key, plan)
+    shape, attrs, nbytes, shape_ref, attrs_ref = plan
     out = torch.empty_like(queries)  # every row is written: sequences by their tiles, the rest zero-filled
     if shape.total_tokens == 0:
         return out
     device = queries.device
-    aux = None
-    if softmax_aux is not None and attrs.num_sinks:
-        aux = softmax_aux.to(torch.float32).contiguous()
-    if not (isinstance(num_seqs, torch.Tensor) and num_seqs.dtype is torch.int32 and num_seqs.device == device and num_seqs.numel() == 1):
-        num_seqs = _num_seqs_tensor(num_seqs, device)
-    with torch.cuda.device(device):
-        stream = torch.cuda.current_stream(device).cuda_stream
+    with _on(device.index):
+        aux = None
+        if softmax_aux is not None and attrs.num_sinks:
+            aux = softmax_aux.to(torch.float32).contiguous()
+        num_seqs = _count(num_seqs, device)
+        stream = _raw_stream(device.index)
         ws = _workspace(nbytes, device, stream)
-        status = _status_word(device)
         rc = _cabi.load().ejk_q8_attention_launch(
             queries.data_ptr(), kv_pages.data_ptr(), kv_scales.data_ptr(), context_lens.data_ptr(), block_tables.data_ptr(),
             query_start_loc.data_ptr(), num_seqs.data_ptr(), None if aux is None else aux.data_ptr(), out.data_ptr(),
-            ws.data_ptr(), nbytes, None if status is None else status.data_ptr(), ctypes.byref(shape), ctypes.byref(attrs), stream)
-        _cabi.check(rc, "ejk_q8_attention_launch")
-        _after(status, "quantized_ragged_page_attention")
+            ws.data_ptr(), nbytes, _status_word(device), shape_ref, attrs_ref, stream)
+        if rc:
+            _cabi.check(rc, "ejk_q8_attention_launch")
+        _after(device, "quantized_ragged_page_attention")
     return out
 
 
@@ -285,7 +321,7 @@ def _plan_write(
     _need_cuda("quantized_kv_write", keys)
     P, _, _, page_size, _ = kv_pages.shape
     shape = _cabi.Q8Shape(T, 1, 1, P, page_size, Hkv, Hkv, D, _DTYPE_CODE[keys.dtype], CODE_DTYPES[kv_pages.dtype], block)
-    return shape, strides[0], strides[1]
+    return shape, ctypes.byref(shape), strides[0], strides[1]
 
 
 @serving_registry.register("quantized_kv_write", Platform.CUDA, Backend.GPU)
@@ -304,21 +340,26 @@ def quantized_kv_write(
     move to it (exactly for e4m3 above its subnormal range, by rounding once more otherwise).  ``read_status`` reports
     NaN and infinities among the rows.
     """
-    key = ("write", _describe(keys), _describe(values), _describe(kv_pages), _describe(kv_scales), _describe(slot_mapping))
-    plan = _plans.get(key)
+    try:
+        key = (keys.shape, keys.dtype, keys.stride(), keys.get_device(), values.shape, values.dtype, values.stride(), values.get_device(),
+               kv_pages.shape, kv_pages.dtype, kv_pages.is_contiguous(), kv_pages.get_device(),
+               kv_scales.shape, kv_scales.dtype, kv_scales.is_contiguous(), kv_scales.get_device(),
+               slot_mapping.shape, slot_mapping.dtype, slot_mapping.is_contiguous(), slot_mapping.get_device(), "write")
+        plan = _plans.get(key)
+    except (AttributeError, TypeError):
+        key = plan = None
     if plan is None:
         plan = _remember(key, _plan_write(keys, values, kv_pages, kv_scales, slot_mapping))
-    shape, key_stride, value_stride = plan
+    shape, shape_ref, key_stride, value_stride = plan
     if shape.total_tokens == 0:
         return kv_pages, kv_scales
     device = keys.device
-    with torch.cuda.device(device):
-        status = _status_word(device)
+    with _on(device.index):
         rc = _cabi.load().ejk_q8_write_launch(
             keys.data_ptr(), values.data_ptr(), key_stride, value_stride, kv_pages.data_ptr(), kv_scales.data_ptr(),
-            slot_mapping.data_ptr(), None if status is None else status.data_ptr(), ctypes.byref(shape),
-            torch.cuda.current_stream(device).cuda_stream)
-    _cabi.check(rc, "ejk_q8_write_launch")
+            slot_mapping.data_ptr(), _status_word(device), shape_ref, _raw_stream(device.index))
+        if rc:
+            _cabi.check(rc, "ejk_q8_write_launch")
     return kv_pages, kv_scales
 
 
@@ -339,7 +380,8 @@ def _plan_read(
     _need_cuda("quantized_kv_read", kv_pages)
     P, Hkv, _, page_size, D = kv_pages.shape
     rows = slot_mapping.shape[0]
-    return _cabi.Q8Shape(rows, 1, 1, P, page_size, Hkv, Hkv, D, _DTYPE_CODE[dtype], CODE_DTYPES[kv_pages.dtype], block)
+    shape = _cabi.Q8Shape(rows, 1, 1, P, page_size, Hkv, Hkv, D, _DTYPE_CODE[dtype], CODE_DTYPES[kv_pages.dtype], block)
+    return shape, ctypes.byref(shape), (2, rows, Hkv, D)
 
 
 @serving_registry.register("quantized_kv_read", Platform.CUDA, Backend.GPU)
@@ -354,21 +396,25 @@ def quantized_kv_read(
 
     A value beyond the range of ``dtype`` saturates; a negative slot gives a row of zeros.
     """
-    key = ("read", _describe(kv_pages), _describe(kv_scales), _describe(slot_mapping), dtype)
-    shape = _plans.get(key)
-    if shape is None:
-        shape = _remember(key, _plan_read(kv_pages, kv_scales, slot_mapping, dtype))
+    try:
+        key = (kv_pages.shape, kv_pages.dtype, kv_pages.is_contiguous(), kv_pages.get_device(),
+               kv_scales.shape, kv_scales.dtype, kv_scales.is_contiguous(), kv_scales.get_device(),
+               slot_mapping.shape, slot_mapping.dtype, slot_mapping.is_contiguous(), slot_mapping.get_device(), dtype, "read")
+        plan = _plans.get(key)
+    except (AttributeError, TypeError):
+        key = plan = None
+    if plan is None:
+        plan = _remember(key, _plan_read(kv_pages, kv_scales, slot_mapping, dtype))
+    shape, shape_ref, out_shape = plan
     device = kv_pages.device
-    out = torch.empty((2, shape.total_tokens, shape.num_kv_heads, shape.head_dim), dtype=dtype, device=device)
-    keys, values = out[0], out[1]
-    if shape.total_tokens == 0:
-        return keys, values
-    with torch.cuda.device(device):
-        status = _status_word(device)
-        rc = _cabi.load().ejk_q8_read_launch(
-            kv_pages.data_ptr(), kv_scales.data_ptr(), slot_mapping.data_ptr(), keys.data_ptr(), values.data_ptr(),
-            None if status is None else status.data_ptr(), ctypes.byref(shape), torch.cuda.current_stream(device).cuda_stream)
-    _cabi.check(rc, "ejk_q8_read_launch")
+    with _on(device.index):
+        keys, values = torch.empty(out_shape, dtype=dtype, device=device).unbind(0)
+        if shape.total_tokens:
+            rc = _cabi.load().ejk_q8_read_launch(
+                kv_pages.data_ptr(), kv_scales.data_ptr(), slot_mapping.data_ptr(), keys.data_ptr(), values.data_ptr(),
+                _status_word(device), shape_ref, _raw_stream(device.index))
+            if rc:
+                _cabi.check(rc, "ejk_q8_read_launch")
     return keys, values
 
 
@@ -398,7 +444,7 @@ def _plan_tables(
     _on_one_device("block_tables", block_tables.device, query_lens=query_lens, context_lens=context_lens,
                    free_pages=free_pages, num_free=num_free, finished=finished)
     _need_cuda("build_page_tables", block_tables)
-    return S, pps, free_pages.shape[0]
+    return S, pps, free_pages.shape[0], 2 * S + 2 + total_tokens, (S, S + 1, total_tokens, 1)
 
 
 @serving_registry.register("build_page_tables", Platform.CUDA, Backend.GPU)
@@ -425,27 +471,31 @@ def build_page_tables(
     out, the row's table is too short, the batch exceeds ``total_tokens``): such a row keeps its length and takes no page,
     and ``read_status`` says so.  Nothing is read back by the host, so the call can be captured into a graph.
     """
-    key = ("tables", _describe(query_lens), _describe(context_lens), _describe(block_tables), _describe(free_pages),
-           _describe(num_free), _describe(finished), page_size, total_tokens)
-    plan = _plans.get(key)
+    try:
+        key = (query_lens.shape, query_lens.dtype, query_lens.is_contiguous(), query_lens.get_device(),
+               context_lens.shape, context_lens.dtype, context_lens.is_contiguous(), context_lens.get_device(),
+               block_tables.shape, block_tables.dtype, block_tables.is_contiguous(), block_tables.get_device(),
+               free_pages.shape, free_pages.dtype, free_pages.is_contiguous(), free_pages.get_device(),
+               num_free.shape, num_free.dtype, num_free.get_device(),
+               None if finished is None else (finished.shape, finished.dtype, finished.is_contiguous(), finished.get_device()),
+               page_size, total_tokens, "tables")
+        plan = _plans.get(key)
+    except (AttributeError, TypeError):
+        key = plan = None
     if plan is None:
         plan = _remember(key, _plan_tables(query_lens, context_lens, block_tables, free_pages, num_free, finished, page_size, total_tokens))
-    S, pps, capacity = plan
+    S, pps, capacity, total, sizes = plan
     device = block_tables.device
-    if not (isinstance(num_seqs, torch.Tensor) and num_seqs.dtype is torch.int32 and num_seqs.device == device and num_seqs.numel() == 1):
-        num_seqs = _num_seqs_tensor(num_seqs, device)
-    # one allocation for the four results, each on a 16-byte boundary
-    n_lens, n_start, n_slots = -(-S // 4) * 4, -(-(S + 1) // 4) * 4, -(-total_tokens // 4) * 4
-    out = torch.empty(n_lens + n_start + n_slots + 1, dtype=torch.int32, device=device)
-    lens, start = out[:S], out[n_lens: n_lens + S + 1]
-    slots, left = out[n_lens + n_start: n_lens + n_start + total_tokens], out[n_lens + n_start + n_slots:]
-    with torch.cuda.device(device):
-        status = _status_word(device)
+    with _on(device.index):
+        num_seqs = _count(num_seqs, device)
+        out = torch.empty(total, dtype=torch.int32, device=device)  # one allocation for the four results
+        base = out.data_ptr()
+        at_slots = base + 4 * (2 * S + 1)
         rc = _cabi.load().ejk_page_tables_launch(
             query_lens.data_ptr(), context_lens.data_ptr(), block_tables.data_ptr(), free_pages.data_ptr(),
-            num_free.data_ptr(), num_seqs.data_ptr(), None if finished is None else finished.data_ptr(), lens.data_ptr(),
-            start.data_ptr(), slots.data_ptr() if total_tokens else None, left.data_ptr(),
-            None if status is None else status.data_ptr(), S, pps, page_size, capacity, total_tokens,
-            torch.cuda.current_stream(device).cuda_stream)
-    _cabi.check(rc, "ejk_page_tables_launch")
-    return lens, start, slots, left
+            num_free.data_ptr(), num_seqs.data_ptr(), None if finished is None else finished.data_ptr(), base, base + 4 * S,
+            at_slots if total_tokens else None, at_slots + 4 * total_tokens, _status_word(device), S, pps, page_size, capacity,
+            total_tokens, _raw_stream(device.index))
+        if rc:
+            _cabi.check(rc, "ejk_page_tables_launch")
+    return out.split_with_sizes(sizes)

@@ -25,6 +25,16 @@ Array = torch.Tensor
 PlatformName = Literal["triton", "pallas", "cuda", "xla", "auto"]
 
 
+def _impl(name: str, platform):
+    return serving_registry.get(name, platform=_resolve_platform(platform), backend=Backend.GPU)
+
+
+# the registry is asked once for the usual case
+_attention, _write, _read, _tables = (
+    _impl(name, None) for name in ("quantized_ragged_page_attention", "quantized_kv_write", "quantized_kv_read", "build_page_tables")
+)
+
+
 def allocate_quantized_kv(
     num_pages: int,
     num_kv_heads: int,
@@ -63,7 +73,7 @@ def build_page_tables(
     platform: PlatformName | None = None,
 ) -> tuple[Array, Array, Array, Array]:
     """``(context_lens, query_start_loc, slot_mapping, num_free)`` of this step; tables and free list in place."""
-    impl = serving_registry.get("build_page_tables", platform=_resolve_platform(platform), backend=Backend.GPU)
+    impl = _tables if platform is None else _impl("build_page_tables", platform)
     return impl(query_lens, context_lens, block_tables, free_pages, num_free, num_seqs, page_size=page_size,
                 total_tokens=total_tokens, finished=finished)
 
@@ -72,7 +82,7 @@ def quantized_kv_write(
     keys: Array, values: Array, kv_pages: Array, kv_scales: Array, slot_mapping: Array, /, *, platform: PlatformName | None = None
 ) -> tuple[Array, Array]:
     """Write a step's rows to the cache in place; returns ``(kv_pages, kv_scales)``."""
-    impl = serving_registry.get("quantized_kv_write", platform=_resolve_platform(platform), backend=Backend.GPU)
+    impl = _write if platform is None else _impl("quantized_kv_write", platform)
     return impl(keys, values, kv_pages, kv_scales, slot_mapping)
 
 
@@ -86,7 +96,7 @@ def quantized_kv_read(
     platform: PlatformName | None = None,
 ) -> tuple[Array, Array]:
     """``(keys, values)`` of the cache's rows at ``slot_mapping``, in 16 bits."""
-    impl = serving_registry.get("quantized_kv_read", platform=_resolve_platform(platform), backend=Backend.GPU)
+    impl = _read if platform is None else _impl("quantized_kv_read", platform)
     return impl(kv_pages, kv_scales, slot_mapping, dtype=dtype)
 
 
@@ -111,7 +121,7 @@ def quantized_ragged_page_attention(
     out_specs: PartitionSpec | None = None,
 ) -> Array:
     """Mixed decode / chunked-prefill attention over the 8-bit cache."""
-    impl = serving_registry.get("quantized_ragged_page_attention", platform=_resolve_platform(platform), backend=Backend.GPU)
+    impl = _attention if platform is None else _impl("quantized_ragged_page_attention", platform)
     out = impl(
         queries, kv_pages, kv_scales, context_lens, block_tables, query_start_loc, num_seqs,
         softmax_scale=softmax_scale, logits_soft_cap=logits_soft_cap, sliding_window=sliding_window, softmax_aux=softmax_aux,
