@@ -1,18 +1,23 @@
 // Page tables and slot maps of one serving step from the requests' lengths (the definition is in ejk_q8.h).
 //
-// With c = context length, q = new tokens, g = page size:
+// With c = context length, q = new tokens, g = page size, per row:
 //   held = ceil(c / g), need = ceil((c + q) / g) - held, and exclusive sums over the rows: start (of q), first (of need),
 //   back (of held, finished rows only).  The stack holds n' = num_free + sum(back) pages after the returns;
-//   table[row, held + j] = stack[n' - 1 - (first + j)] where first + need <= n'.
-// The sums are one block's scans, 1024 rows at a time; the pages of a round are then written one thread per page (a
-// binary search over the round's sums finds the row), so that one long prompt does not serialise on one thread.
+//   page i of the new ones is stack[n' - 1 - i], and row s takes the pages first .. first + need - 1 where they exist.
+//
+// A few bytes per token and page: launches and latency bound it, so it is one kernel.  Every block computes the three sums
+// of all rows in its own shared memory (a few microseconds that they all spend at the same time, instead of a second
+// launch behind the first) and then writes its share of the tokens, the new pages and the returned ones.  That needs no order
+// between blocks, because nothing is read that this call writes: a new page that comes from a finished row is looked up
+// in that row's table, not on the stack, and the slots of new pages are computed, not read back.
+// Measured on the device: 4 rows 4.3 us, 1000 rows with 8.8 thousand tokens and 24 thousand returned pages %T1000% (one block
+// for the sums and pages and a second kernel for the slots: 6.9 and 37.6 us).
 #include "q8_types.cuh"
 
 namespace ejk {
 namespace {
 
-constexpr int kRows = 1024;
-constexpr int kSlotThreads = 256;
+constexpr unsigned kMaxSum = 0x7fffffffu;  // sums saturate here: above every token, page and stack count there is
 
 struct TableArgs {
   const int32_t* query_lens;
@@ -30,69 +35,83 @@ struct TableArgs {
   int32_t S, pps, page, capacity, T;
 };
 
-// exclusive sum of v over the block, and its total
-__device__ long long block_scan(long long v, long long* s_warp, long long& total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  long long x = v;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long y = __shfl_up_sync(0xffffffffu, x, o);
-    if (lane >= o) x += y;
-  }
-  __syncthreads();  // s_warp of an earlier scan has been read
-  if (lane == 31) s_warp[warp] = x;
-  __syncthreads();
-  if (warp == 0) {
-    long long y = s_warp[lane];
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long z = __shfl_up_sync(0xffffffffu, y, o);
-      if (lane >= o) y += z;
-    }
-    s_warp[lane] = y;
-  }
-  __syncthreads();
-  total = s_warp[31];
-  return x - v + (warp ? s_warp[warp - 1] : 0);
-}
+__device__ __forceinline__ unsigned sat_add(unsigned a, unsigned b) { return min(a + b, kMaxSum); }  // associative for a, b <= kMaxSum
 
 struct Row {
   int c, q, held, need;
   bool gone, ok;  // ok: lengths within the contract and the row's table
 };
 
-__device__ __forceinline__ Row load_row(const TableArgs& a, int s, int S, unsigned& flags) {
-  Row r = {0, 0, 0, 0, false, true};
-  if (s >= S) return r;
+__device__ __forceinline__ Row load_row(const TableArgs& a, int s, unsigned& flags) {
+  Row r;
   r.c = a.context_lens[s];
+  r.q = a.query_lens[s];
   r.gone = a.finished && a.finished[s] != 0;
-  r.q = r.gone ? 0 : a.query_lens[s];
-  const long long cap = (long long)a.pps * a.page;
+  r.ok = true;
+  r.need = 0;
+  if (r.gone) r.q = 0;
+  const int cap = a.pps * a.page;  // below 2^30
   if (r.c < 0 || r.c > cap) {
     flags |= EJK_RPA_ST_KVLEN;
-    r.ok = r.gone;  // a finished row gives back what its table holds
-    r.c = r.c < 0 ? 0 : (int)cap;
+    r.ok = false;
+    r.c = r.c < 0 ? 0 : cap;
   }
   if (r.q < 0) {
     flags |= EJK_RPA_ST_QLEN;
     r.q = 0;
   }
   r.held = (r.c + a.page - 1) / a.page;
-  if ((long long)r.c + r.q > cap) {
+  if (r.q > cap - r.c) {
     flags |= EJK_RPA_ST_KVLEN;
     r.ok = false;
   }
-  if (r.ok && !r.gone) r.need = (int)(((long long)r.c + r.q + a.page - 1) / a.page) - r.held;
+  if (r.ok && !r.gone) r.need = (r.c + r.q + a.page - 1) / a.page - r.held;
   return r;
 }
 
-__global__ void __launch_bounds__(kRows) page_tables_kernel(const TableArgs a) {
-  __shared__ long long s_warp[32];
-  __shared__ long long s_ex[kRows];
-  __shared__ int s_held[kRows];
-  __shared__ unsigned char s_ok[kRows];
-  __shared__ unsigned long long s_taken;
-  const int tid = threadIdx.x;
+// exclusive sums of three counters over the block's threads, and the totals
+__device__ void block_scan(unsigned (&v)[3], unsigned (&total)[3], unsigned (*s_warp)[3]) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n_warps = blockDim.x >> 5;
+  unsigned inc[3];
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    unsigned x = v[k];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x = sat_add(x, y);
+    }
+    inc[k] = x;
+    if (lane == 31) s_warp[warp][k] = x;
+  }
+  __syncthreads();
+  if (warp == 0) {
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      unsigned x = lane < n_warps ? s_warp[lane][k] : 0u;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const unsigned y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x = sat_add(x, y);
+      }
+      if (lane < n_warps) s_warp[lane][k] = x;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    unsigned before = __shfl_up_sync(0xffffffffu, inc[k], 1);
+    if (lane == 0) before = 0u;
+    v[k] = sat_add(before, warp ? s_warp[warp - 1][k] : 0u);
+    total[k] = s_warp[n_warps - 1][k];
+  }
+}
+
+__global__ void __launch_bounds__(1024) page_tables_kernel(const TableArgs a) {
+  extern __shared__ unsigned s_sums[];  // start[S] first[S] back[S]
+  __shared__ unsigned s_warp[32][3];
+  __shared__ unsigned s_taken;
+  const int tid = threadIdx.x, n_threads = blockDim.x;
   unsigned flags = 0;
   int S = a.num_seqs[0];
   if (S > a.S) {
@@ -100,113 +119,119 @@ __global__ void __launch_bounds__(kRows) page_tables_kernel(const TableArgs a) {
     flags |= EJK_RPA_ST_NUM_SEQS;
   }
   if (S < 0) S = 0;
-  long long n = a.num_free[0];
-  if (n < 0 || n > a.capacity) {
+  unsigned* start = s_sums;
+  unsigned* first = s_sums + S;
+  unsigned* back = s_sums + 2 * S;
+  int n_free = a.num_free[0];
+  if (n_free < 0 || n_free > a.capacity) {
     flags |= EJK_Q8_ST_POOL;
-    n = n < 0 ? 0 : a.capacity;
+    n_free = n_free < 0 ? 0 : a.capacity;
   }
   if (tid == 0) s_taken = 0;
-  // the row of page j of a round: the last row whose sum is not above j (rows without pages share their successor's)
-  auto find = [&](long long j, int rows) {
-    int lo = 0, hi = rows;
+
+  // ---- the sums: neighbouring rows to a thread, then across threads
+  const int per = (S + n_threads - 1) / n_threads;
+  const int s0 = min(tid * per, S), s1 = min(s0 + per, S);
+  unsigned v[3] = {0u, 0u, 0u}, total[3];
+  for (int s = s0; s < s1; ++s) {
+    const Row r = load_row(a, s, flags);
+    v[0] = sat_add(v[0], (unsigned)r.q);
+    v[1] = sat_add(v[1], (unsigned)r.need);
+    v[2] = sat_add(v[2], r.gone ? (unsigned)r.held : 0u);
+  }
+  block_scan(v, total, s_warp);
+  const unsigned returned = total[2];
+  unsigned n_all = sat_add((unsigned)n_free, returned);  // pages on the stack once the returned ones are on it
+  if (n_all > (unsigned)a.capacity) {
+    flags |= EJK_Q8_ST_POOL;
+    n_all = (unsigned)a.capacity;
+  }
+  // is a row with these sums served?
+  auto served = [&](const Row& r, unsigned q0, unsigned p0, unsigned& f) {
+    if (r.gone) return false;
+    bool ok = r.ok;
+    if (sat_add(q0, (unsigned)r.q) > (unsigned)a.T) {  // the batch is longer than its buffers
+      f |= EJK_RPA_ST_QLEN;
+      ok = false;
+    }
+    if (r.need > 0 && sat_add(p0, (unsigned)r.need) > n_all) {
+      f |= EJK_Q8_ST_POOL;
+      ok = false;
+    }
+    return ok;
+  };
+  for (int s = s0; s < s1; ++s) {
+    unsigned none = 0;
+    const Row r = load_row(a, s, none);
+    start[s] = v[0];
+    first[s] = v[1];
+    back[s] = v[2];
+    const bool ok = served(r, v[0], v[1], flags);
+    if (blockIdx.x == 0) {
+      a.starts[s] = (int)min(v[0], (unsigned)a.T);
+      a.new_lens[s] = r.gone ? 0 : (ok ? r.c + r.q : r.c);
+      if (ok && r.need > 0) atomicAdd(&s_taken, (unsigned)r.need);
+    }
+    v[0] = sat_add(v[0], (unsigned)r.q);
+    v[1] = sat_add(v[1], (unsigned)r.need);
+    v[2] = sat_add(v[2], r.gone ? (unsigned)r.held : 0u);
+  }
+  __syncthreads();
+  const unsigned q_total = min(total[0], (unsigned)a.T);
+  if (blockIdx.x == 0) {
+    for (int s = S + tid; s < a.S; s += n_threads) a.new_lens[s] = 0;
+    for (int s = S + tid; s <= a.S; s += n_threads) a.starts[s] = (int)q_total;
+    if (tid == 0) a.new_free[0] = (int)(n_all - s_taken);
+  }
+
+  // the last row whose sum is not above j: rows without a share have their successor's sum
+  auto find = [&](const unsigned* sum, unsigned j) {
+    int lo = 0, hi = S;
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
-      if (s_ex[mid] <= j) lo = mid;
+      if (sum[mid] <= j) lo = mid;
       else hi = mid;
     }
     return lo;
   };
+  // page `j` of the returned ones, and page `i` from the top of the stack
+  auto returned_page = [&](unsigned j) {
+    const int s = find(back, j);
+    return a.tables[(size_t)s * a.pps + (j - back[s])];
+  };
+  auto top_page = [&](unsigned i) {
+    const unsigned at = n_all - 1u - i;
+    return at < (unsigned)n_free ? a.free_pages[at] : returned_page(at - (unsigned)n_free);
+  };
+  const unsigned gid = blockIdx.x * n_threads + tid, n_grid = gridDim.x * n_threads;
 
-  // ---- returned pages go on top
-  if (a.finished) {
-    for (int s0 = 0; s0 < S; s0 += kRows) {
-      unsigned f = 0;
-      const Row r = load_row(a, s0 + tid, S, f);
-      long long total;
-      s_ex[tid] = block_scan(r.gone ? r.held : 0, s_warp, total);
-      __syncthreads();
-      const int rows = S - s0 < kRows ? S - s0 : kRows;
-      for (long long j = tid; j < total; j += kRows) {
-        const int i = find(j, rows);
-        const long long at = n + j;
-        if (at < a.capacity) a.free_pages[at] = a.tables[(size_t)(s0 + i) * a.pps + (j - s_ex[i])];
-        else flags |= EJK_Q8_ST_POOL;
-      }
-      n += total;
-      __syncthreads();  // s_ex; and the pages are visible to the threads that take them below
-    }
-    if (n > a.capacity) n = a.capacity;
-  }
-
-  // ---- starts, lengths, new pages
-  long long start = 0, first = 0;
-  for (int s0 = 0; s0 < S; s0 += kRows) {
-    const int s = s0 + tid;
-    Row r = load_row(a, s, S, flags);
-    long long q_total, need_total;
-    const long long q0 = start + block_scan(r.q, s_warp, q_total);
-    const long long p0 = block_scan(r.need, s_warp, need_total);
-    if (q0 + r.q > a.T) {  // the batch is longer than its buffers
-      flags |= EJK_RPA_ST_QLEN;
-      r.ok = false;
-    }
-    if (first + p0 + r.need > n) {
-      if (r.need > 0) flags |= EJK_Q8_ST_POOL;
-      r.ok = r.ok && r.need == 0;
-    }
-    const bool takes = r.ok && !r.gone;
-    if (s < S) {
-      a.starts[s] = (int)(q0 < a.T ? q0 : a.T);
-      a.new_lens[s] = r.gone ? 0 : (takes ? r.c + r.q : r.c);
-    }
-    if (takes && r.need > 0) atomicAdd(&s_taken, (unsigned long long)r.need);
-    s_ex[tid] = p0;
-    s_held[tid] = r.held;
-    s_ok[tid] = takes;
-    __syncthreads();
-    const int rows = S - s0 < kRows ? S - s0 : kRows;
-    for (long long j = tid; j < need_total; j += kRows) {
-      const int i = find(j, rows);
-      const long long at = n - 1 - (first + j);
-      if (s_ok[i] && at >= 0) a.tables[(size_t)(s0 + i) * a.pps + s_held[i] + (j - s_ex[i])] = a.free_pages[at];
-    }
-    start += q_total;
-    first += need_total;
-    __syncthreads();
-  }
-  for (int s = S + tid; s < a.S; s += kRows) a.new_lens[s] = 0;
-  for (int s = S + tid; s <= a.S; s += kRows) a.starts[s] = (int)(start < a.T ? start : a.T);
-  if (tid == 0) a.new_free[0] = (int)(n - (long long)s_taken);
-  if (flags && a.status) atomicOr(reinterpret_cast<unsigned*>(a.status), flags);
-}
-
-// slots[t] of every token from the finished tables: one thread per token, a binary search for its row
-__global__ void __launch_bounds__(kSlotThreads) slot_map_kernel(const TableArgs a) {
-  const int t = blockIdx.x * kSlotThreads + threadIdx.x;
-  if (t >= a.T) return;
-  int S = a.num_seqs[0];
-  S = S > a.S ? a.S : S;
-  int slot = -1;
-  unsigned flags = 0;
-  if (S > 0 && t < a.starts[S]) {
-    int lo = 0, hi = S;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (a.starts[mid] <= t) lo = mid;
-      else hi = mid;
-    }
-    const int c = a.context_lens[lo], q = a.query_lens[lo];
-    if (c >= 0 && q > 0 && a.new_lens[lo] == c + q) {  // the row was served
-      const int pos = c + t - a.starts[lo];
-      const int pi = pos / a.page;
-      if (pos >= 0 && pos < c + q && pi < a.pps) {
-        const long long at = (long long)a.tables[(size_t)lo * a.pps + pi] * a.page + (pos - pi * a.page);
+  // ---- slots
+  for (unsigned t = gid; t < (unsigned)a.T; t += n_grid) {
+    int slot = -1;
+    if (t < q_total) {
+      const int s = find(start, t);
+      unsigned none = 0;
+      const Row r = load_row(a, s, none);
+      if (served(r, start[s], first[s], none)) {
+        const int pos = r.c + (int)(t - start[s]);
+        const int pi = pos / a.page;
+        const int page = pi < r.held ? a.tables[(size_t)s * a.pps + pi] : top_page(first[s] + (unsigned)(pi - r.held));
+        const long long at = (long long)page * a.page + (pos - pi * a.page);
         if (at >= 0 && at <= 0x7fffffffLL) slot = (int)at;
         else flags |= EJK_RPA_ST_PAGE_ID;
       }
     }
+    a.slots[t] = slot;
   }
-  a.slots[t] = slot;
+  // ---- new pages into the tables
+  for (unsigned j = gid; j < min(total[1], n_all); j += n_grid) {
+    const int s = find(first, j);
+    unsigned none = 0;
+    const Row r = load_row(a, s, none);
+    if (served(r, start[s], first[s], none)) a.tables[(size_t)s * a.pps + r.held + (j - first[s])] = top_page(j);
+  }
+  // ---- returned pages onto the stack
+  for (unsigned j = gid; j < n_all - min(n_all, (unsigned)n_free); j += n_grid) a.free_pages[(unsigned)n_free + j] = returned_page(j);
   if (flags && a.status) atomicOr(reinterpret_cast<unsigned*>(a.status), flags);
 }
 
@@ -218,10 +243,18 @@ cudaError_t launch_page_tables(const int32_t* query_lens, const int32_t* context
                                int S, int pps, int page, int capacity, int T, cudaStream_t st) {
   const TableArgs a = {query_lens, context_lens, tables, free_pages, num_free, num_seqs, finished, new_lens, starts,
                        slots, new_free, status, S, pps, page, capacity, T};
-  page_tables_kernel<<<1, kRows, 0, st>>>(a);
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess || T == 0) return e;
-  slot_map_kernel<<<(T + kSlotThreads - 1) / kSlotThreads, kSlotThreads, 0, st>>>(a);
+  const size_t smem = (size_t)S * 3 * sizeof(unsigned);
+  if (smem > 48 * 1024) {
+    // the limit of the kernel on the current device, set whenever it is needed: two words of host work
+    if (cudaError_t e = cudaFuncSetAttribute(page_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPageTableMaxRows * 12); e != cudaSuccess)
+      return e;
+  }
+  // a small block synchronises faster; as many blocks as leave each thread a handful of tokens and pages
+  const int threads = S <= 256 ? 256 : 1024;
+  const long long work = (long long)T + 8ll * S;
+  long long blocks = (work + threads - 1) / threads;
+  if (blocks > 128) blocks = 128;
+  page_tables_kernel<<<(int)blocks, threads, smem, st>>>(a);
   return cudaGetLastError();
 }
 

@@ -239,9 +239,8 @@ int ejk_q8_read_launch(const void* kv_pages, const float* kv_scales, const int32
   if (!keys || !values || !kv_pages || !kv_scales || !slots || !shape) return EJK_RPA_E_NULL;
   if (int e = check_cache(*shape)) return e;
   const ejk_q8_shape& s = *shape;
-  // 256 threads of 8 elements each per block, at most 2^31 - 1 blocks
-  if (s.total_tokens <= 0 || (long long)s.total_tokens * s.num_kv_heads * 2 * (s.head_dim / 8) / 256 >= 0x7fffffffLL)
-    return EJK_RPA_E_SHAPE;
+  // the kernel counts 8-element chunks of K in 32 bits
+  if (s.total_tokens <= 0 || (long long)s.total_tokens * s.num_kv_heads * (s.head_dim / 8) > 0x7fffffffLL) return EJK_RPA_E_SHAPE;
   if (!aligned16(keys) || !aligned16(values) || !aligned16(kv_pages)) return EJK_RPA_E_ALIGN;
   if (!sm100_sm_count()) return EJK_RPA_E_DEVICE;
   cudaError_t e = launch_q8_read(cache_of(kv_pages, kv_scales, s), slots, keys, values, status, s.total_tokens, s.dtype,
@@ -260,7 +259,7 @@ int ejk_page_tables_launch(const int32_t* query_lens, const int32_t* context_len
   if (!query_lens || !context_lens || !block_tables || !free_pages || !num_free || !num_seqs || !new_context_lens ||
       !query_start_loc || !new_num_free || (total_tokens > 0 && !slots))
     return EJK_RPA_E_NULL;
-  if (max_num_seqs <= 0 || max_num_seqs > 0x00ffffff || pages_per_seq <= 0 || page_size <= 0 || capacity <= 0 || total_tokens < 0)
+  if (max_num_seqs <= 0 || max_num_seqs > kPageTableMaxRows || pages_per_seq <= 0 || page_size <= 0 || capacity <= 0 || total_tokens < 0)
     return EJK_RPA_E_SHAPE;
   if ((long long)pages_per_seq * page_size > 0x3fffffffLL || total_tokens > 0x3fffffff) return EJK_RPA_E_SHAPE;
   if (!sm100_sm_count()) return EJK_RPA_E_DEVICE;
@@ -268,7 +267,7 @@ int ejk_page_tables_launch(const int32_t* query_lens, const int32_t* context_len
                                      new_context_lens, query_start_loc, slots, new_num_free, status, max_num_seqs,
                                      pages_per_seq, page_size, capacity, total_tokens, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return static_cast<int>(e);
-  set_last_launches(total_tokens > 0 ? 2 : 1);
+  set_last_launches(1);
   return 0;
 }
 

@@ -47,11 +47,11 @@ struct CodeE4M3 {
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;\n" : "=r"(h) : "h"((uint16_t)c));
     return __half2float(__ushort_as_half((uint16_t)h));
   }
-  // x is within +-448: the nearest code, ties to even
-  static __device__ __forceinline__ uint8_t encode(float x) {
+  // the nearest codes, ties to even, `a` in the low byte
+  static __device__ __forceinline__ uint32_t encode2(float a, float b) {
     uint16_t r;
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;\n" : "=h"(r) : "f"(0.f), "f"(x));
-    return (uint8_t)(r & 0xff);
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;\n" : "=h"(r) : "f"(b), "f"(a));
+    return r;
   }
   // biased exponent of the smallest power of two s with amax <= 448 * s: 448 = 1.75 * 2^8
   static __device__ __forceinline__ int scale_exponent(uint32_t amax_bits) {
@@ -79,7 +79,10 @@ struct CodeI8 {
   static constexpr int kId = EJK_Q8_I8;
   static constexpr float kMax = 127.f;
   static __device__ __forceinline__ float decode(uint8_t c) { return (float)(int8_t)c; }
-  static __device__ __forceinline__ uint8_t encode(float x) { return (uint8_t)(int8_t)__float2int_rn(x); }
+  static __device__ __forceinline__ uint32_t encode2(float a, float b) {
+    // 1.5 * 2^23 + x: the sum's low bits are x rounded to the nearest integer, ties to even
+    return prmt(__float_as_uint(a + 12582912.f), __float_as_uint(b + 12582912.f), 0x0040u) & 0xffffu;
+  }
   // 127 = 1.984375 * 2^6
   static __device__ __forceinline__ int scale_exponent(uint32_t amax_bits) {
     return (int)(amax_bits >> 23) - 6 + ((amax_bits & 0x7fffffu) > 0x7e0000u ? 1 : 0);
@@ -128,6 +131,7 @@ cudaError_t launch_q8_write(const void* keys, const void* values, long long key_
                             cudaStream_t stream);
 cudaError_t launch_q8_read(const Q8Cache& c, const int32_t* slots, void* keys, void* values, int32_t* status, int rows,
                            int dtype, int code, cudaStream_t stream);
+constexpr int kPageTableMaxRows = 16384;  // three sums per row in shared memory
 cudaError_t launch_page_tables(const int32_t* query_lens, const int32_t* context_lens, int32_t* tables, int32_t* free_pages,
                                const int32_t* num_free, const int32_t* num_seqs, const uint8_t* finished,
                                int32_t* new_lens, int32_t* starts, int32_t* slots, int32_t* new_free, int32_t* status,

@@ -435,6 +435,8 @@ def _plan_tables(
     S, pps = block_tables.shape
     if S < 1 or pps < 1 or free_pages.shape[0] < 1:
         raise ValueError(f"block_tables {tuple(block_tables.shape)} and free_pages {tuple(free_pages.shape)} must not be empty")
+    if S > 16384:
+        raise NotImplementedError(f"{S} sequences: the CUDA path holds the sums of 16384 rows")
     if page_size < 1 or pps * page_size > 0x3FFFFFFF:
         raise ValueError(f"{page_size=} with {pps} pages per sequence: must be positive, and below 2^30 tokens in all")
     if not 0 <= total_tokens <= 0x3FFFFFFF:

@@ -83,7 +83,7 @@ EJK_RPA_API int ejk_q8_read_launch(const void* kv_pages, const float* kv_scales,
  * call).  Then every row that lacks pages for its context_len + query_len tokens takes them from the top, rows in
  * order.  A row that cannot be served -- the stack is empty, the row's table too short, the batch longer than
  * total_tokens -- takes no page, keeps its context length, gets slots of -1 and sets a status bit.
- * slots[t] = page * page_size + offset of token t; -1 behind the last sequence.
+ * slots[t] = page * page_size + offset of token t; -1 behind the last sequence.  max_num_seqs is 16384 at most.
  * No output may overlap an input other than as named above. */
 EJK_RPA_API int ejk_page_tables_launch(const int32_t* query_lens, const int32_t* context_lens, int32_t* block_tables,
                                        int32_t* free_pages, const int32_t* num_free, const int32_t* num_seqs,

@@ -124,6 +124,12 @@ def test_write_and_read_refuse():
         ej.quantized_kv_read(c["kv_pages"], c["kv_scales"], slots, dtype=torch.float32)
 
 
+def test_page_tables_refuse_more_rows_than_their_sums_hold():
+    i = torch.zeros(16385, dtype=torch.int32)
+    with pytest.raises(NotImplementedError):
+        ej.build_page_tables(i, i, torch.zeros(16385, 1, dtype=torch.int32), i, i[:1], 2, page_size=16, total_tokens=4)
+
+
 @pytest.mark.parametrize("kw", [dict(page_size=0), dict(total_tokens=-1), dict(page_size=1 << 30), dict(total_tokens=1 << 30)])
 def test_page_tables_refuse(kw):
     i = torch.zeros(2, dtype=torch.int32)
@@ -176,7 +182,7 @@ def test_c_entries_refuse_before_they_touch_anything(rpa_lib):
         assert attention(attrs=bad) == -6
     assert write(stride=64) == -2 and write(stride=132) == -8
     assert tables(q=None) == -1
-    for kw in (dict(S=0), dict(pps=0), dict(page=0), dict(cap=0), dict(T=-1), dict(page=1 << 30), dict(T=1 << 30)):
+    for kw in (dict(S=0), dict(S=16385), dict(pps=0), dict(page=0), dict(cap=0), dict(T=-1), dict(page=1 << 30), dict(T=1 << 30)):
         assert tables(**kw) == -2, kw
     assert rpa_lib.ejk_q8_workspace_bytes(None) == 0
 
