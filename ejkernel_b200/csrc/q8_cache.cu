@@ -273,10 +273,10 @@ cudaError_t write_dispatch(const void* keys, const void* values, long long ks, l
                            const int32_t* slots, int32_t* status, int rows, cudaStream_t st) {
   const T* k = static_cast<const T*>(keys);
   const T* v = static_cast<const T*>(values);
-  // rows that a CTA looks through: up to 512 rows one each, then what keeps about as many windows (12 thousand rows in blocks of
+  // rows that a CTA looks through: up to 1024 rows one each, then what keeps about as many windows (12 thousand rows in blocks of
   // 32, 75 MB: %WINDOW%)
   int window = 1;
-  while (window < 32 && window < (1 << c.block_shift) && rows / window > 512) window *= 2;
+  while (window < 32 && window < (1 << c.block_shift) && rows / window > 1024) window *= 2;
   const dim3 grid((rows + window - 1) / window, (2 * c.Hkv + kWriteThreads / 32 - 1) / (kWriteThreads / 32));
   switch (c.D) {
     case 64: q8_write_kernel<T, Code, 64><<<grid, kWriteThreads, 0, st>>>(k, v, ks, vs, c, slots, status, rows, window); break;

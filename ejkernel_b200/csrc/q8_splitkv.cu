@@ -102,10 +102,6 @@ template <>
 __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) {
   return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
 }
-template <>
-__device__ __forceinline__ float2 unpack2<__half>(uint32_t w) {
-  return __half22float2(*reinterpret_cast<const __half2*>(&w));
-}
 
 template <typename T, typename Code, int D, int NT, int NS>
 __global__ void __launch_bounds__(kThreads, (Cfg<D, NT, NS>::CTAS))
@@ -165,26 +161,6 @@ q8_splitkv_kernel(const __grid_constant__ CUtensorMap tmap, const Params p, cons
     int wid = 0;
     if (lane == 0) wid = atomicAdd(&p.header[kHdrQueue], 1);
     wid = __shfl_sync(0xffffffffu, wid, 0);
-    // page id of a key of a sequence; one that is out of range is reported and read as page 0
-    auto split_key = [&](int key, int& off) {
-      int pi;
-      if (p.page_shift >= 0) {
-        pi = key >> p.page_shift;
-        off = key & (p.page_size - 1);
-      } else {
-        pi = key / p.page_size;
-        off = key - pi * p.page_size;
-      }
-      return pi;
-    };
-    auto page_of = [&](const int32_t* tab, int pi) {
-      int page = __ldg(tab + pi);
-      if ((unsigned)page >= (unsigned)p.num_pages) {
-        flags |= EJK_RPA_ST_PAGE_ID;
-        page = 0;
-      }
-      return page;
-    };
     bool alive = true;
     while (alive) {
       if (wid >= n_work) {
@@ -212,14 +188,32 @@ q8_splitkv_kernel(const __grid_constant__ CUtensorMap tmap, const Params p, cons
       int wid_next = 0;
       if (lane == 0) wid_next = atomicAdd(&p.header[kHdrQueue], 1);  // consumed only at the next item
       const int32_t* tab = p.block_tables + (size_t)u.seq * p.pages_per_seq;
+      // page of the block of tokens that this lane fetches; read a stage ahead, so that its latency lies under the stage before
+      auto page_of = [&](int pos, int& off) {
+        const int key = pos + (lane << pb_shift);
+        int pi;
+        if (p.page_shift >= 0) {
+          pi = key >> p.page_shift;
+          off = key & (p.page_size - 1);
+        } else {
+          pi = key / p.page_size;
+          off = key - pi * p.page_size;
+        }
+        return lane < blocks_per_stage && key < u.kv_end ? __ldg(tab + pi) : 0;
+      };
+      int off_next = 0, page_next = page_of(u.kv_begin, off_next);
       bool first = true;
       for (int pos = u.kv_begin; first || pos < u.kv_end; pos += TK) {
         int nblk = (u.kv_end - pos + pb - 1) >> pb_shift;
         if (nblk > blocks_per_stage) nblk = blocks_per_stage;
         if (nblk < 0) nblk = 0;
-        // this lane's page, fetched before the wait so that its latency is hidden
-        int page = 0, off = 0;
-        if (lane < nblk) page = page_of(tab, split_key(pos + (lane << pb_shift), off));
+        int page = page_next;
+        const int off = off_next;
+        page_next = page_of(pos + TK, off_next);
+        if ((unsigned)page >= (unsigned)p.num_pages) {  // reported, and read as page 0
+          flags |= EJK_RPA_ST_PAGE_ID;
+          page = 0;
+        }
         if (!mbar_wait(bar_empty + s * 8, empty_parity, abort_flag, wait_ns)) {
           alive = false;
           break;
@@ -232,18 +226,21 @@ q8_splitkv_kernel(const __grid_constant__ CUtensorMap tmap, const Params p, cons
             asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;\n" ::"r"(full), "r"((uint32_t)nblk * box_bytes) : "memory");
           __syncwarp();
           if (lane < nblk) tma_load_5d(smem_base + s * C::STAGE_BYTES + lane * box_bytes, &tmap, full, 0, off, 0, 2 * h, page);
-          // scales of the blocks that the stage's keys lie in: K's, then V's
+          // scales of the blocks that the stage's keys lie in: K's, then V's.  Block e starts at key (e0 + e) << sb_shift, or
+          // at the stage's first key; the lane that fetches that key's tokens knows its page
           const int e0 = pos >> sb_shift;
           const int last = (u.kv_end < pos + TK ? u.kv_end : pos + TK) - 1;
           const int n_e = last >= pos ? (last >> sb_shift) - e0 + 1 : 0;
           const uint32_t sdst = smem_base + C::OFF_SCALE + s * (2 * TK * 4);
-          for (int e = lane; e < n_e; e += 32) {
-            int eoff;
-            const int key = (e0 + e) << sb_shift;
-            const int pi = split_key(key > pos ? key : pos, eoff);
-            const long long at = (((long long)page_of(tab, pi) * Hkv + h) * 2) * scales_per_page + (eoff >> sb_shift);
-            cp_async4(sdst + e * 4, cache.scales + at);
-            cp_async4(sdst + (TK + e) * 4, cache.scales + at + scales_per_page);
+          for (int e = lane; e - lane < n_e; e += 32) {
+            const int from = max(((e0 + e) << sb_shift) - pos, 0);  // tokens into the stage
+            const int at_lane = (from >> pb_shift) & 31;
+            const int pg = __shfl_sync(0xffffffffu, page, at_lane), of = __shfl_sync(0xffffffffu, off, at_lane);
+            if (e < n_e) {
+              const long long at = ((long long)pg * Hkv + h) * (2 * scales_per_page) + ((of + (from & (pb - 1))) >> sb_shift);
+              cp_async4(sdst + e * 4, cache.scales + at);
+              cp_async4(sdst + (TK + e) * 4, cache.scales + at + scales_per_page);
+            }
           }
         }
         if (first) {
