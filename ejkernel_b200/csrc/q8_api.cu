@@ -49,6 +49,24 @@ int check_attention(const ejk_q8_shape& s) {
   return check_rpa_shape(as_rpa(s));
 }
 
+// The workspace: the split-KV kernel's arrival counters, which are zero between calls, its parts, and behind them what the
+// planner of the tensor tiles needs.
+struct Q8Workspace {
+  size_t part_ml_off, part_o_off, tiles_off, total;
+};
+Q8Workspace q8_workspace(const ejk_q8_shape& s, int n_sm, bool with_tiles) {
+  const size_t rt = s.num_q_heads / s.num_kv_heads > 8 ? 16 : 8, slots = 2 * 2 * (size_t)n_sm;
+  auto up = [](size_t x) { return (x + 255) / 256 * 256; };
+  Q8Workspace w;
+  w.part_ml_off = EJK_Q8_TICKET_BYTES;
+  w.part_o_off = up(w.part_ml_off + slots * rt * sizeof(float2));
+  w.tiles_off = up(w.part_o_off + slots * rt * s.head_dim * sizeof(float));
+  w.total = w.tiles_off + (with_tiles ? workspace_layout(as_rpa(s), n_sm).total_split : 0);
+  return w;
+}
+// can the batch hold a sequence of several tokens, for the tensor tiles?
+bool tiles_possible(const ejk_q8_shape& s) { return s.total_tokens > s.max_num_seqs && q8_prefill_supported(s.head_dim); }
+
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 bool finite(float x) { return x == x && !std::isinf(x); }
 
@@ -63,9 +81,8 @@ size_t ejk_q8_workspace_bytes(const ejk_q8_shape* shape) {
   if (!shape || check_attention(*shape) != 0) return 0;
   const int n_sm = sm100_sm_count();
   if (!n_sm) return 0;
-  const WorkspaceLayout L = workspace_layout(as_rpa(*shape), n_sm);
-  // shapes that can hold a multi-token sequence also get room for the parts of tensor-tile items cut along KV
-  return shape->total_tokens > shape->max_num_seqs && q8_prefill_supported(shape->head_dim) ? L.total_split : L.total;
+  if (3 * 2 * n_sm * sizeof(int32_t) > EJK_Q8_TICKET_BYTES) return 0;
+  return q8_workspace(*shape, n_sm, tiles_possible(*shape)).total;
 }
 
 int ejk_q8_attention_launch(const void* queries, const void* kv_pages, const float* kv_scales,
@@ -87,8 +104,10 @@ int ejk_q8_attention_launch(const void* queries, const void* kv_pages, const flo
   if (!aligned16(queries) || !aligned16(kv_pages) || !aligned16(kv_scales) || !aligned16(out)) return EJK_RPA_E_ALIGN;
   const int n_sm = sm100_sm_count();
   if (!n_sm) return EJK_RPA_E_DEVICE;
-  const WorkspaceLayout L = workspace_layout(as_rpa(s), n_sm);
-  if (workspace_bytes < L.total || (reinterpret_cast<uintptr_t>(workspace) & 255)) return EJK_RPA_E_WORKSPACE;
+  if (3 * 2 * n_sm * sizeof(int32_t) > EJK_Q8_TICKET_BYTES) return EJK_RPA_E_DEVICE;
+  const bool tiles = tiles_possible(s);
+  const Q8Workspace W = q8_workspace(s, n_sm, tiles);
+  if (workspace_bytes < W.total || (reinterpret_cast<uintptr_t>(workspace) & 255)) return EJK_RPA_E_WORKSPACE;
 
   const LaunchOptions opt = launch_options();
   const bool use_tma = opt.path != 1 && q8_tma_supported(s.page_size);
@@ -134,22 +153,10 @@ int ejk_q8_attention_launch(const void* queries, const void* kv_pages, const flo
   }
 
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  p.header = reinterpret_cast<int32_t*>(ws + L.header_off);
-  p.units = reinterpret_cast<Unit*>(ws + L.units_off);
-  p.punits = reinterpret_cast<Unit*>(ws + L.punits_off);
-  p.merge = reinterpret_cast<MergeItem*>(ws + L.merge_off);
-  p.tickets = reinterpret_cast<int32_t*>(ws + L.tickets_off);
-  p.part_o = reinterpret_cast<float*>(ws + L.part_o_off);
-  p.part_ml = reinterpret_cast<float2*>(ws + L.part_ml_off);
-  p.C2 = 2 * s.num_kv_heads;
-  p.rows_per_tile = L.rows_per_tile;
-  p.max_units = L.max_units;
-  p.max_merge = L.max_merge;
-  p.max_slots = L.max_slots;
-  p.max_punits = L.max_punits;
-  p.target_units = L.target_units;
-  p.target_units_max = L.target_units_max;
-  p.even_units = 2 * n_sm / s.num_kv_heads;
+  p.tickets = reinterpret_cast<int32_t*>(ws);
+  p.part_ml = reinterpret_cast<float2*>(ws + W.part_ml_off);
+  p.part_o = reinterpret_cast<float*>(ws + W.part_o_off);
+  p.rows_per_tile = p.G > 8 ? 16 : 8;
   p.min_chunk = opt.min_chunk;
   if (a.num_kv_pages_per_block > 0) {  // per-call hint: the smallest KV chunk, in pages
     long long chunk = (long long)a.num_kv_pages_per_block * s.page_size;
@@ -163,15 +170,6 @@ int ejk_q8_attention_launch(const void* queries, const void* kv_pages, const flo
   p.tma_block_shift = log2_exact(p.tma_block_tokens);
   p.wait_timeout_ms = opt.wait_ms;
   p.test_withhold = opt.test_withhold;
-  p.sort_items = opt.sort_items;
-  {
-    // the chunks of a row tile are combined by the last one to finish where a tile gets two at most, by a kernel of
-    // their own otherwise (the rule of ejk_rpa_launch)
-    const long long by_len = ((long long)s.pages_per_seq * s.page_size + p.min_chunk - 1) / p.min_chunk;
-    const bool few = (long long)L.target_units <= 2ll * s.total_tokens || by_len <= 2;
-    p.fused_merge = (opt.fused_merge == 2 || (opt.fused_merge == 1 && few)) ? 1 : 0;
-  }
-  p.prefill_item_rows = prefill_rows_per_item(s.head_dim);
   // Batches that can hold a sequence with many query rows also get the tensor-tile kernel; whether one qualifies is
   // decided by the planner on the device.
   int prefill_rows = opt.prefill_rows;
@@ -179,38 +177,50 @@ int ejk_q8_attention_launch(const void* queries, const void* kv_pages, const flo
     const long long r = (long long)a.num_queries_per_block * p.G;
     prefill_rows = r > 0x40000000ll ? 0x40000000 : (int)r;
   }
-  const bool use_prefill = prefill_rows > 0 && q8_prefill_supported(s.head_dim) &&
-                           (long long)s.total_tokens * p.G >= prefill_rows && s.total_tokens > s.max_num_seqs;
+  const bool use_prefill = tiles && prefill_rows > 0 && (long long)s.total_tokens * p.G >= prefill_rows;
   p.prefill_min_rows = use_prefill ? prefill_rows : 0;
   p.prefill_share = opt.prefill_share;
-  if (use_prefill && opt.prefill_split && workspace_bytes >= L.total_split) {
-    p.pprefix = reinterpret_cast<int32_t*>(ws + L.pprefix_off);
-    p.ptickets = reinterpret_cast<int32_t*>(ws + L.ptickets_off);
-    p.ppart_ml = reinterpret_cast<float2*>(ws + L.ppart_ml_off);
-    p.ppart_o = reinterpret_cast<float*>(ws + L.ppart_o_off);
-    p.prefill_split = opt.prefill_split;
+  if (use_prefill) {
+    const WorkspaceLayout L = workspace_layout(as_rpa(s), n_sm);
+    uint8_t* wt = ws + W.tiles_off;
+    p.header = reinterpret_cast<int32_t*>(wt + L.header_off);
+    p.units = reinterpret_cast<Unit*>(wt + L.units_off);
+    p.punits = reinterpret_cast<Unit*>(wt + L.punits_off);
+    p.merge = reinterpret_cast<MergeItem*>(wt + L.merge_off);
+    p.max_units = L.max_units;
+    p.max_merge = L.max_merge;
+    p.max_slots = L.max_slots;
+    p.max_punits = L.max_punits;
+    p.target_units = L.target_units;
+    p.target_units_max = L.target_units_max;
+    p.sort_items = opt.sort_items;
+    p.prefill_item_rows = prefill_rows_per_item(s.head_dim);
+    if (opt.prefill_split) {
+      p.pprefix = reinterpret_cast<int32_t*>(wt + L.pprefix_off);
+      p.ptickets = reinterpret_cast<int32_t*>(wt + L.ptickets_off);
+      p.ppart_ml = reinterpret_cast<float2*>(wt + L.ppart_ml_off);
+      p.ppart_o = reinterpret_cast<float*>(wt + L.ppart_o_off);
+      p.prefill_split = opt.prefill_split;
+    }
   }
   // Kernels of one call are launched as programmatic dependents: each waits on the device for what it needs of the one
   // before, the planner for whatever precedes the call.
   const bool pdl = opt.overlap != 0;
   p.pdl = pdl ? (use_prefill ? 1 : 2) : 0;
   int launches = 0;
-  cudaError_t e = launch_plan(p, st, pdl);
-  if (e != cudaSuccess) return static_cast<int>(e);
-  ++launches;
+  cudaError_t e;
   if (use_prefill) {
+    Params plan = p;  // the planner clears counters of its own
+    plan.tickets = reinterpret_cast<int32_t*>(ws + W.tiles_off + workspace_layout(as_rpa(s), n_sm).tickets_off);
+    e = launch_plan(plan, st, pdl);
+    if (e != cudaSuccess) return static_cast<int>(e);
     e = launch_q8_prefill(p, c, s.dtype, s.code_dtype, n_sm, st, pdl);
     if (e != cudaSuccess) return static_cast<int>(e);
-    ++launches;
+    launches += 2;
   }
   e = launch_q8_splitkv(p, c, s.dtype, s.code_dtype, n_sm, st, pdl);
   if (e != cudaSuccess) return static_cast<int>(e);
   ++launches;
-  if (!p.fused_merge) {
-    e = launch_merge(p, s.dtype, n_sm, st, pdl);
-    if (e != cudaSuccess) return static_cast<int>(e);
-    ++launches;
-  }
   set_last_launches(launches);
   return 0;
 }

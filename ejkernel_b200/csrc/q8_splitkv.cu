@@ -4,14 +4,19 @@
 //   O   += (p_j * v_scale_j) v_j,  l += p_j;   out = O / l
 //
 // The kernel is a stream of the cache: every byte of K and V is read once per kv head and costs 2 * G multiply-adds, so
-// DRAM bounds it, and everything else has to stay out of the way.  Work items, queue, partials and merge are those of
-// rpa_splitkv_tma.cu; what differs follows from the codes:
-//   * a stage is 128 tokens of one head, fetched by one producer warp as TMA boxes of up to 64 tokens.  A head's page is
+// DRAM bounds it, and everything else has to stay out of the way.
+//   * Work: the 128-token stages of all (row tile, kv head) pairs form one sequence that is cut into equal quotas, one per
+//     CTA.  Every CTA finds its quota itself, from the lengths (a scan of a microsecond that all CTAs do at the same time):
+//     no planner runs before this kernel, no queue is drawn from, no SM waits for the last item of another.  A pair that
+//     straddles a quota boundary is finished by several CTAs; the last of them to arrive combines their parts, in part order,
+//     sixteen at a time.  A CTA has two partial pieces at most, so the parts of all calls fit 2 slots per CTA.
+//   * A stage is 128 tokens of one head, fetched by one producer warp as TMA boxes of up to 64 tokens.  A head's page is
 //     contiguous, so a box of 16 tokens at head_dim 128 is two runs of 2 KB.  The stage's scales come beside it with 4-byte
 //     cp.async copies that arrive on the same mbarrier: no wait of the producer stands between two stages.
-//   * four consumer warps take 32 tokens each.  Codes go to f16 in registers, which is exact for both types, and both
+//   * Four consumer warps take 32 tokens each.  Codes go to f16 in registers, which is exact for both types, and both
 //     products run on f16 mma.sync with float32 sums.  8-bit operands would halve the mma work, which is not what bounds
-//     the kernel, and would round q and p to 3 bits of mantissa.
+//     the kernel, and would round q and p to 3 bits of mantissa.  (Eight warps in two teams that take the stages in turn
+//     were slower: 0.50 ms against 0.37 for 128 sequences of 8192 keys; the registers go down to 96.)
 //   * k_scale multiplies the finished dot product, v_scale the probability: two multiplications a token and row, none per
 //     element.  p * v_scale has to fit f16: a warp divides v_scale by a power of two, chosen from the largest scale that
 //     it has met so that the product is at most 2^15, and moves it as it moves m.  What is below 2^-24 of that
@@ -36,14 +41,25 @@ constexpr int kConsumerWarps = 4;
 constexpr int kThreads = (kConsumerWarps + 1) * 32;
 constexpr int kRing = 8;
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kMergeInFlight = 8;     // partials whose loads the last-arriver merge keeps in flight per row
+constexpr int kMergeInFlight = 8;     // parts whose loads a merge keeps in flight per row
+constexpr int kGroup = 16;            // parts that are combined at a time: more go through groups
 constexpr float kLazyRescale = 8.0f;  // rescale the accumulators only when the max grows by 2^8: p <= 2^8
 constexpr int kVBits = 6;             // the largest v_scale met so far is taken to [2^6, 2^7): p * v_scale <= 2^15 < 65504
 
+// One piece of work of a CTA: stages of one (row tile, kv head).  Of a pair that several CTAs share, u.n_chunks is the number of
+// parts, u.chunk_idx this part's number and u.merge_idx the CTA of part 0; u.slot is where this part goes, u.pad where part 0 is.
 struct ItemDesc {
   Unit u;
   int32_t h;
-  int32_t pad[3];
+  int32_t first;  // the CTA's first piece
+  int32_t pad[2];
+};
+
+// What a CTA works out before it starts: the sequences that hold the first and the last stage of its quota, and the stages (per
+// head) of the sequences before them.
+struct Share {
+  long long base[2];
+  int seq[2];
 };
 
 template <int D, int NT, int NS>
@@ -69,10 +85,12 @@ struct Cfg {
   static constexpr int OFF_RING = (OFF_ROWL + RT * 4 + 63) / 64 * 64;
   static constexpr int OFF_META = OFF_RING + kRing * (int)sizeof(ItemDesc);
   static constexpr int OFF_BAR = OFF_META + NS * 8;  // full[NS], empty[NS], cbar
-  static constexpr int OFF_ABORT = OFF_BAR + (2 * NS + 1) * 8;
+  static constexpr int OFF_SHARE = OFF_BAR + (2 * NS + 1) * 8;
+  static constexpr int OFF_ABORT = OFF_SHARE + (int)sizeof(Share);
   static constexpr int SMEM_BYTES = OFF_ABORT + 16 + 1024;  // + alignment slack
   static constexpr int CTAS = SMEM_BYTES <= 112 * 1024 ? 2 : 1;
   static_assert(SMEM_BYTES <= 227 * 1024, "shared memory budget");
+  static_assert(NT == 2 || D == 256 || CTAS == 2, "two CTAs per SM for the usual shapes");
 };
 
 __device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2,
@@ -103,6 +121,68 @@ __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) {
   return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
 }
 
+// ---- the stages of a sequence ----
+struct Seq {
+  int q_start, q_len, kv_len, tiles;  // tiles = 0: nothing to do here
+};
+__device__ __forceinline__ Seq load_seq(const Params& p, int s, int rows_per_tile, unsigned& flags) {
+  const int q0 = __ldg(p.query_start_loc + s), q1 = __ldg(p.query_start_loc + s + 1);
+  int kv = __ldg(p.context_lens + s);
+  const int kv_cap = p.pages_per_seq * p.page_size;
+  if (kv < 0 || kv > kv_cap) {
+    flags |= EJK_RPA_ST_KVLEN;
+    kv = kv < 0 ? 0 : kv_cap;
+  }
+  int ql = q1 - q0;
+  if (ql < 0 || q0 < 0 || q1 > p.T) {
+    flags |= EJK_RPA_ST_QLEN;
+    ql = 0;
+  }
+  if (ql > kv) flags |= EJK_RPA_ST_QLEN;  // rows at negative positions see no key and produce 0
+  const int rows = ql * p.G;
+  const bool tiles_elsewhere = p.prefill_min_rows > 0 && rows >= p.prefill_min_rows;  // served by tensor tiles
+  return {q0, ql, kv, tiles_elsewhere ? 0 : (rows + rows_per_tile - 1) / rows_per_tile};
+}
+// keys [lo, hi) that some row of tile t sees; lo is rounded down to where boxes may start.  Returns the stages, at least one
+__device__ __forceinline__ int tile_stages(const Params& p, const Seq& q, int t, int rows_per_tile, int& lo, int& hi) {
+  const int r_first = t * rows_per_tile;
+  const int r_last = min(r_first + rows_per_tile, q.q_len * p.G) - 1;
+  const int base = q.kv_len - q.q_len;
+  hi = max(base + r_last / p.G + 1, 0);
+  lo = 0;
+  if (p.window > 0) lo = max(base + r_first / p.G - p.window + 1, 0) / kTileTokens * kTileTokens;
+  hi = max(hi, lo);
+  return max((hi - lo + 127) >> 7, 1);
+}
+__device__ __forceinline__ long long seq_stages(const Params& p, const Seq& q, int rows_per_tile) {
+  long long n = 0;
+  int lo, hi;
+  for (int t = 0; t < q.tiles; ++t) n += tile_stages(p, q, t, rows_per_tile, lo, hi);
+  return n;
+}
+
+// ---- combining the parts of a pair ----
+// Arrival counters, three per CTA, zero between calls: atomicInc with the number of arrivals as its limit takes a counter back to
+// zero with the last of them.  [c]: the first sixteen parts of the pair that begins in CTA c; [n + c]: the sixteen parts that
+// begin with CTA c's, of a pair that begins earlier; [2n + c]: the groups of the pair that begins in CTA c.
+struct Arrival {
+  int count;   // parts (or groups) to combine now; 0: others are still to come
+  int stride;  // in parts
+  int part0;
+  bool last;   // they are all there is
+};
+__device__ __forceinline__ Arrival arrive_part(int* tickets, int n_cta, int c0, int part, int n_parts) {
+  const int g = part / kGroup;
+  const int size = min(kGroup, n_parts - g * kGroup);
+  const unsigned old = atomicInc(reinterpret_cast<unsigned*>(tickets + (g ? n_cta + c0 + g * kGroup : c0)), (unsigned)size - 1u);
+  return {old == (unsigned)size - 1u ? size : 0, 1, g * kGroup, n_parts <= kGroup};
+}
+__device__ __forceinline__ Arrival arrive_group(int* tickets, int n_cta, int c0, int n_parts) {
+  const int groups = (n_parts + kGroup - 1) / kGroup;
+  const unsigned old = atomicInc(reinterpret_cast<unsigned*>(tickets + 2 * n_cta + c0), (unsigned)groups - 1u);
+  return {old == (unsigned)groups - 1u ? groups : 0, kGroup, 0, true};
+}
+
 template <typename T, typename Code, int D, int NT, int NS>
 __global__ void __launch_bounds__(kThreads, (Cfg<D, NT, NS>::CTAS))
 q8_splitkv_kernel(const __grid_constant__ CUtensorMap tmap, const Params p, const Q8Cache cache) {
@@ -122,6 +202,7 @@ q8_splitkv_kernel(const __grid_constant__ CUtensorMap tmap, const Params p, cons
   ItemDesc* ring = reinterpret_cast<ItemDesc*>(smem + C::OFF_RING);
   int2* metas = reinterpret_cast<int2*>(smem + C::OFF_META);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::OFF_ABORT);
+  Share* share = reinterpret_cast<Share*>(smem + C::OFF_SHARE);
   const uint32_t bar_full = smem_base + C::OFF_BAR;
   const uint32_t bar_empty = bar_full + NS * 8;
   const uint32_t bar_c = bar_empty + NS * 8;
@@ -145,9 +226,65 @@ q8_splitkv_kernel(const __grid_constant__ CUtensorMap tmap, const Params p, cons
     asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
   }
   __syncthreads();
-  // launched as a programmatic dependent of the planner: everything above overlapped its tail
+  // launched as a programmatic dependent: everything above overlapped the tail of what came before.  Behind the tensor-tile
+  // kernel there is nothing to wait for: it is released by CTAs that have themselves waited for all earlier work
   if (p.pdl & 2) pdl_wait();
-  const int n_work = p.header[kHdrNumUnits] * Hkv;
+
+  // ---- this CTA's quota of the stages
+  int S = __ldg(p.num_seqs);
+  if (S > p.S_max) {
+    flags |= EJK_RPA_ST_NUM_SEQS;
+    S = p.S_max;
+  }
+  if (S < 0) S = 0;
+  const int n_cta = (int)gridDim.x;
+  int quota;
+  long long g0, g1;
+  {
+    long long* s_sum = reinterpret_cast<long long*>(obuf);  // not in use yet
+    const int per = (S + kThreads - 1) / kThreads;
+    const int a = min(tid * per, S), b = min(a + per, S);
+    long long mine = 0;
+    for (int i = a; i < b; ++i) mine += seq_stages(p, load_seq(p, i, RT, flags), RT);
+    if (blockIdx.x != 0) flags = 0;  // one CTA reports
+    long long incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long y = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += y;
+    }
+    if (lane == 31) s_sum[warp] = incl;
+    __syncthreads();
+    long long before = incl - mine, total = 0;
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; ++w) {
+      if (w < warp) before += s_sum[w];
+      total += s_sum[w];
+    }
+    const long long all = total * Hkv;
+    const long long even = (all + n_cta - 1) / n_cta;
+    quota = (int)max(even, (long long)(p.min_chunk >> 7));  // shorter pieces cost more to combine than they save
+    g0 = min((long long)blockIdx.x * quota, all);
+    g1 = min(g0 + quota, all);
+    if (g0 < g1 && mine > 0) {
+      for (int e = 0; e < 2; ++e) {
+        const long long g = e ? g1 - 1 : g0;
+        if (g < before * Hkv || g >= (before + mine) * Hkv) continue;
+        long long base = before;
+        unsigned none = 0;
+        for (int i = a; i < b; ++i) {
+          const long long n = seq_stages(p, load_seq(p, i, RT, none), RT);
+          if (g < (base + n) * Hkv) {
+            share->base[e] = base;
+            share->seq[e] = i;
+            break;
+          }
+          base += n;
+        }
+      }
+    }
+    __syncthreads();
+  }
 
   if (warp == kConsumerWarps) {
     // =============================== producer warp ===============================
@@ -158,12 +295,37 @@ q8_splitkv_kernel(const __grid_constant__ CUtensorMap tmap, const Params p, cons
     uint32_t empty_parity = 1;  // a fresh barrier passes a wait on parity 1: all stages start empty
     int k = 0;
     int fills = 0;  // stages announced so far
-    int wid = 0;
-    if (lane == 0) wid = atomicAdd(&p.header[kHdrQueue], 1);
-    wid = __shfl_sync(0xffffffffu, wid, 0);
+    // where the next piece starts: stage `rel` (per head sequence, heads one after the other) of tile t of sequence sq
+    long long g = g0;
+    int sq = 0, t = 0;
+    long long rel = 0;
+    Seq cur = {0, 0, 0, 0};
+    // 32 sequences' lengths at a time, one per lane
+    int seq_block = -1;
+    Seq ahead = {0, 0, 0, 0};
+    auto fetch_seq = [&](int i) {
+      if ((i >> 5) != seq_block) {
+        seq_block = i >> 5;
+        unsigned none = 0;
+        const int mine = seq_block * 32 + lane;
+        ahead = {0, 0, 0, 0};
+        if (mine < S) ahead = load_seq(p, mine, RT, none);
+      }
+      Seq q;
+      q.q_start = __shfl_sync(0xffffffffu, ahead.q_start, i & 31);
+      q.q_len = __shfl_sync(0xffffffffu, ahead.q_len, i & 31);
+      q.kv_len = __shfl_sync(0xffffffffu, ahead.kv_len, i & 31);
+      q.tiles = __shfl_sync(0xffffffffu, ahead.tiles, i & 31);
+      return q;
+    };
+    if (g < g1) {
+      sq = share->seq[0];
+      rel = g - share->base[0] * Hkv;
+      cur = fetch_seq(sq);
+    }
     bool alive = true;
     while (alive) {
-      if (wid >= n_work) {
+      if (g >= g1) {
         // end-of-stream marker for the consumers
         if (!mbar_wait(bar_empty + s * 8, empty_parity, abort_flag, wait_ns)) break;
         if (lane == 0) {
@@ -174,19 +336,48 @@ q8_splitkv_kernel(const __grid_constant__ CUtensorMap tmap, const Params p, cons
         ++fills;
         break;
       }
-      const int ui = wid / Hkv;
-      const int h = wid - ui * Hkv;
-      Unit u;
-      {
-        const int4* src = reinterpret_cast<const int4*>(p.units + ui);
-        const int4 a = __ldg(src), b = __ldg(src + 1), c3 = __ldg(src + 2);
-        u.seq = a.x; u.row0 = a.y; u.kv_begin = a.z; u.kv_end = a.w;
-        u.slot = b.x; u.q_start = b.y; u.q_len = b.z; u.kv_len = b.w;
-        u.merge_idx = c3.x; u.chunk_idx = c3.y; u.n_chunks = c3.z; u.pad = 0;
+      // the tile that holds stage `rel`
+      int lo = 0, hi = 0, n_t = 0;
+      while (true) {
+        if (t >= cur.tiles) {
+          if (++sq >= S) break;
+          cur = fetch_seq(sq);
+          t = 0;
+          continue;
+        }
+        n_t = tile_stages(p, cur, t, RT, lo, hi);
+        if (rel < (long long)n_t * Hkv) break;
+        rel -= (long long)n_t * Hkv;
+        ++t;
       }
+      if (sq >= S) {  // only if the lengths change under the call
+        *abort_flag = 1;
+        break;
+      }
+      const int h = (int)(rel / n_t), st = (int)(rel - (long long)h * n_t);
+      const int take = (int)min((long long)(n_t - st), g1 - g);
+      Unit u;
+      u.seq = sq;
+      u.row0 = t * RT;
+      u.kv_begin = lo + st * TK;
+      u.kv_end = st + take == n_t ? hi : lo + (st + take) * TK;
+      u.q_start = cur.q_start;
+      u.q_len = cur.q_len;
+      u.kv_len = cur.kv_len;
+      {
+        const long long fs = g - st;  // the pair's first stage
+        const int c0 = (int)(fs / quota), c1 = (int)((fs + n_t - 1) / quota);
+        u.n_chunks = c1 - c0 + 1;
+        u.chunk_idx = (int)blockIdx.x - c0;
+        u.merge_idx = c0;
+        // slot 2c: the piece that CTA c begins with, 2c + 1: the one that it ends with
+        u.pad = fs == (long long)c0 * quota ? 2 * c0 : 2 * c0 + 1;
+        u.slot = u.n_chunks == 1 ? -1 : (u.chunk_idx == 0 ? u.pad : 2 * (int)blockIdx.x);
+      }
+      const bool first_piece = g == g0;
+      g += take;
+      rel += take;
       const int ring_slot = k % kRing;
-      int wid_next = 0;
-      if (lane == 0) wid_next = atomicAdd(&p.header[kHdrQueue], 1);  // consumed only at the next item
       const int32_t* tab = p.block_tables + (size_t)u.seq * p.pages_per_seq;
       // page of the block of tokens that this lane fetches; read a stage ahead, so that its latency lies under the stage before
       auto page_of = [&](int pos, int& off) {
@@ -219,7 +410,7 @@ q8_splitkv_kernel(const __grid_constant__ CUtensorMap tmap, const Params p, cons
           break;
         }
         // test hook: the stage is never announced, the consumers' wait for it must run out
-        const bool withhold = (p.test_withhold & 1) && wid == 0 && first;
+        const bool withhold = (p.test_withhold & 1) && blockIdx.x == 0 && k == 0 && first;
         const uint32_t full = bar_full + s * 8;
         if (!withhold) {
           if (lane == 0 && nblk > 0)  // the bytes are expected before the first copy can report them; no arrival yet
@@ -249,6 +440,7 @@ q8_splitkv_kernel(const __grid_constant__ CUtensorMap tmap, const Params p, cons
             ItemDesc d;
             d.u = u;
             d.h = h;
+            d.first = first_piece;
             ring[ring_slot] = d;
           }
           constexpr int QCH = D / 8;  // 16-byte chunks of a row: 8, 16 or 32 neighbouring lanes hold one row
@@ -306,7 +498,6 @@ q8_splitkv_kernel(const __grid_constant__ CUtensorMap tmap, const Params p, cons
         }
       }
       ++k;
-      wid = __shfl_sync(0xffffffffu, wid_next, 0);
     }
     // Leave only after every bulk copy this warp issued has landed: wait (bounded) for the
     // consumers to drain all stages, which implies all "full" phases completed.
@@ -354,6 +545,7 @@ q8_splitkv_kernel(const __grid_constant__ CUtensorMap tmap, const Params p, cons
     float v_norm = 1.f;  // power of two that the V scales are multiplied by
     int s = 0;
     uint32_t full_parity = 0, c_parity = 0;
+    int arrived = 0, owed = 0;  // thread 0: bit 0 / 1 = the CTA's first / another shared piece has been counted; its group not yet
 
     auto consumer_sync = [&]() -> bool {
       __syncwarp();
@@ -370,6 +562,7 @@ q8_splitkv_kernel(const __grid_constant__ CUtensorMap tmap, const Params p, cons
       const ItemDesc& it = ring[meta.x];
       const Unit u = it.u;
       const int h = it.h;
+      const bool first_piece = it.first != 0;
       const int pos = meta.y;
       const uint32_t sbase = smem_base + s * C::STAGE_BYTES;
       const int rows_total = u.q_len * G;
@@ -710,103 +903,121 @@ q8_splitkv_kernel(const __grid_constant__ CUtensorMap tmap, const Params p, cons
                   Mma<T>::pack(v.x * scl, v.y * scl);
           }
         } else {
-          float* po = p.part_o + ((size_t)u.slot * Hkv + h) * RT * D;
-          float2* pml = p.part_ml + ((size_t)u.slot * Hkv + h) * RT;
+          float* po = p.part_o + (size_t)u.slot * RT * D;
+          float2* pml = p.part_ml + (size_t)u.slot * RT;
           for (int i = tid; i < n_rows * (D / 4); i += kCT) {
             const int r = i / (D / 4), d = (i % (D / 4)) * 4;
             const float4 v = *reinterpret_cast<float4*>(&obuf[r * D + d]);
             *reinterpret_cast<float4*>(po + r * D + d) = v;
           }
           if (tid < n_rows) pml[tid] = make_float2(row_m[tid], row_l[tid]);
-          if (p.fused_merge) {
-            // Last-arriver merge: publish this chunk's partial, take a ticket for (tile, kv head); the
-            // chunk that draws the last ticket combines all of them, in chunk order, so the result
-            // does not depend on which chunk finished last.  No CTA ever waits for another.
+          // Last-arriver merge: publish this part, take a ticket; whoever draws the last one combines the parts, in part
+          // order, so that the result does not depend on who that is.  No CTA ever waits for another.
+          const int c0 = u.merge_idx;
+          bool groups = false;
+          bool ok = true;
+          while (true) {
             __threadfence();
-            if (!consumer_sync()) break;
+            if (!(ok = consumer_sync())) break;
             if (tid == 0) {
-              const int old = atomicAdd(&p.tickets[(size_t)u.merge_idx * Hkv + h], 1);
-              row_l[0] = (old == u.n_chunks - 1) ? 1.f : 0.f;  // row_l/row_m were consumed above
+              const Arrival a = groups ? arrive_group(p.tickets, n_cta, c0, u.n_chunks)
+                                       : arrive_part(p.tickets, n_cta, c0, u.chunk_idx, u.n_chunks);
+              // row_l was consumed above
+              row_l[0] = __int_as_float(a.count);
+              row_l[1] = __int_as_float(a.stride);
+              row_l[2] = __int_as_float(a.part0);
+              row_l[3] = __int_as_float(a.last);
+              const int bit = first_piece ? 1 : 2;
+              arrived |= bit;
+              owed = a.count && !a.last ? owed | bit : owed & ~bit;
             }
-            if (!consumer_sync()) break;
-            const bool last = row_l[0] != 0.f;
-            if (last) {
-              __threadfence();
-              constexpr int VPL = D / 32;
-              const int slot0 = u.slot - u.chunk_idx;
-              T* out = reinterpret_cast<T*>(p.out);
-              for (int r = warp; r < n_rows; r += kConsumerWarps) {
-                float m_tot = -INFINITY;
-                for (int c = lane; c < u.n_chunks; c += 32)
-                  m_tot = fmaxf(m_tot, __ldcg(&p.part_ml[((size_t)(slot0 + c) * Hkv + h) * RT + r]).x);
+            if (!(ok = consumer_sync())) break;
+            const int count = __float_as_int(row_l[0]), stride = __float_as_int(row_l[1]), part0 = __float_as_int(row_l[2]);
+            const bool last = __float_as_int(row_l[3]) != 0;
+            if (count == 0) break;
+            __threadfence();
+            constexpr int VPL = D / 32;
+            T* out = reinterpret_cast<T*>(p.out);
+            auto slot_of = [&](int i) {
+              const int part = part0 + i * stride;
+              return part == 0 ? u.pad : 2 * (c0 + part);
+            };
+            for (int r = warp; r < n_rows; r += kConsumerWarps) {
+              // lane i holds part i's maximum and sum (count <= 32)
+              const float2 ml = lane < count ? __ldcg(&p.part_ml[(size_t)slot_of(lane) * RT + r]) : make_float2(-INFINITY, 0.f);
+              float m_tot = ml.x;
 #pragma unroll
-                for (int o = 16; o > 0; o >>= 1) m_tot = fmaxf(m_tot, __shfl_xor_sync(0xffffffffu, m_tot, o));
-                const float mu = (m_tot == -INFINITY) ? 0.f : m_tot;
-                float accm[VPL];
+              for (int o = 16; o > 0; o >>= 1) m_tot = fmaxf(m_tot, __shfl_xor_sync(0xffffffffu, m_tot, o));
+              const float mu = (m_tot == -INFINITY) ? 0.f : m_tot;
+              const float f_mine = fast_exp2(ml.x - mu);
+              float l_tot = ml.y * f_mine;
 #pragma unroll
-                for (int i = 0; i < VPL; ++i) accm[i] = 0.f;
-                float l_tot = 0.f;
-                // kMergeInFlight chunks' loads in flight at a time (each is an L2 round trip); the sums still run in
-                // chunk order
-                for (int c0 = 0; c0 < u.n_chunks; c0 += kMergeInFlight) {
-                  float2 ml[kMergeInFlight];
-                  float vv[kMergeInFlight][VPL];
+              for (int o = 16; o > 0; o >>= 1) l_tot += __shfl_xor_sync(0xffffffffu, l_tot, o);
+              float accm[VPL];
 #pragma unroll
-                  for (int j = 0; j < kMergeInFlight; ++j) {
-                    const int c = min(c0 + j, u.n_chunks - 1);
-                    const size_t base = ((size_t)(slot0 + c) * Hkv + h) * RT + r;
-                    ml[j] = __ldcg(&p.part_ml[base]);
-                    const float* src = p.part_o + base * D + lane * VPL;
-                    if constexpr (VPL == 2) {
-                      const float2 v = __ldcg(reinterpret_cast<const float2*>(src));
-                      vv[j][0] = v.x;
-                      vv[j][1] = v.y;
-                    } else {
+              for (int i = 0; i < VPL; ++i) accm[i] = 0.f;
+              for (int i0 = 0; i0 < count; i0 += kMergeInFlight) {
+                float vv[kMergeInFlight][VPL];
 #pragma unroll
-                      for (int i = 0; i < VPL; i += 4) {
-                        const float4 v = __ldcg(reinterpret_cast<const float4*>(src + i));
-                        vv[j][i] = v.x;
-                        vv[j][i + 1] = v.y;
-                        vv[j][i + 2] = v.z;
-                        vv[j][i + 3] = v.w;
-                      }
-                    }
-                  }
+                for (int j = 0; j < kMergeInFlight; ++j) {
+                  const float* src = p.part_o + ((size_t)slot_of(min(i0 + j, count - 1)) * RT + r) * D + lane * VPL;
+                  if constexpr (VPL == 2) {
+                    const float2 v = __ldcg(reinterpret_cast<const float2*>(src));
+                    vv[j][0] = v.x;
+                    vv[j][1] = v.y;
+                  } else {
 #pragma unroll
-                  for (int j = 0; j < kMergeInFlight; ++j) {
-                    if (c0 + j < u.n_chunks) {
-                      const float f = fast_exp2(ml[j].x - mu);
-                      l_tot += ml[j].y * f;
-#pragma unroll
-                      for (int i = 0; i < VPL; ++i) accm[i] += vv[j][i] * f;
+                    for (int i = 0; i < VPL; i += 4) {
+                      const float4 v = __ldcg(reinterpret_cast<const float4*>(src + i));
+                      vv[j][i] = v.x;
+                      vv[j][i + 1] = v.y;
+                      vv[j][i + 2] = v.z;
+                      vv[j][i + 3] = v.w;
                     }
                   }
                 }
-                const int R = u.row0 + r;
-                const int qt = R / G, g = R - qt * G;
-                const int hq = h * G + g;
-                float scl = 1.f, l_fin = l_tot;
-                if (p.num_sinks > 0) {
-                  const int srow = (p.sink_rows == p.Hq) ? hq : (p.sink_rows == Hkv ? h : 0);
-                  const float* sk = p.sinks + (size_t)srow * p.num_sinks;
-                  float sm = -INFINITY;
-                  for (int i = 0; i < p.num_sinks; ++i) sm = fmaxf(sm, sk[i] * kLog2e);
-                  const float m_fin = fmaxf(m_tot, sm);
-                  const float mf = (m_fin == -INFINITY) ? 0.f : m_fin;
-                  scl = fast_exp2(m_tot - mf);
-                  l_fin = l_tot * scl;
-                  for (int i = 0; i < p.num_sinks; ++i) l_fin += fast_exp2(sk[i] * kLog2e - mf);
-                }
-                scl = (l_fin > 0.f) ? scl / l_fin : 0.f;
-                T* dst = out + ((size_t)(u.q_start + qt) * p.Hq + hq) * D + lane * VPL;
-                {
 #pragma unroll
-                  for (int i = 0; i < VPL; i += 2)
-                    *reinterpret_cast<uint32_t*>(dst + i) = Mma<T>::pack(accm[i] * scl, accm[i + 1] * scl);
+                for (int j = 0; j < kMergeInFlight; ++j) {
+                  const float f = __shfl_sync(0xffffffffu, f_mine, min(i0 + j, 31));
+                  if (i0 + j < count) {
+#pragma unroll
+                    for (int i = 0; i < VPL; ++i) accm[i] += vv[j][i] * f;
+                  }
                 }
               }
+              if (!last) {
+                // a group: its sum takes the place of its first part
+                float* dst = p.part_o + ((size_t)slot_of(0) * RT + r) * D + lane * VPL;
+#pragma unroll
+                for (int i = 0; i < VPL; i += 2) *reinterpret_cast<float2*>(dst + i) = make_float2(accm[i], accm[i + 1]);
+                if (lane == 0) p.part_ml[(size_t)slot_of(0) * RT + r] = make_float2(m_tot, l_tot);
+                continue;
+              }
+              const int R = u.row0 + r;
+              const int qt = R / G, g = R - qt * G;
+              const int hq = h * G + g;
+              float scl = 1.f, l_fin = l_tot;
+              if (p.num_sinks > 0) {
+                const int srow = (p.sink_rows == p.Hq) ? hq : (p.sink_rows == Hkv ? h : 0);
+                const float* sk = p.sinks + (size_t)srow * p.num_sinks;
+                float sm = -INFINITY;
+                for (int i = 0; i < p.num_sinks; ++i) sm = fmaxf(sm, sk[i] * kLog2e);
+                const float m_fin = fmaxf(m_tot, sm);
+                const float mf = (m_fin == -INFINITY) ? 0.f : m_fin;
+                scl = fast_exp2(m_tot - mf);
+                l_fin = l_tot * scl;
+                for (int i = 0; i < p.num_sinks; ++i) l_fin += fast_exp2(sk[i] * kLog2e - mf);
+              }
+              scl = (l_fin > 0.f) ? scl / l_fin : 0.f;
+              T* dst = out + ((size_t)(u.q_start + qt) * p.Hq + hq) * D + lane * VPL;
+#pragma unroll
+              for (int i = 0; i < VPL; i += 2)
+                *reinterpret_cast<uint32_t*>(dst + i) = Mma<T>::pack(accm[i] * scl, accm[i + 1] * scl);
             }
+            if (last) break;
+            groups = true;
           }
+          if (!ok) break;
         }
         // The next item's writes to mbuf/lbuf come before its first consumer_sync, but they only
         // race with readers of mbuf/lbuf, and those finished before the first combine step's sync above; its
@@ -819,9 +1030,40 @@ q8_splitkv_kernel(const __grid_constant__ CUtensorMap tmap, const Params p, cons
       }
     }
     if (*abort_flag) flags |= EJK_RPA_ST_TIMEOUT;
+    if (*abort_flag && tid == 0 && g0 < g1) {
+      // Giving up: the shared pieces that were not counted are counted now, with no data, so that the counters are zero again
+      // after the call (the outputs are invalid, which the status says).
+      for (int e = 0; e < 2; ++e) {
+        const long long g = e ? g1 - 1 : g0;
+        unsigned none = 0;
+        const Seq q = load_seq(p, share->seq[e], RT, none);
+        long long rel = g - share->base[e] * Hkv;
+        int lo, hi, n_t = 1;
+        for (int t = 0; t < q.tiles; ++t) {
+          n_t = tile_stages(p, q, t, RT, lo, hi);
+          if (rel < (long long)n_t * Hkv) break;
+          rel -= (long long)n_t * Hkv;
+        }
+        const long long fs = g - rel % n_t;
+        const int c0 = (int)(fs / quota), c1 = (int)((fs + n_t - 1) / quota);
+        const int bit = fs <= g0 ? 1 : 2;  // the CTA's first piece, or another
+        if (c0 == c1) continue;
+        bool group_next = (owed & bit) != 0;
+        if (!(arrived & bit)) {
+          const Arrival a = arrive_part(p.tickets, n_cta, c0, (int)blockIdx.x - c0, c1 - c0 + 1);
+          group_next = a.count && !a.last;
+        }
+        if (group_next) arrive_group(p.tickets, n_cta, c0, c1 - c0 + 1);
+        arrived |= bit;
+        owed &= ~bit;
+      }
+    }
   }
   if (flags && p.status) atomicOr(reinterpret_cast<unsigned*>(p.status), flags);
-  zero_tail_rows(p.out, p.header[kHdrTailStart], p.T, (size_t)p.Hq * D * sizeof(T));
+  {
+    const int tail = S > 0 ? __ldg(p.query_start_loc + S) : __ldg(p.query_start_loc);
+    zero_tail_rows(p.out, min(max(tail, 0), p.T), p.T, (size_t)p.Hq * D * sizeof(T));
+  }
   // In a mixed batch this grid is a programmatic dependent of the prefill-tile grid and never waited for it
   // (the two write different rows).  Whatever follows in the stream, though, is only ordered after THIS grid:
   // one thread per CTA now waits for the prefill grid, so this grid cannot complete before it, and a later

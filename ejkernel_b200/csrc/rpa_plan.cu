@@ -234,11 +234,6 @@ __global__ void __launch_bounds__(kPlanThreads) rpa_plan_kernel(const Params p) 
     // 0.451 -> 0.442 ms, one of four 0.864 -> 0.842, one of two 1.635 -> 1.616.  Batches of many tiles with a chunk
     // or two each (256 decode sequences of up to 8k tokens) are faster with fewer, longer items.
     if (p.target_units_max > p.target_units && (unsigned long long)s_tiles * 4ull <= tgt) tgt = (unsigned long long)p.target_units_max;
-    // With very few row tiles one wave of equal items is better still: every CTA has exactly one, and there are as few partials
-    // as CTAs (each tile's last chunk may be short, hence the tiles are taken off).  8-bit cache, 4 sequences of
-    // 60k-131k tokens on one kv head.
-    if (p.even_units > 0 && s_tiles > 0 && (unsigned long long)s_tiles * 8ull <= (unsigned long long)p.even_units)
-      tgt = (unsigned long long)(p.even_units - s_tiles);
     unsigned long long c = (total + tgt - 1) / tgt;
     c = ((c + kTileTokens - 1) / kTileTokens) * kTileTokens;
     if (c < (unsigned long long)p.min_chunk) c = p.min_chunk;

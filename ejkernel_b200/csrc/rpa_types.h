@@ -94,7 +94,6 @@ struct Params {
   int32_t rows_per_tile;
   int32_t max_units, max_merge, max_slots, target_units, min_chunk;
   int32_t target_units_max;  // the planner may aim for this many items instead (see its pass 1); sizes the workspace
-  int32_t even_units;  // 8-bit cache: > 0 = a batch of few row tiles is cut into this many equal items, one per CTA
   int32_t max_punits;
   int32_t prefill_item_rows; // rows one prefill work item covers (128 per tile, 1 or 2 tiles per CTA)
   int32_t Dkv;               // elements between consecutive combined heads of kv_pages (head_dim, or the padded

@@ -149,11 +149,14 @@ def _after(device: torch.device, what: str) -> None:
 
 def _workspace(nbytes: int, device: torch.device, stream: int) -> torch.Tensor:
     if _capturing():
-        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        ws[: _cabi.Q8_TICKET_BYTES].zero_()  # a step of the graph: its memory may have had other uses
+        return ws
     key = (device.index, stream)
     ws = _scratch.pop(key, None)
     if ws is None or ws.shape[0] < nbytes:
         ws = torch.empty(1 << max(16, (nbytes - 1).bit_length()), dtype=torch.uint8, device=device)
+        ws[: _cabi.Q8_TICKET_BYTES].zero_()
     _scratch[key] = ws  # the most recently used stands last
     if len(_scratch) > _MAX_STREAMS:
         del _scratch[next(iter(_scratch))]

@@ -42,7 +42,12 @@ typedef struct ejk_q8_shape {
   int32_t scale_block;   /* tokens that share a scale: a power of two that divides page_size */
 } ejk_q8_shape;
 
-/* Scratch that ejk_q8_attention_launch needs for this static shape on the current device (0: invalid shape). */
+/* The first bytes of an attention workspace: counters that have to be zero when a workspace is used for the first time.  Every
+ * call leaves them zero, one whose waits ran out (EJK_RPA_ST_TIMEOUT) included; the rest needs no initialisation. */
+#define EJK_Q8_TICKET_BYTES 8192
+
+/* Scratch that ejk_q8_attention_launch needs for this static shape on the current device (0: invalid shape).  One workspace
+ * serves any number of calls that are ordered on the device, of any shapes that fit. */
 EJK_RPA_API size_t ejk_q8_workspace_bytes(const ejk_q8_shape* shape);
 
 /* Ragged attention over the 8-bit cache.  Operands, masks, sinks and zero rows as ejk_rpa_launch; `attrs.q_scale` and
