@@ -49,7 +49,7 @@ EXPORTS = (
 )
 
 # declared in include/ejk_q8.h
-Q8_TICKET_BYTES = 8192
+Q8_TICKET_BYTES = 16384
 Q8_EXPORTS = (
     "ejk_q8_workspace_bytes",
     "ejk_q8_attention_launch",

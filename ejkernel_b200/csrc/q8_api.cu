@@ -81,7 +81,7 @@ size_t ejk_q8_workspace_bytes(const ejk_q8_shape* shape) {
   if (!shape || check_attention(*shape) != 0) return 0;
   const int n_sm = sm100_sm_count();
   if (!n_sm) return 0;
-  if (3 * 2 * n_sm * sizeof(int32_t) > EJK_Q8_TICKET_BYTES) return 0;
+  if (kQ8TicketsPerCta * 2 * n_sm * sizeof(int32_t) > EJK_Q8_TICKET_BYTES) return 0;
   return q8_workspace(*shape, n_sm, tiles_possible(*shape)).total;
 }
 
@@ -104,7 +104,7 @@ int ejk_q8_attention_launch(const void* queries, const void* kv_pages, const flo
   if (!aligned16(queries) || !aligned16(kv_pages) || !aligned16(kv_scales) || !aligned16(out)) return EJK_RPA_E_ALIGN;
   const int n_sm = sm100_sm_count();
   if (!n_sm) return EJK_RPA_E_DEVICE;
-  if (3 * 2 * n_sm * sizeof(int32_t) > EJK_Q8_TICKET_BYTES) return EJK_RPA_E_DEVICE;
+  if (kQ8TicketsPerCta * 2 * n_sm * sizeof(int32_t) > EJK_Q8_TICKET_BYTES) return EJK_RPA_E_DEVICE;
   const bool tiles = tiles_possible(s);
   const Q8Workspace W = q8_workspace(s, n_sm, tiles);
   if (workspace_bytes < W.total || (reinterpret_cast<uintptr_t>(workspace) & 255)) return EJK_RPA_E_WORKSPACE;

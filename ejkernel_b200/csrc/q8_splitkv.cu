@@ -11,8 +11,9 @@
 //     straddles a quota boundary is finished by several CTAs; the last of them to arrive combines their parts, in part order,
 //     sixteen at a time.  A CTA has two partial pieces at most, so the parts of all calls fit 2 slots per CTA.
 //   * A stage is 128 tokens of one head, fetched by one producer warp as TMA boxes of up to 64 tokens.  A head's page is
-//     contiguous, so a box of 16 tokens at head_dim 128 is two runs of 2 KB.  The stage's scales come beside it with 4-byte
-//     cp.async copies that arrive on the same mbarrier: no wait of the producer stands between two stages.
+//     contiguous, so a box of 16 tokens at head_dim 128 is two runs of 2 KB.  A second producer warp brings what goes with the
+//     stage: its scales, with 4-byte cp.async copies that arrive on the same mbarrier, and the query rows of a new piece.  (With
+//     one warp for both, its latency per stage, 1.4 us, bounded the kernel.)
 //   * Four consumer warps take 32 tokens each.  Codes go to f16 in registers, which is exact for both types, and both
 //     products run on f16 mma.sync with float32 sums.  8-bit operands would halve the mma work, which is not what bounds
 //     the kernel, and would round q and p to 3 bits of mantissa.  (Eight warps in two teams that take the stages in turn
@@ -38,7 +39,7 @@ namespace ejk {
 namespace {
 
 constexpr int kConsumerWarps = 4;
-constexpr int kThreads = (kConsumerWarps + 1) * 32;
+constexpr int kThreads = (kConsumerWarps + 2) * 32;
 constexpr int kRing = 8;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kMergeInFlight = 8;     // parts whose loads a merge keeps in flight per row
@@ -76,13 +77,8 @@ struct Cfg {
   static constexpr int OFF_SCALE = NS * STAGE_BYTES;              // per stage: TK scales of K, TK of V (at most)
   static constexpr int OFF_Q = OFF_SCALE + NS * 2 * TK * 4;
   static constexpr int OFF_QFAC = OFF_Q + NS * Q_BYTES;           // per stage: 2^-k of each query row
-  static constexpr int OFF_OBUF = OFF_QFAC + NS * RT * 4;
-  static constexpr int OFF_MBUF = OFF_OBUF + RT * D * 4;
-  static constexpr int OFF_LBUF = OFF_MBUF + kConsumerWarps * RT * 4;
-  static constexpr int OFF_ROWSCALE = OFF_LBUF + kConsumerWarps * RT * 4;
-  static constexpr int OFF_ROWM = OFF_ROWSCALE + RT * 4;
-  static constexpr int OFF_ROWL = OFF_ROWM + RT * 4;
-  static constexpr int OFF_RING = (OFF_ROWL + RT * 4 + 63) / 64 * 64;
+  static constexpr int OFF_ML = (OFF_QFAC + NS * RT * 4 + 7) / 8 * 8;  // two pieces' (m, l) of each warp and row
+  static constexpr int OFF_RING = (OFF_ML + 2 * kConsumerWarps * RT * 8 + 63) / 64 * 64;
   static constexpr int OFF_META = OFF_RING + kRing * (int)sizeof(ItemDesc);
   static constexpr int OFF_BAR = OFF_META + NS * 8;  // full[NS], empty[NS], cbar
   static constexpr int OFF_SHARE = OFF_BAR + (2 * NS + 1) * 8;
@@ -90,6 +86,7 @@ struct Cfg {
   static constexpr int SMEM_BYTES = OFF_ABORT + 16 + 1024;  // + alignment slack
   static constexpr int CTAS = SMEM_BYTES <= 112 * 1024 ? 2 : 1;
   static_assert(SMEM_BYTES <= 227 * 1024, "shared memory budget");
+  static_assert(kConsumerWarps * RT * D * 4 <= STAGE_BYTES, "a piece's last stage takes the warps' accumulators");
   static_assert(NT == 2 || D == 256 || CTAS == 2, "two CTAs per SM for the usual shapes");
 };
 
@@ -162,7 +159,7 @@ __device__ __forceinline__ long long seq_stages(const Params& p, const Seq& q, i
 }
 
 // ---- combining the parts of a pair ----
-// Arrival counters, three per CTA, zero between calls: atomicInc with the number of arrivals as its limit takes a counter back to
+// Arrival counters, three per CTA and consumer warp (each merges rows of its own), zero between calls: atomicInc with the number of arrivals as its limit takes a counter back to
 // zero with the last of them.  [c]: the first sixteen parts of the pair that begins in CTA c; [n + c]: the sixteen parts that
 // begin with CTA c's, of a pair that begins earlier; [2n + c]: the groups of the pair that begins in CTA c.
 struct Arrival {
@@ -193,12 +190,7 @@ q8_splitkv_kernel(const __grid_constant__ CUtensorMap tmap, const Params p, cons
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t smem_base = smem_u32(smem);
-  float* obuf = reinterpret_cast<float*>(smem + C::OFF_OBUF);
-  float* mbuf = reinterpret_cast<float*>(smem + C::OFF_MBUF);
-  float* lbuf = reinterpret_cast<float*>(smem + C::OFF_LBUF);
-  float* row_scale = reinterpret_cast<float*>(smem + C::OFF_ROWSCALE);
-  float* row_m = reinterpret_cast<float*>(smem + C::OFF_ROWM);
-  float* row_l = reinterpret_cast<float*>(smem + C::OFF_ROWL);
+  float2* mlbuf = reinterpret_cast<float2*>(smem + C::OFF_ML);
   ItemDesc* ring = reinterpret_cast<ItemDesc*>(smem + C::OFF_RING);
   int2* metas = reinterpret_cast<int2*>(smem + C::OFF_META);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::OFF_ABORT);
@@ -217,7 +209,7 @@ q8_splitkv_kernel(const __grid_constant__ CUtensorMap tmap, const Params p, cons
 
   if (tid == 0) {
     for (int s = 0; s < NS; ++s) {
-      mbar_init(bar_full + s * 8, 1 + 32);  // the announcement, and every producer lane's scale copies
+      mbar_init(bar_full + s * 8, 2 + 32);  // both producers' announcements, and every scale copying lane
       mbar_init(bar_empty + s * 8, kConsumerWarps);
     }
     mbar_init(bar_c, kConsumerWarps);
@@ -241,7 +233,7 @@ q8_splitkv_kernel(const __grid_constant__ CUtensorMap tmap, const Params p, cons
   int quota;
   long long g0, g1;
   {
-    long long* s_sum = reinterpret_cast<long long*>(obuf);  // not in use yet
+    long long* s_sum = reinterpret_cast<long long*>(mlbuf);  // not in use yet
     const int per = (S + kThreads - 1) / kThreads;
     const int a = min(tid * per, S), b = min(a + per, S);
     long long mine = 0;
@@ -286,8 +278,11 @@ q8_splitkv_kernel(const __grid_constant__ CUtensorMap tmap, const Params p, cons
     __syncthreads();
   }
 
-  if (warp == kConsumerWarps) {
-    // =============================== producer warp ===============================
+  if (warp >= kConsumerWarps) {
+    // =============================== producer warps ===============================
+    // Both walk the same pieces and stages.  The first issues the stages' boxes; the second brings their scales and, with the
+    // first stage of a piece, its descriptor and query rows.
+    const bool boxes = warp == kConsumerWarps;
     const int blocks_per_stage = TK >> pb_shift;
     const uint32_t box_bytes = (uint32_t)pb * 2 * D;
     const int scales_per_page = p.page_size >> sb_shift;
@@ -329,10 +324,10 @@ q8_splitkv_kernel(const __grid_constant__ CUtensorMap tmap, const Params p, cons
         // end-of-stream marker for the consumers
         if (!mbar_wait(bar_empty + s * 8, empty_parity, abort_flag, wait_ns)) break;
         if (lane == 0) {
-          metas[s] = make_int2(-1, 0);
+          if (!boxes) metas[s] = make_int2(-1, 0);
           mbar_arrive(bar_full + s * 8);
         }
-        cp_async_arrive(bar_full + s * 8);
+        if (!boxes) cp_async_arrive(bar_full + s * 8);
         ++fills;
         break;
       }
@@ -402,7 +397,7 @@ q8_splitkv_kernel(const __grid_constant__ CUtensorMap tmap, const Params p, cons
         const int off = off_next;
         page_next = page_of(pos + TK, off_next);
         if ((unsigned)page >= (unsigned)p.num_pages) {  // reported, and read as page 0
-          flags |= EJK_RPA_ST_PAGE_ID;
+          if (boxes) flags |= EJK_RPA_ST_PAGE_ID;
           page = 0;
         }
         if (!mbar_wait(bar_empty + s * 8, empty_parity, abort_flag, wait_ns)) {
@@ -412,11 +407,15 @@ q8_splitkv_kernel(const __grid_constant__ CUtensorMap tmap, const Params p, cons
         // test hook: the stage is never announced, the consumers' wait for it must run out
         const bool withhold = (p.test_withhold & 1) && blockIdx.x == 0 && k == 0 && first;
         const uint32_t full = bar_full + s * 8;
-        if (!withhold) {
-          if (lane == 0 && nblk > 0)  // the bytes are expected before the first copy can report them; no arrival yet
-            asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;\n" ::"r"(full), "r"((uint32_t)nblk * box_bytes) : "memory");
+        if (boxes && !withhold) {
+          if (lane == 0) {
+            if (nblk > 0) mbar_arrive_expect_tx(full, (uint32_t)nblk * box_bytes);
+            else mbar_arrive(full);
+          }
           __syncwarp();
           if (lane < nblk) tma_load_5d(smem_base + s * C::STAGE_BYTES + lane * box_bytes, &tmap, full, 0, off, 0, 2 * h, page);
+        }
+        if (!boxes && !withhold) {
           // scales of the blocks that the stage's keys lie in: K's, then V's.  Block e starts at key (e0 + e) << sb_shift, or
           // at the stage's first key; the lane that fetches that key's tokens knows its page
           const int e0 = pos >> sb_shift;
@@ -434,8 +433,8 @@ q8_splitkv_kernel(const __grid_constant__ CUtensorMap tmap, const Params p, cons
             }
           }
         }
-        if (first) {
-          // the item's descriptor and query tile travel with its first stage
+        if (!boxes && first) {
+          // the piece's descriptor and query tile travel with its first stage
           if (lane == 0) {
             ItemDesc d;
             d.u = u;
@@ -484,7 +483,7 @@ q8_splitkv_kernel(const __grid_constant__ CUtensorMap tmap, const Params p, cons
         }
         __syncwarp();  // what the lanes wrote is ordered before the announcement
         ++fills;
-        if (!withhold) {
+        if (!boxes && !withhold) {
           if (lane == 0) {
             metas[s] = make_int2(ring_slot, pos);
             mbar_arrive(full);
@@ -545,7 +544,8 @@ q8_splitkv_kernel(const __grid_constant__ CUtensorMap tmap, const Params p, cons
     float v_norm = 1.f;  // power of two that the V scales are multiplied by
     int s = 0;
     uint32_t full_parity = 0, c_parity = 0;
-    int arrived = 0, owed = 0;  // thread 0: bit 0 / 1 = the CTA's first / another shared piece has been counted; its group not yet
+    int pieces = 0;
+    int arrived = 0, owed = 0;  // bit 0 / 1 = the CTA's first / another shared piece has been counted; its group not yet
 
     auto consumer_sync = [&]() -> bool {
       __syncwarp();
@@ -778,12 +778,12 @@ q8_splitkv_kernel(const __grid_constant__ CUtensorMap tmap, const Params p, cons
           }
         }
       }
-      // this warp is done with the stage's bytes (query fragments are in registers by now)
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar_empty + s * 8);
-
       if (pos + TK >= u.kv_end) {
-        // ---- end of item: combine the four warps ----
+        // ---- end of the piece.  The warps' accumulators meet in the memory of its last stage: with the first barrier every
+        // warp is done with the stage and has published its rows' (m, l), with the second all accumulators are there; from
+        // then on the warps go their own ways, each with its own rows.
+        float2* ml = mlbuf + (pieces & 1) * (kConsumerWarps * RT);  // two, for a warp that is a piece ahead
+        ++pieces;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -792,20 +792,13 @@ q8_splitkv_kernel(const __grid_constant__ CUtensorMap tmap, const Params p, cons
             l += __shfl_xor_sync(0xffffffffu, l, 4);
             l += __shfl_xor_sync(0xffffffffu, l, 8);
             l += __shfl_xor_sync(0xffffffffu, l, 16);
-            if (lane < 4) {
-              const int r = nt * 8 + lane * 2 + j;
-              mbuf[warp * RT + r] = m_run[nt][j];
-              lbuf[warp * RT + r] = l;
-            }
+            if (lane < 4) ml[warp * RT + nt * 8 + lane * 2 + j] = make_float2(m_run[nt][j], l);
           }
         if (!consumer_sync()) break;
-        // Every lane derives the rescale factors of its own rows from the four (m, l) pairs; the
-        // accumulators are then added into obuf in four rounds, warp w handling the d-slice
-        // (w + round) % 4, so each address receives its four contributions in a fixed order and
-        // the result does not depend on warp timing (no floating-point atomics).
-        // (v_back undoes the power of two that this warp took the V scales by)
+        // accumulators relative to the rows' common maximum (v_back undoes the power of two that this warp took the V scales
+        // by).  Row r, head-dim lane d of warp w is at [w][r][d], with d's 16-lane block XORed by r / 2 against bank conflicts
+        float* sum = reinterpret_cast<float*>(smem + s * C::STAGE_BYTES);
         const float v_back = power_of_two_inverse(v_norm);
-        float f_own[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -813,216 +806,144 @@ q8_splitkv_kernel(const __grid_constant__ CUtensorMap tmap, const Params p, cons
             const int r = nt * 8 + (lane & 3) * 2 + j;
             float mt = -INFINITY;
 #pragma unroll
-            for (int w = 0; w < kConsumerWarps; ++w) mt = fmaxf(mt, mbuf[w * RT + r]);
-            const float mu = (mt == -INFINITY) ? 0.f : mt;
-            f_own[nt][j] = fast_exp2(m_run[nt][j] - mu) * v_back;
+            for (int w = 0; w < kConsumerWarps; ++w) mt = fmaxf(mt, ml[w * RT + r].x);
+            const float f = fast_exp2(m_run[nt][j] - ((mt == -INFINITY) ? 0.f : mt)) * v_back;
+            // accumulator rows g / g+8 of block mt are head-dim lanes 16mt + 2g / + 1 (see the V fragments)
+            float* row = sum + (warp * RT + r) * D + (lane >> 2) * 2;
+#pragma unroll
+            for (int mt16 = 0; mt16 < KT; ++mt16)
+              *reinterpret_cast<float2*>(row + (mt16 ^ (lane & 3)) * 16) = make_float2(acc[nt][mt16][j] * f, acc[nt][mt16][j + 2] * f);
           }
-        if (tid < RT) {
-          const int r = tid;
-          float mt = -INFINITY;
+        if (!consumer_sync()) break;
+        constexpr int VPL = D / 32;   // columns per lane
+        constexpr int RPW = RT / kConsumerWarps;  // rows per warp: warp, warp + 4, ...
+        T* out = reinterpret_cast<T*>(p.out);
+        auto store_row = [&](int r, float m_tot, float l_tot, const float (&o)[VPL]) {
+          const int R = u.row0 + r;
+          const int qt = R / G, gq = R - qt * G;
+          const int hq = h * G + gq;
+          float scl = 1.f, l_fin = l_tot;
+          if (p.num_sinks > 0) {
+            // attention sinks join the denominator only
+            const int srow = (p.sink_rows == p.Hq) ? hq : (p.sink_rows == Hkv ? h : 0);
+            const float* sk = p.sinks + (size_t)srow * p.num_sinks;
+            float sm = -INFINITY;
+            for (int i = 0; i < p.num_sinks; ++i) sm = fmaxf(sm, sk[i] * kLog2e);
+            const float m_fin = fmaxf(m_tot, sm);
+            const float mf = (m_fin == -INFINITY) ? 0.f : m_fin;
+            scl = fast_exp2(m_tot - mf);
+            l_fin = l_tot * scl;
+            for (int i = 0; i < p.num_sinks; ++i) l_fin += fast_exp2(sk[i] * kLog2e - mf);
+          }
+          scl = (l_fin > 0.f) ? scl / l_fin : 0.f;
+          uint32_t* dst = reinterpret_cast<uint32_t*>(out + ((size_t)(u.q_start + qt) * p.Hq + hq) * D + lane * VPL);
 #pragma unroll
-          for (int w = 0; w < kConsumerWarps; ++w) mt = fmaxf(mt, mbuf[w * RT + r]);
-          const float mu = (mt == -INFINITY) ? 0.f : mt;
-          float lt = 0.f;
+          for (int i = 0; i < VPL; i += 2) dst[i / 2] = Mma<T>::pack(o[i] * scl, o[i + 1] * scl);
+        };
+        auto store_part = [&](int slot, int r, float m_tot, float l_tot, const float (&o)[VPL]) {
+          float* dst = p.part_o + ((size_t)slot * RT + r) * D + lane * VPL;
 #pragma unroll
-          for (int w = 0; w < kConsumerWarps; ++w) lt += lbuf[w * RT + r] * fast_exp2(mbuf[w * RT + r] - mu);
-          float scl = 1.f;
-          if (u.slot < 0) {
-            float l_fin = lt;
-            if (p.num_sinks > 0 && r < n_rows) {
-              // attention sinks join the denominator only
-              const int R = u.row0 + r;
-              const int hq = h * G + (R % G);
-              const int srow = (p.sink_rows == p.Hq) ? hq : (p.sink_rows == Hkv ? h : 0);
-              const float* sk = p.sinks + (size_t)srow * p.num_sinks;
-              float sm = -INFINITY;
-              for (int i = 0; i < p.num_sinks; ++i) sm = fmaxf(sm, sk[i] * kLog2e);
-              const float m_fin = fmaxf(mt, sm);
-              const float mf = (m_fin == -INFINITY) ? 0.f : m_fin;
-              scl = fast_exp2(mt - mf);
-              l_fin = lt * scl;
-              for (int i = 0; i < p.num_sinks; ++i) l_fin += fast_exp2(sk[i] * kLog2e - mf);
+          for (int i = 0; i < VPL; i += 2) *reinterpret_cast<float2*>(dst + i) = make_float2(o[i], o[i + 1]);
+          if (lane == 0) p.part_ml[(size_t)slot * RT + r] = make_float2(m_tot, l_tot);
+        };
+#pragma unroll
+        for (int ri = 0; ri < RPW; ++ri) {
+          const int r = warp + ri * kConsumerWarps;
+          float m_tot = -INFINITY, l_tot = 0.f;
+#pragma unroll
+          for (int w = 0; w < kConsumerWarps; ++w) m_tot = fmaxf(m_tot, ml[w * RT + r].x);
+          const float mu = (m_tot == -INFINITY) ? 0.f : m_tot;
+#pragma unroll
+          for (int w = 0; w < kConsumerWarps; ++w) l_tot += ml[w * RT + r].y * fast_exp2(ml[w * RT + r].x - mu);
+          const int col = lane * VPL;
+          const float* src = sum + r * D + (((col >> 4) ^ ((r >> 1) & 3)) << 4) + (col & 15);
+          float o[VPL];
+#pragma unroll
+          for (int i = 0; i < VPL; ++i) o[i] = 0.f;
+#pragma unroll
+          for (int w = 0; w < kConsumerWarps; ++w)
+#pragma unroll
+            for (int i = 0; i < VPL; i += 2) {
+              const float2 v = *reinterpret_cast<const float2*>(src + w * RT * D + i);
+              o[i] += v.x;
+              o[i + 1] += v.y;
             }
-            scl = (l_fin > 0.f) ? scl / l_fin : 0.f;
-          }
-          row_scale[r] = scl;
-          row_m[r] = mt;
-          row_l[r] = lt;
+          if (r >= n_rows) continue;
+          if (u.slot < 0) store_row(r, m_tot, l_tot, o);
+          else store_part(u.slot, r, m_tot, l_tot, o);
         }
-        bool alive_c = true;
-#pragma unroll
-        for (int round = 0; round < kConsumerWarps; ++round) {
-          const int slice = (warp + round) % kConsumerWarps;
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            const int r0 = nt * 8 + (lane & 3) * 2;
-            const float f0 = f_own[nt][0], f1 = f_own[nt][1];
-#pragma unroll
-            for (int mi = 0; mi < KT / kConsumerWarps; ++mi) {
-              // compile-time accumulator index in every branch keeps acc[] in registers
-#pragma unroll
-              for (int sl = 0; sl < kConsumerWarps; ++sl) {
-                if (sl == slice) {
-                  const int mt = sl * (KT / kConsumerWarps) + mi;
-                  // accumulator rows g / g+8 of block mt are head-dim lanes 16mt + 2g / + 1 (see the V fragments)
-                  constexpr int HI = 1;
-                  const int d = mt * 16 + (lane >> 2) * 2;
-                  float* o0 = &obuf[r0 * D + d];
-                  float* o1 = &obuf[(r0 + 1) * D + d];
-                  if (round == 0) {
-                    o0[0] = acc[nt][mt][0] * f0;
-                    o0[HI] = acc[nt][mt][2] * f0;
-                    o1[0] = acc[nt][mt][1] * f1;
-                    o1[HI] = acc[nt][mt][3] * f1;
-                  } else {
-                    o0[0] += acc[nt][mt][0] * f0;
-                    o0[HI] += acc[nt][mt][2] * f0;
-                    o1[0] += acc[nt][mt][1] * f1;
-                    o1[HI] += acc[nt][mt][3] * f1;
-                  }
-                }
-              }
-            }
-          }
-          if (!consumer_sync()) {
-            alive_c = false;
-            break;
-          }
-        }
-        if (!alive_c) break;
-        constexpr int kCT = kConsumerWarps * 32;
-        if (u.slot < 0) {
-          T* out = reinterpret_cast<T*>(p.out);
-          for (int i = tid; i < n_rows * (D / 2); i += kCT) {
-            const int r = i / (D / 2), d = (i % (D / 2)) * 2;
-            const int R = u.row0 + r;
-            const int qt = R / G, g = R - qt * G;
-            const float scl = row_scale[r];
-            const float2 v = *reinterpret_cast<float2*>(&obuf[r * D + d]);
-            *reinterpret_cast<uint32_t*>(out + ((size_t)(u.q_start + qt) * p.Hq + h * G + g) * D + d) =
-                  Mma<T>::pack(v.x * scl, v.y * scl);
-          }
-        } else {
-          float* po = p.part_o + (size_t)u.slot * RT * D;
-          float2* pml = p.part_ml + (size_t)u.slot * RT;
-          for (int i = tid; i < n_rows * (D / 4); i += kCT) {
-            const int r = i / (D / 4), d = (i % (D / 4)) * 4;
-            const float4 v = *reinterpret_cast<float4*>(&obuf[r * D + d]);
-            *reinterpret_cast<float4*>(po + r * D + d) = v;
-          }
-          if (tid < n_rows) pml[tid] = make_float2(row_m[tid], row_l[tid]);
-          // Last-arriver merge: publish this part, take a ticket; whoever draws the last one combines the parts, in part
-          // order, so that the result does not depend on who that is.  No CTA ever waits for another.
-          const int c0 = u.merge_idx;
+        // the stage can go back (its memory was written by ordinary stores, the next box comes through the async proxy)
+        asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_empty + s * 8);
+        if (u.slot >= 0) {
+          // Last-arriver merge of this warp's rows: publish the part, take a ticket; whoever draws the last one combines the
+          // parts, in part order, so that the result does not depend on who that is.  Nobody ever waits for another CTA.
+          const int c0 = u.merge_idx, bit = first_piece ? 1 : 2;
+          int* tickets = p.tickets + warp * 3 * n_cta;
           bool groups = false;
-          bool ok = true;
           while (true) {
             __threadfence();
-            if (!(ok = consumer_sync())) break;
-            if (tid == 0) {
-              const Arrival a = groups ? arrive_group(p.tickets, n_cta, c0, u.n_chunks)
-                                       : arrive_part(p.tickets, n_cta, c0, u.chunk_idx, u.n_chunks);
-              // row_l was consumed above
-              row_l[0] = __int_as_float(a.count);
-              row_l[1] = __int_as_float(a.stride);
-              row_l[2] = __int_as_float(a.part0);
-              row_l[3] = __int_as_float(a.last);
-              const int bit = first_piece ? 1 : 2;
-              arrived |= bit;
-              owed = a.count && !a.last ? owed | bit : owed & ~bit;
-            }
-            if (!(ok = consumer_sync())) break;
-            const int count = __float_as_int(row_l[0]), stride = __float_as_int(row_l[1]), part0 = __float_as_int(row_l[2]);
-            const bool last = __float_as_int(row_l[3]) != 0;
+            __syncwarp();
+            Arrival a = {0, 0, 0, true};
+            if (lane == 0) a = groups ? arrive_group(tickets, n_cta, c0, u.n_chunks) : arrive_part(tickets, n_cta, c0, u.chunk_idx, u.n_chunks);
+            const int count = __shfl_sync(0xffffffffu, a.count, 0), stride = __shfl_sync(0xffffffffu, a.stride, 0);
+            const int part0 = __shfl_sync(0xffffffffu, a.part0, 0);
+            const bool last = __shfl_sync(0xffffffffu, (int)a.last, 0) != 0;
+            arrived |= bit;
+            owed = count && !last ? owed | bit : owed & ~bit;
             if (count == 0) break;
             __threadfence();
-            constexpr int VPL = D / 32;
-            T* out = reinterpret_cast<T*>(p.out);
             auto slot_of = [&](int i) {
               const int part = part0 + i * stride;
               return part == 0 ? u.pad : 2 * (c0 + part);
             };
+#pragma unroll 1
             for (int r = warp; r < n_rows; r += kConsumerWarps) {
               // lane i holds part i's maximum and sum (count <= 32)
-              const float2 ml = lane < count ? __ldcg(&p.part_ml[(size_t)slot_of(lane) * RT + r]) : make_float2(-INFINITY, 0.f);
-              float m_tot = ml.x;
+              const float2 mlp = lane < count ? __ldcg(&p.part_ml[(size_t)slot_of(lane) * RT + r]) : make_float2(-INFINITY, 0.f);
+              float m_tot = mlp.x;
 #pragma unroll
               for (int o = 16; o > 0; o >>= 1) m_tot = fmaxf(m_tot, __shfl_xor_sync(0xffffffffu, m_tot, o));
               const float mu = (m_tot == -INFINITY) ? 0.f : m_tot;
-              const float f_mine = fast_exp2(ml.x - mu);
-              float l_tot = ml.y * f_mine;
+              const float f_mine = fast_exp2(mlp.x - mu);
+              float l_tot = mlp.y * f_mine;
 #pragma unroll
               for (int o = 16; o > 0; o >>= 1) l_tot += __shfl_xor_sync(0xffffffffu, l_tot, o);
-              float accm[VPL];
+              float o[VPL];
 #pragma unroll
-              for (int i = 0; i < VPL; ++i) accm[i] = 0.f;
+              for (int i = 0; i < VPL; ++i) o[i] = 0.f;
               for (int i0 = 0; i0 < count; i0 += kMergeInFlight) {
-                float vv[kMergeInFlight][VPL];
+                float2 v[kMergeInFlight][VPL / 2];
 #pragma unroll
                 for (int j = 0; j < kMergeInFlight; ++j) {
                   const float* src = p.part_o + ((size_t)slot_of(min(i0 + j, count - 1)) * RT + r) * D + lane * VPL;
-                  if constexpr (VPL == 2) {
-                    const float2 v = __ldcg(reinterpret_cast<const float2*>(src));
-                    vv[j][0] = v.x;
-                    vv[j][1] = v.y;
-                  } else {
 #pragma unroll
-                    for (int i = 0; i < VPL; i += 4) {
-                      const float4 v = __ldcg(reinterpret_cast<const float4*>(src + i));
-                      vv[j][i] = v.x;
-                      vv[j][i + 1] = v.y;
-                      vv[j][i + 2] = v.z;
-                      vv[j][i + 3] = v.w;
-                    }
-                  }
+                  for (int i = 0; i < VPL / 2; ++i) v[j][i] = __ldcg(reinterpret_cast<const float2*>(src) + i);
                 }
 #pragma unroll
                 for (int j = 0; j < kMergeInFlight; ++j) {
                   const float f = __shfl_sync(0xffffffffu, f_mine, min(i0 + j, 31));
                   if (i0 + j < count) {
 #pragma unroll
-                    for (int i = 0; i < VPL; ++i) accm[i] += vv[j][i] * f;
+                    for (int i = 0; i < VPL / 2; ++i) {
+                      o[2 * i] += v[j][i].x * f;
+                      o[2 * i + 1] += v[j][i].y * f;
+                    }
                   }
                 }
               }
-              if (!last) {
-                // a group: its sum takes the place of its first part
-                float* dst = p.part_o + ((size_t)slot_of(0) * RT + r) * D + lane * VPL;
-#pragma unroll
-                for (int i = 0; i < VPL; i += 2) *reinterpret_cast<float2*>(dst + i) = make_float2(accm[i], accm[i + 1]);
-                if (lane == 0) p.part_ml[(size_t)slot_of(0) * RT + r] = make_float2(m_tot, l_tot);
-                continue;
-              }
-              const int R = u.row0 + r;
-              const int qt = R / G, g = R - qt * G;
-              const int hq = h * G + g;
-              float scl = 1.f, l_fin = l_tot;
-              if (p.num_sinks > 0) {
-                const int srow = (p.sink_rows == p.Hq) ? hq : (p.sink_rows == Hkv ? h : 0);
-                const float* sk = p.sinks + (size_t)srow * p.num_sinks;
-                float sm = -INFINITY;
-                for (int i = 0; i < p.num_sinks; ++i) sm = fmaxf(sm, sk[i] * kLog2e);
-                const float m_fin = fmaxf(m_tot, sm);
-                const float mf = (m_fin == -INFINITY) ? 0.f : m_fin;
-                scl = fast_exp2(m_tot - mf);
-                l_fin = l_tot * scl;
-                for (int i = 0; i < p.num_sinks; ++i) l_fin += fast_exp2(sk[i] * kLog2e - mf);
-              }
-              scl = (l_fin > 0.f) ? scl / l_fin : 0.f;
-              T* dst = out + ((size_t)(u.q_start + qt) * p.Hq + hq) * D + lane * VPL;
-#pragma unroll
-              for (int i = 0; i < VPL; i += 2)
-                *reinterpret_cast<uint32_t*>(dst + i) = Mma<T>::pack(accm[i] * scl, accm[i + 1] * scl);
+              if (last) store_row(r, m_tot, l_tot, o);
+              else store_part(slot_of(0), r, m_tot, l_tot, o);  // a group: its sum takes the place of its first part
             }
             if (last) break;
             groups = true;
           }
-          if (!ok) break;
         }
-        // The next item's writes to mbuf/lbuf come before its first consumer_sync, but they only
-        // race with readers of mbuf/lbuf, and those finished before the first combine step's sync above; its
-        // writes to obuf/row_* come after its first consumer_sync, which every warp reaches only
-        // after finishing the loops above.
+      } else {
+        // this warp is done with the stage's bytes (query fragments are in registers by now)
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_empty + s * 8);
       }
       if (++s == NS) {
         s = 0;
@@ -1030,7 +951,7 @@ q8_splitkv_kernel(const __grid_constant__ CUtensorMap tmap, const Params p, cons
       }
     }
     if (*abort_flag) flags |= EJK_RPA_ST_TIMEOUT;
-    if (*abort_flag && tid == 0 && g0 < g1) {
+    if (*abort_flag && lane == 0 && g0 < g1) {
       // Giving up: the shared pieces that were not counted are counted now, with no data, so that the counters are zero again
       // after the call (the outputs are invalid, which the status says).
       for (int e = 0; e < 2; ++e) {
@@ -1050,10 +971,10 @@ q8_splitkv_kernel(const __grid_constant__ CUtensorMap tmap, const Params p, cons
         if (c0 == c1) continue;
         bool group_next = (owed & bit) != 0;
         if (!(arrived & bit)) {
-          const Arrival a = arrive_part(p.tickets, n_cta, c0, (int)blockIdx.x - c0, c1 - c0 + 1);
+          const Arrival a = arrive_part(p.tickets + warp * 3 * n_cta, n_cta, c0, (int)blockIdx.x - c0, c1 - c0 + 1);
           group_next = a.count && !a.last;
         }
-        if (group_next) arrive_group(p.tickets, n_cta, c0, c1 - c0 + 1);
+        if (group_next) arrive_group(p.tickets + warp * 3 * n_cta, n_cta, c0, c1 - c0 + 1);
         arrived |= bit;
         owed &= ~bit;
       }

@@ -119,6 +119,7 @@ void set_last_launches(int n);
 
 // launchers
 cudaError_t launch_q8_gather(const Params& p, const Q8Cache& c, int dtype, int code, cudaStream_t stream);
+constexpr int kQ8TicketsPerCta = 12;  // arrival counters of the split-KV kernel: 3 per consumer warp
 // the pipelined kernel: page sizes that are multiples of 8
 bool q8_tma_supported(int page_size);
 cudaError_t q8_tensor_map(CUtensorMap* map, const Q8Cache& c, int box_tokens);

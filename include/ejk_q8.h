@@ -44,7 +44,7 @@ typedef struct ejk_q8_shape {
 
 /* The first bytes of an attention workspace: counters that have to be zero when a workspace is used for the first time.  Every
  * call leaves them zero, one whose waits ran out (EJK_RPA_ST_TIMEOUT) included; the rest needs no initialisation. */
-#define EJK_Q8_TICKET_BYTES 8192
+#define EJK_Q8_TICKET_BYTES 16384
 
 /* Scratch that ejk_q8_attention_launch needs for this static shape on the current device (0: invalid shape).  One workspace
  * serves any number of calls that are ordered on the device, of any shapes that fit. */
