@@ -481,3 +481,176 @@ def test_tables_that_cannot_be_served():
     r["num_seqs"] = 0
     check_tables(r, 16, 5)
     check_tables(make_requests([0, 0], [5, 40], page=16, pps=8, seed=9, done=[1]), 16, 0)
+
+
+# ------------------------------------------------------------------------------------------ together, as they are used
+
+
+class Loop:
+    """A serving loop's state: requests come, decode and go; the plain twin keeps every token's K and V in float64 rows of the
+    cache, through the oracle's write."""
+
+    def __init__(self, code, half, *, rows=6, pages=64, page=16, block=16, Hq=4, Hkv=2, dim=64, seed=0):
+        self.g = torch.Generator().manual_seed(seed)
+        self.code, self.half, self.page, self.Hq, self.Hkv, self.dim, self.rows = code, half, page, Hq, Hkv, dim, rows
+        self.kv, self.scales = ej.modules.operations.allocate_quantized_kv(pages, Hkv, page, dim, dtype=code, scale_block=block)
+        self.tables = torch.full((rows, 32), -1, dtype=torch.int32, device="cuda")  # 512 tokens: the longest request gets 420
+        self.free = torch.randperm(pages, generator=self.g).to(torch.int32).cuda()
+        self.num_free = torch.tensor([pages], dtype=torch.int32, device="cuda")
+        self.lens = torch.zeros(rows, dtype=torch.int32, device="cuda")
+        self.n = torch.tensor([rows], dtype=torch.int32, device="cuda")
+        self.cpu = dict(kv=self.kv.cpu(), scales=self.scales.cpu(), tables=self.tables.cpu(), free=self.free.cpu(), num_free=pages, lens=self.lens.cpu())
+
+    def inputs(self, q, tokens):
+        r = lambda h: torch.randn((tokens, h, self.dim), generator=self.g).to(self.half)  # noqa: E731
+        return dict(q=torch.tensor(q, dtype=torch.int32), x=r(self.Hq), k=r(self.Hkv) * float(2.0 ** int(torch.randint(-4, 5, (1,), generator=self.g))), v=r(self.Hkv))
+
+    def step(self, i, done=None):
+        lens, start, slots, num_free = ej.build_page_tables(i["q"], self.lens, self.tables, self.free, self.num_free, self.n, page_size=self.page,
+                                                            total_tokens=i["x"].shape[0], finished=done)
+        ej.quantized_kv_write(i["k"], i["v"], self.kv, self.scales, slots)
+        out = ej.quantized_ragged_page_attention(i["x"], self.kv, self.scales, lens, self.tables, start, self.n)
+        self.lens.copy_(lens)
+        self.num_free.copy_(num_free)
+        return out, start
+
+    def plain(self, i, done=None):
+        c = self.cpu
+        lens, start, slots, c["num_free"], tables, free = q8_oracle.page_tables(i["q"], c["lens"], c["tables"], c["free"], c["num_free"], self.rows, self.page, i["x"].shape[0], done)
+        c["lens"], c["tables"], c["free"] = torch.tensor(lens, dtype=torch.int32), torch.from_numpy(tables), torch.from_numpy(free)
+        codes, scales = q8_oracle.write(i["k"], i["v"], c["kv"], c["scales"], torch.tensor(slots, dtype=torch.int32))
+        c["kv"], c["scales"] = torch.from_numpy(codes).float().to(self.code), torch.from_numpy(scales).float()
+        return dict(q=i["x"], codes=c["kv"], scales=c["scales"], ctx=c["lens"], tab=c["tables"], start=torch.tensor(start, dtype=torch.int32), n=self.rows)
+
+
+STEPS = [([40, 1, 0, 130, 7, 3], ()), ([1, 1, 20, 1, 1, 1], ()), ([1, 1, 1, 1, 0, 1], (4,)), ([1, 17, 1, 0, 9, 1], (3,)), ([1, 1, 1, 1, 1, 1], ())]
+
+
+@pytest.mark.parametrize("code, half", [(torch.int8, torch.bfloat16), (torch.float8_e4m3fn, torch.float16)])
+def test_a_serving_loop_of_the_operators(code, half):
+    loop = Loop(code, half)
+    for q, gone in STEPS:
+        i = loop.inputs(q, sum(q) + 5)
+        done = torch.zeros(loop.rows, dtype=torch.bool)
+        done[list(gone)] = True
+        c = {k: v.cuda() for k, v in i.items()}
+        out, _ = loop.step(c, done.cuda())
+        b = loop.plain(i, done)
+        check(b, out)
+        assert torch.equal(loop.lens.cpu(), loop.cpu["lens"]) and torch.equal(loop.tables.cpu(), loop.cpu["tables"])
+        assert np.array_equal(loop.kv.cpu().float().numpy(), loop.cpu["kv"].float().numpy())
+
+
+@pytest.mark.parametrize("tokens", [6, 200])
+def test_a_step_is_captured_and_replayed(tokens):
+    """One graph per batch shape, replayed on new inputs; two graphs of the same operators, in turn, and eager calls between."""
+    loop = Loop(torch.int8, torch.bfloat16, pages=200, seed=3)
+    first = loop.inputs([20, 1, 5, 2, 70, 3], 101)
+    eager, _ = loop.step({k: v.cuda() for k, v in first.items()})
+    check(loop.plain(first), eager)
+    q = [1] * 6 if tokens == 6 else [100, 1, 1, 64, 30, 1]
+    static = {k: v.cuda() for k, v in loop.inputs(q, tokens).items()}
+    keep = [t.clone() for t in (loop.kv, loop.scales, loop.tables, loop.free, loop.num_free, loop.lens)]
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out, _ = loop.step(static)
+        graphs.append((graph, out))
+    for t, k in zip((loop.kv, loop.scales, loop.tables, loop.free, loop.num_free, loop.lens), keep):
+        assert torch.equal(t.view(torch.uint8) if t.dtype == torch.int8 else t, k.view(torch.uint8) if k.dtype == torch.int8 else k)  # capturing runs nothing
+    for turn in range(4):
+        i = loop.inputs(q, tokens)
+        for k, v in i.items():
+            static[k].copy_(v)
+        graph, out = graphs[turn % 2]
+        graph.replay()
+        b = loop.plain(i)
+        check(b, out)
+        again = ej.quantized_ragged_page_attention(static["x"], loop.kv, loop.scales, loop.lens, loop.tables, b["start"].cuda(), loop.n)
+        assert torch.equal(again, out)
+
+
+def test_two_streams_at_once():
+    """Each stream has its own scratch: calls that overlap on the device do not disturb one another."""
+    batches = [make_batch([(1, 9000 + 100 * s), (1, 400), (40, 700)], Hq=8, Hkv=1, dim=128, page=16, block=16, code=CODES[s], half=torch.bfloat16, seed=20 + s) for s in range(2)]
+    gpu = [{k: v.cuda() if isinstance(v, torch.Tensor) else v for k, v in b.items()} for b in batches]
+    alone = [run(b) for b in gpu]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    outs = [[], []]
+    for _ in range(10):
+        for s, (stream, b) in enumerate(zip(streams, gpu)):
+            with torch.cuda.stream(stream):
+                outs[s].append(run(b))
+    torch.cuda.synchronize()
+    for s in range(2):
+        check(batches[s], alone[s])
+        assert all(torch.equal(o, alone[s]) for o in outs[s])
+
+
+def test_results_do_not_depend_on_the_run():
+    """No atomics on values: the parts of a row are combined in a fixed order."""
+    b = make_batch([(1, 20000), (1, 777), (3, 6000), (200, 900)], Hq=8, Hkv=2, dim=64, page=16, block=16, code=torch.int8, half=torch.float16, seed=30)
+    gpu = {k: v.cuda() if isinstance(v, torch.Tensor) else v for k, v in b.items()}
+    outs = [run(gpu) for _ in range(6)]
+    assert all(torch.equal(o, outs[0]) for o in outs)
+
+
+def test_workspace_counters_are_zero_after_every_call(option):
+    from ejkernel_b200.kernels._cuda.quantized_kv import _interface
+
+    b = make_batch([(1, 20000), (1, 50), (2, 3000)], Hq=8, Hkv=1, dim=128, page=16, block=16, code=torch.int8, half=torch.bfloat16, seed=31)
+    good = run(b)
+    counters = lambda: [int(torch.count_nonzero(w[: _cabi.Q8_TICKET_BYTES])) for w in _interface._scratch.values()]  # noqa: E731
+    assert counters() and not any(counters())
+    option("wait_ms", 5)
+    option("test_withhold", 1)
+    run(b)
+    assert read_status() & _cabi.ST_TIMEOUT and not any(counters())
+    option("test_withhold", 0)
+    option("wait_ms", 2000)
+    assert torch.equal(run(b), good)
+
+
+@pytest.mark.parametrize("name, value", [("path", 1), ("overlap", 0), ("min_chunk", 64), ("min_chunk", 4096), ("prefill_rows", 0), ("prefill_rows", 1)])
+def test_options(option, name, value):
+    b = make_batch([(1, 2000), (5, 300), (70, 300), (1, 1)], Hq=8, Hkv=2, dim=128, page=16, block=4, code=torch.float8_e4m3fn, half=torch.bfloat16, seed=32)
+    option(name, value)
+    check(b, run(b))
+
+
+def test_a_cache_beyond_32_bit_offsets():
+    """Pages whose bytes lie past 2^32, codes and scales of several gigabytes."""
+    pages, heads, page, dim = 36000, 8, 32, 256
+    kv = torch.zeros((pages, heads, 2, page, dim), dtype=torch.int8, device="cuda")
+    scales = torch.ones((pages, heads, 2, page), dtype=torch.float32, device="cuda")
+    assert kv.numel() > 2**32
+    g = torch.Generator().manual_seed(40)
+    lens = [(1, 100), (3, 40), (64, 64)]
+    b = make_batch(lens, Hq=16, Hkv=heads, dim=dim, page=page, block=1, code=torch.int8, half=torch.bfloat16, seed=41, spare=0)
+    far = pages - 1 - torch.arange(b["codes"].shape[0])
+    kv[far.cuda()], scales[far.cuda()] = b["codes"].cuda(), b["scales"].cuda()
+    tab = torch.where(b["tab"] >= 0, far.to(torch.int32)[b["tab"].clamp(min=0).long()], -1)
+    out = ej.quantized_ragged_page_attention(b["q"].cuda(), kv, scales, b["ctx"].cuda(), tab.cuda(), b["start"].cuda(), b["n"])
+    check(b, out)
+    x = torch.randn((5, heads, dim), generator=g).to(torch.float16)
+    slots = torch.arange(far[0] * page + 3, far[0] * page + 8, dtype=torch.int32)
+    ej.quantized_kv_write(x.cuda(), x.cuda(), kv, scales, slots.cuda())
+    k, v = ej.quantized_kv_read(kv, scales, slots.cuda(), dtype=torch.float16)
+    step = x.float().abs().amax(-1, keepdim=True) / 63  # a scale is above amax / 127 / 2 ... amax / 127
+    assert bool(((k.cpu().float() - x.float()).abs() <= step * 0.51).all()) and torch.equal(k, v)
+
+
+def test_misaligned_views_are_refused():
+    kv, scales = ej.modules.operations.allocate_quantized_kv(2, 1, 16, 64, dtype=torch.int8)
+    flat = torch.zeros(2 * 64 + 8, dtype=torch.bfloat16, device="cuda")
+    x = flat[4: 4 + 128].view(2, 1, 64)
+    slots = torch.tensor([0, 1], dtype=torch.int32, device="cuda")
+    with pytest.raises(_cabi.RpaLibraryError, match="aligned"):
+        ej.quantized_kv_write(x, x, kv, scales, slots)
+    i = torch.zeros(4, dtype=torch.int32, device="cuda")
+    with pytest.raises(_cabi.RpaLibraryError, match="aligned"):
+        ej.quantized_ragged_page_attention(x, kv, scales, i[:1], i[:1].view(1, 1), i[:2], 1)
+    with pytest.raises(ValueError, match="is on"):
+        ej.quantized_kv_write(x.contiguous(), x, kv.cpu(), scales, slots)
