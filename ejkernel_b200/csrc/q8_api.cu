@@ -49,19 +49,35 @@ int check_attention(const ejk_q8_shape& s) {
   return check_rpa_shape(as_rpa(s));
 }
 
-// The workspace: the split-KV kernel's arrival counters, which are zero between calls, its parts, and behind them what the
-// planner of the tensor tiles needs.
+// The workspace: the split-KV kernel's arrival counters, which are zero between calls, and its parts; where the batch can hold
+// tensor tiles, their work list and the parts of items that are cut along KV (two tiles of 128 rows, two parts per CTA).
 struct Q8Workspace {
-  size_t part_ml_off, part_o_off, tiles_off, total;
+  size_t part_ml_off, part_o_off, header_off, items_off, prefix_off, item_tickets_off, item_ml_off, item_o_off, total;
+  int max_items;
 };
 Q8Workspace q8_workspace(const ejk_q8_shape& s, int n_sm, bool with_tiles) {
-  const size_t rt = s.num_q_heads / s.num_kv_heads > 8 ? 16 : 8, slots = 2 * 2 * (size_t)n_sm;
-  auto up = [](size_t x) { return (x + 255) / 256 * 256; };
+  const int G = s.num_q_heads / s.num_kv_heads;
+  const size_t rt = G > 8 ? 16 : 8, slots = 2 * 2 * (size_t)n_sm;
   Q8Workspace w;
-  w.part_ml_off = EJK_Q8_TICKET_BYTES;
-  w.part_o_off = up(w.part_ml_off + slots * rt * sizeof(float2));
-  w.tiles_off = up(w.part_o_off + slots * rt * s.head_dim * sizeof(float));
-  w.total = w.tiles_off + (with_tiles ? workspace_layout(as_rpa(s), n_sm).total_split : 0);
+  size_t off = EJK_Q8_TICKET_BYTES;
+  auto take = [&](size_t bytes) {
+    const size_t at = off;
+    off = (off + bytes + 255) / 256 * 256;
+    return at;
+  };
+  w.part_ml_off = take(slots * rt * sizeof(float2));
+  w.part_o_off = take(slots * rt * s.head_dim * sizeof(float));
+  if (with_tiles) {
+    w.max_items = (int)((long long)s.total_tokens * G / kPrefillRows + s.max_num_seqs);
+    const size_t rows = 2 * (size_t)n_sm * 2 * kPrefillRows;
+    w.header_off = take(kHdrWords * sizeof(int32_t));
+    w.items_off = take((size_t)w.max_items * sizeof(Unit));
+    w.prefix_off = take(((size_t)w.max_items + 1) * sizeof(int32_t));
+    w.item_tickets_off = take((size_t)w.max_items * s.num_kv_heads * 2 * 4 * sizeof(int32_t));
+    w.item_ml_off = take(rows * sizeof(float2));
+    w.item_o_off = take(rows * s.head_dim * sizeof(float));
+  }
+  w.total = off;
   return w;
 }
 // can the batch hold a sequence of several tokens, for the tensor tiles?
@@ -181,25 +197,15 @@ int ejk_q8_attention_launch(const void* queries, const void* kv_pages, const flo
   p.prefill_min_rows = use_prefill ? prefill_rows : 0;
   p.prefill_share = opt.prefill_share;
   if (use_prefill) {
-    const WorkspaceLayout L = workspace_layout(as_rpa(s), n_sm);
-    uint8_t* wt = ws + W.tiles_off;
-    p.header = reinterpret_cast<int32_t*>(wt + L.header_off);
-    p.units = reinterpret_cast<Unit*>(wt + L.units_off);
-    p.punits = reinterpret_cast<Unit*>(wt + L.punits_off);
-    p.merge = reinterpret_cast<MergeItem*>(wt + L.merge_off);
-    p.max_units = L.max_units;
-    p.max_merge = L.max_merge;
-    p.max_slots = L.max_slots;
-    p.max_punits = L.max_punits;
-    p.target_units = L.target_units;
-    p.target_units_max = L.target_units_max;
-    p.sort_items = opt.sort_items;
-    p.prefill_item_rows = prefill_rows_per_item(s.head_dim);
+    p.header = reinterpret_cast<int32_t*>(ws + W.header_off);
+    p.punits = reinterpret_cast<Unit*>(ws + W.items_off);
+    p.max_punits = W.max_items;
+    p.prefill_item_rows = 2 * kPrefillRows;
     if (opt.prefill_split) {
-      p.pprefix = reinterpret_cast<int32_t*>(wt + L.pprefix_off);
-      p.ptickets = reinterpret_cast<int32_t*>(wt + L.ptickets_off);
-      p.ppart_ml = reinterpret_cast<float2*>(wt + L.ppart_ml_off);
-      p.ppart_o = reinterpret_cast<float*>(wt + L.ppart_o_off);
+      p.pprefix = reinterpret_cast<int32_t*>(ws + W.prefix_off);
+      p.ptickets = reinterpret_cast<int32_t*>(ws + W.item_tickets_off);
+      p.ppart_ml = reinterpret_cast<float2*>(ws + W.item_ml_off);
+      p.ppart_o = reinterpret_cast<float*>(ws + W.item_o_off);
       p.prefill_split = opt.prefill_split;
     }
   }
@@ -210,9 +216,7 @@ int ejk_q8_attention_launch(const void* queries, const void* kv_pages, const flo
   int launches = 0;
   cudaError_t e;
   if (use_prefill) {
-    Params plan = p;  // the planner clears counters of its own
-    plan.tickets = reinterpret_cast<int32_t*>(ws + W.tiles_off + workspace_layout(as_rpa(s), n_sm).tickets_off);
-    e = launch_plan(plan, st, pdl);
+    e = launch_q8_plan(p, n_sm, st, pdl);
     if (e != cudaSuccess) return static_cast<int>(e);
     e = launch_q8_prefill(p, c, s.dtype, s.code_dtype, n_sm, st, pdl);
     if (e != cudaSuccess) return static_cast<int>(e);

@@ -400,7 +400,7 @@ q8_prefill_kernel(const Params p, const Q8Cache cache) {
             *items_pub = k + 1;
           }
           // meta.x = ring slot | 0x100 on the first stage of an item | 0x200 when the item has rows for tile 1
-          const bool two = NT == 2 && u.q_len * G > u.row0 + kBM;
+          const bool two = NT == 2 && u.slot > kBM && u.q_len * G > u.row0 + kBM;
           raw_metas[st] = make_int2(ring_slot | (first ? 0x100 : 0) | (two ? 0x200 : 0), pos);
           const uint32_t bytes = (uint32_t)nblk * (uint32_t)pb * 2 * D;
           if (withhold) {
@@ -779,7 +779,7 @@ q8_prefill_kernel(const Params p, const Q8Cache cache) {
       if (u.seq < 0) break;
       int n_stages = (u.kv_end - u.kv_begin + kBN - 1) / kBN;
       if (n_stages < 1) n_stages = 1;
-      const bool two = NT == 2 && u.q_len * G > u.row0 + kBM;  // the item has rows for both tiles
+      const bool two = NT == 2 && u.slot > kBM && u.q_len * G > u.row0 + kBM;  // the item has rows for both tiles
       const bool active = (x == 0) || two;
       if (!active) {  // the item has no rows for this tile
         __syncwarp();
@@ -950,7 +950,7 @@ q8_prefill_kernel(const Params p, const Q8Cache cache) {
           if (q_pending) {
             __threadfence_block();
             const Unit un = ring[k % kRingP].u;
-            q_pending = un.seq >= 0 && (x == 0 || un.q_len * G > un.row0 + kBM);
+            q_pending = un.seq >= 0 && (x == 0 || (un.slot > kBM && un.q_len * G > un.row0 + kBM));
             if (q_pending) {
               q_fetch(un, ring[k % kRingP].h);
               q_ready = true;

@@ -108,13 +108,12 @@ __device__ __forceinline__ float to_float<__half>(__half x) { return __half2floa
 
 // host side, shared by the entry points (defined in rpa_api.cu)
 struct LaunchOptions {
-  int waves, min_chunk, prefill_rows, prefill_share, prefill_split, sort_items, overlap, fused_merge, wait_ms, path, test_withhold;
+  int min_chunk, prefill_rows, prefill_share, prefill_split, overlap, wait_ms, path, test_withhold;
 };
 LaunchOptions launch_options();
 // SM count of the current device; 0: no device, or not an sm_100 one
 int sm100_sm_count();
 int check_rpa_shape(const ejk_rpa_shape& s);
-WorkspaceLayout workspace_layout(const ejk_rpa_shape& s, int n_sm);
 void set_last_launches(int n);
 
 // launchers
@@ -125,6 +124,7 @@ bool q8_tma_supported(int page_size);
 cudaError_t q8_tensor_map(CUtensorMap* map, const Q8Cache& c, int box_tokens);
 cudaError_t launch_q8_splitkv(const Params& p, const Q8Cache& c, int dtype, int code, int n_sm, cudaStream_t stream, bool pdl);
 // tcgen05 tiles for sequences with many query rows (head_dim 64 and 128)
+cudaError_t launch_q8_plan(const Params& p, int n_sm, cudaStream_t stream, bool pdl);
 bool q8_prefill_supported(int head_dim);
 cudaError_t launch_q8_prefill(const Params& p, const Q8Cache& c, int dtype, int code, int n_sm, cudaStream_t stream, bool pdl);
 cudaError_t launch_q8_write(const void* keys, const void* values, long long key_stride, long long value_stride,

@@ -144,17 +144,16 @@ WorkspaceLayout layout_for(const ejk_rpa_shape& s, int n_sm) {
 
 }  // namespace
 
-// for the entry points of the 8-bit cache (q8_api.cu), which share the options, the planner and its workspace
+// for the entry points of the 8-bit cache (q8_api.cu), which share the options
 LaunchOptions launch_options() {
-  return {g_opt.waves, g_opt.min_chunk, g_opt.prefill_rows, g_opt.prefill_share, g_opt.prefill_split, g_opt.sort_items,
-          g_opt.overlap, g_opt.fused_merge, g_opt.wait_ms, g_opt.path, g_opt.test_withhold};
+  return {g_opt.min_chunk, g_opt.prefill_rows, g_opt.prefill_share, g_opt.prefill_split, g_opt.overlap, g_opt.wait_ms, g_opt.path,
+          g_opt.test_withhold};
 }
 int sm100_sm_count() {
   const DeviceInfo* d = device_info();
   return d && d->cc_major == 10 ? d->sm_count : 0;
 }
 int check_rpa_shape(const ejk_rpa_shape& s) { return check_shape(&s); }
-WorkspaceLayout workspace_layout(const ejk_rpa_shape& s, int n_sm) { return layout_for(s, n_sm); }
 void set_last_launches(int n) { t_last_launches = n; }
 
 }  // namespace ejk

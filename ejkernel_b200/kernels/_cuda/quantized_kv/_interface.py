@@ -264,8 +264,7 @@ def quantized_ragged_page_attention(
                block_tables.shape, block_tables.dtype, block_tables.is_contiguous(), block_tables.get_device(),
                query_start_loc.shape, query_start_loc.dtype, query_start_loc.is_contiguous(), query_start_loc.get_device(),
                None if softmax_aux is None else (softmax_aux.shape, softmax_aux.dtype, softmax_aux.get_device()),
-               softmax_scale, logits_soft_cap, sliding_window, num_kv_pages_per_block, num_queries_per_block,
-               _cabi.get_option_cached("waves"))
+               softmax_scale, logits_soft_cap, sliding_window, num_kv_pages_per_block, num_queries_per_block, "attention")
         plan = _plans.get(key)
     except (AttributeError, TypeError):  # not tensors, not hashable: the full check says what is wrong
         key = plan = None
