@@ -110,8 +110,10 @@ __global__ void __launch_bounds__(kThreads) q8_plan_kernel(const Params p, int n
     if (keys) atomicAdd(&s_decode_keys, keys);
   }
   __syncthreads();
-  // Few items leave SMs idle: with 128 rows each there are twice as many, of about half the time
-  const bool half = (long long)s_items[0] * p.Hkv * 2 <= n_cta;
+  // Rows of an item: an item of 128 takes about 0.6 of the time of one of 256 (one tile's softmax warps have the SM to
+  // themselves), which pays where it does not cost rounds over the SMs
+  const long long rounds256 = ((long long)s_items[0] * p.Hkv + n_cta - 1) / n_cta, rounds128 = ((long long)s_items[1] * p.Hkv + n_cta - 1) / n_cta;
+  const bool half = rounds128 * 5 < rounds256 * 8;
   const int item_rows = half ? kPrefillRows : 2 * kPrefillRows;
   const int n_items = half ? s_items[1] : s_items[0];
   const bool fits = n_items <= p.max_punits;
