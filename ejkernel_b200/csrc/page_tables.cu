@@ -10,8 +10,8 @@
 // launch behind the first) and then writes its share of the tokens, the new pages and the returned ones.  That needs no order
 // between blocks, because nothing is read that this call writes: a new page that comes from a finished row is looked up
 // in that row's table, not on the stack, and the slots of new pages are computed, not read back.
-// Measured on the device: 4 rows 4.3 us, 1000 rows with 8.8 thousand tokens and 24 thousand returned pages %T1000% (one block
-// for the sums and pages and a second kernel for the slots: 6.9 and 37.6 us).
+// Measured on the device: 4 rows 4.2 us, 1000 rows with 9 thousand tokens and 25 thousand returned pages 9.6 us (one block for the
+// sums and pages and a second kernel for the slots: 6.9 and 37.6 us).
 #include "q8_types.cuh"
 
 namespace ejk {

@@ -117,7 +117,7 @@ int ejk_q8_attention_launch(const void* queries, const void* kv_pages, const flo
   if (a.q_scale != 0.f || a.out_scale != 0.f) return EJK_RPA_E_ARG;
   if (a.num_sinks < 0 || (a.num_sinks > 0 && !softmax_aux)) return EJK_RPA_E_ARG;
   if (a.num_sinks > 0 && a.sink_rows != s.num_q_heads && a.sink_rows != s.num_kv_heads && a.sink_rows != 1) return EJK_RPA_E_ARG;
-  if (!aligned16(queries) || !aligned16(kv_pages) || !aligned16(kv_scales) || !aligned16(out)) return EJK_RPA_E_ALIGN;
+  if (!aligned16(queries) || !aligned16(kv_pages) || (reinterpret_cast<uintptr_t>(kv_scales) & 3) || !aligned16(out)) return EJK_RPA_E_ALIGN;
   const int n_sm = sm100_sm_count();
   if (!n_sm) return EJK_RPA_E_DEVICE;
   if (kQ8TicketsPerCta * 2 * n_sm * sizeof(int32_t) > EJK_Q8_TICKET_BYTES) return EJK_RPA_E_DEVICE;

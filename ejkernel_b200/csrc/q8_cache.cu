@@ -147,7 +147,8 @@ __device__ __forceinline__ unsigned write_block(const T* __restrict__ src, long 
 // A block of the batch is found by its first row: row t opens one if row t - 1 is elsewhere.  A CTA looks through `window` rows
 // for such rows -- one in short batches, where every row may open a block and parallelism is what counts, more in long ones,
 // where most rows open none and most CTAs would start for nothing -- and a warp of it takes one (head, K or V).
-// DRAM bounds the long batches (2 bytes in, 1 byte out per element), the chain slots -> rows -> codes the short ones: %WRITE%
+// DRAM bounds the long batches (2 bytes in, 1 byte out per element), the chain slots -> rows -> codes the short ones:
+// 12 thousand f16 rows of 8 heads of 128 in blocks of 32 (75 MB) 20 us = 3.7 TB/s, 256 decode tokens 5.2 us, one token 1.9 us.
 template <typename T, typename Code, int D>
 __global__ void __launch_bounds__(kWriteThreads)
 q8_write_kernel(const T* __restrict__ keys, const T* __restrict__ values, long long key_stride, long long value_stride,
@@ -209,7 +210,8 @@ q8_write_kernel(const T* __restrict__ keys, const T* __restrict__ values, long l
 }
 
 // Eight elements of K and of V of two rows per thread: four independent 8-byte loads in flight, 16-byte stores.  DRAM bounds
-// it: 65536 rows of 8 heads of 128 (403 MB) %READ%
+// it: 65536 rows of 8 heads of 128 (403 MB) 75.8 us = 5.3 TB/s, 0.82 of the measured copy rate (one 8-byte load per
+// thread: 136 us).
 template <typename T, typename Code>
 __global__ void __launch_bounds__(kReadThreads)
 q8_read_kernel(const Q8Cache c, const int32_t* __restrict__ slots, uint4* __restrict__ keys, uint4* __restrict__ values,
@@ -274,7 +276,7 @@ cudaError_t write_dispatch(const void* keys, const void* values, long long ks, l
   const T* k = static_cast<const T*>(keys);
   const T* v = static_cast<const T*>(values);
   // rows that a CTA looks through: up to 1024 rows one each, then what keeps about as many windows (12 thousand rows in blocks of
-  // 32, 75 MB: %WINDOW%)
+  // 32: 24 us with windows of 32, 20 us with 16)
   int window = 1;
   while (window < 32 && window < (1 << c.block_shift) && rows / window > 1024) window *= 2;
   const dim3 grid((rows + window - 1) / window, (2 * c.Hkv + kWriteThreads / 32 - 1) / (kWriteThreads / 32));

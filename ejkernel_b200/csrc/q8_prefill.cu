@@ -2,9 +2,8 @@
 //
 //     S[128 x 64] = Q[128 x D] . Kc^T,   P = 2^(S * k_scale * scale * log2 e - m),   O += P . (Vc * v_scale / v_ref)
 //
-// The tiles, barriers, KV split and epilogue are those of rpa_prefill_sm100.cu (two 128-row tiles per CTA, 64-token
-// stages, S and P.V issued by single threads, one softmax thread per row).  (The turns that the tiles of
-// that kernel take at the exponentials cost more than they give here: 1.49 ms with, 1.39 without, 4 x 2048 rows over 8192 keys.)
+// The tiles, barriers, KV split and epilogue are those of rpa_prefill_sm100.cu: two 128-row tiles per CTA, 64-token stages, S and
+// P.V issued by single threads, one softmax thread per row.
 // What the codes add is a pipeline in front:
 //
 //   producer warp --raw stage (codes: bulk copies; scales: 4-byte cp.async)--> four converter warps --16-bit stage--> MMAs
@@ -22,6 +21,13 @@
 //     what is below 2^-31 of the largest weight is lost.
 //   * registers: 16 warps have 128 registers a thread; the issuing warps and the converters give theirs to the softmax
 //     warps (setmaxnreg: 64 + 72 + 2 * 184 <= 4 * 128).
+//
+// What bounds it: neither the tensor pipe nor the exponentials (each about a third busy) but the softmax threads' instructions
+// and the instruction cache that five roles share; a stage of two tiles takes 3200 cycles where the 16-bit kernel takes 2500.
+// 4 sequences x 2048 rows over 8192 keys, 32 heads over 8 kv heads of 128: 1.34 ms = 716 TFLOP/s (16-bit operator 1.05 ms); on the
+// way there: all of a stage unrolled in the converters 2.57, a rolled loop 1.73, no rare paths in the common kernel and paired
+// float32 instructions 1.49, no turns between the tiles at the exponentials (which the 16-bit kernel gains from) 1.39, a planner
+// of its own 1.34.  Tried and dropped: two threads per row with half of the columns each (1.73), eight converter warps (1.46).
 //
 // Warp roles (512 threads with two tiles, 384 with one; one CTA per SM, persistent over the planner's prefill queue):
 //   warp 0 producer, warp 1 S of tile 0 (and the TMEM allocation), warp 2 S of tile 1, warp 3 P.V of all tiles,
