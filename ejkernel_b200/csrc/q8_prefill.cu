@@ -20,16 +20,19 @@
 //   * P is f16.  Its reference sits 2^7 below the maximum it was chosen for, which puts the weights between 2^15 and 2^-24:
 //     what is below 2^-31 of the largest weight is lost.
 //   * registers: 16 warps have 128 registers a thread; the issuing warps and the converters give theirs to the softmax
-//     warps (setmaxnreg: 64 + 72 + 2 * 184 <= 4 * 128).
+//     warps (setmaxnreg: 72 + 72 + 2 * 184 = 4 * 128).
 //
 // What bounds it: neither the tensor pipe nor the exponentials (each about a third busy) but the softmax threads' instructions
 // and the instruction cache that five roles share; a stage of two tiles takes 3200 cycles where the 16-bit kernel takes 2500.
 // 4 sequences x 2048 rows over 8192 keys, 32 heads over 8 kv heads of 128: 1.34 ms = 716 TFLOP/s (16-bit operator 1.05 ms); on the
 // way there: all of a stage unrolled in the converters 2.57, a rolled loop 1.73, no rare paths in the common kernel and paired
 // float32 instructions 1.49, no turns between the tiles at the exponentials (which the 16-bit kernel gains from) 1.39, a planner
-// of its own 1.34.  Tried and dropped: two threads per row with half of the columns each (1.73), eight converter warps (1.46).
+// of its own 1.34.  With blocks of 4 tokens 4 chunks of up to 2048 rows (504 us) take 565 us, with a soft cap 804: 664 and 898 before
+// the factors and tanh went two columns to an instruction.  An item of one tile is bound by how long a stage takes to come through:
+// 24 mixed requests with pages of 24 tokens 82 us while the producer divided for each page and scale, 65 with the stepped indexes.
+// Tried and dropped: two threads per row with half of the columns each (1.73), eight converter warps (1.46).
 //
-// Warp roles (512 threads with two tiles, 384 with one; one CTA per SM, persistent over the planner's prefill queue):
+// Warp roles (512 threads, one CTA per SM, persistent over the items of q8_plan.cu):
 //   warp 0 producer, warp 1 S of tile 0 (and the TMEM allocation), warp 2 S of tile 1, warp 3 P.V of all tiles,
 //   warps 4-7 converters, warps 8-11 softmax of tile 0, warps 12-15 of tile 1.
 //
@@ -68,18 +71,18 @@ struct ItemDescP {
 template <int D>
 struct CfgP {
   static constexpr int BN = 64;                       // tokens per KV stage
-  static constexpr int NT = (D <= 128) ? 2 : 1;       // 128-row tiles per CTA (TMEM holds one 256-column O)
+  static constexpr int NT = 2;                        // 128-row tiles per CTA
   static constexpr int SM_WARPS = 4;                  // softmax warps per tile: one thread per row
   static constexpr int CV_WARPS = 4;                  // converter warps
   static constexpr int THREADS = 32 * (4 + CV_WARPS + SM_WARPS * NT);
   static constexpr int REGS = 65536 / THREADS / 8 * 8;  // per thread at launch
-  static constexpr int REGS_ISSUE = 64, REGS_CONVERT = 72, REGS_SOFTMAX = 184;
+  static constexpr int REGS_ISSUE = 72, REGS_CONVERT = 72, REGS_SOFTMAX = 184;
   static_assert(REGS_ISSUE + REGS_CONVERT + NT * REGS_SOFTMAX <= (2 + NT) * REGS, "setmaxnreg.inc draws on the block's own registers");
   static constexpr int RAW_BYTES = BN * 2 * D;        // a stage of codes: [K|V][BN][D]
   static constexpr int STAGE_BYTES = BN * 2 * D * 2;  // a stage of 16-bit values
   // 16-bit stages and stages of codes: what shared memory holds beside the query tiles
-  static constexpr int NS = (D == 64) ? 6 : (D == 128) ? 3 : 2;
-  static constexpr int NR = (D == 64) ? 4 : (D == 128) ? 3 : 1;
+  static constexpr int NS = (D == 64) ? 6 : 3;
+  static constexpr int NR = (D == 64) ? 4 : 3;
   static constexpr int GROUP_BYTES = 8 * 2 * D * 2;   // one 8-token group of a 16-bit stage: [K|V][D/64][8][64]
   static constexpr int V_OFF = (D / 64) * 1024;
   static constexpr int Q_BYTES = kBM * D * 2;
@@ -149,6 +152,16 @@ __device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c
 __device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul_f32x2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float fast_reciprocal(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(r) : "f"(x));
   return r;
 }
 __device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, __half2 b) {
@@ -241,7 +254,7 @@ q8_prefill_kernel(const Params p, const Q8Cache cache) {
   // one SM together.  So this kernel keeps only as many CTAs as make it end about when the other does; the rest exit at
   // once and hand their SMs over (the rule of rpa_prefill_sm100.cu).
   int n_cta = (int)gridDim.x;
-  if ((p.pdl & 1) && p.prefill_share > 0 && D <= 128) {
+  if ((p.pdl & 1) && p.prefill_share > 0) {
     const float stages = (float)p.header[kHdrPrefillStages] * (float)Hkv;           // (item, head) stages of 64 tokens
     const float dec_bytes = (float)p.header[kHdrTotalKeys] * (float)Hkv * (float)(2 * D);
     // one stage of two 128-row tiles, and what a soft cap's tanh adds
@@ -268,6 +281,7 @@ q8_prefill_kernel(const Params p, const Q8Cache cache) {
     const int sb_shift = cache.block_shift;
     const int scales_per_page = p.page_size >> sb_shift;
     const size_t plane_bytes = (size_t)p.page_size * D;
+    const int step_pages = kBN / p.page_size, step_off = kBN % p.page_size;
     int gi = 0;  // stage counter of this CTA
     int k = 0;
     // Whole (item, head) pairs from the planner's longest-first queue, or, where that schedule is clearly worse, equal
@@ -356,8 +370,11 @@ q8_prefill_kernel(const Params p, const Q8Cache cache) {
       if (!split && lane == 0) wid_next = atomicAdd(&p.header[kHdrPrefillQueue], 1);
       const int32_t* tab = p.block_tables + (size_t)u.seq * p.pages_per_seq;
       bool first = true;
-      auto split_key = [&](int key, int& off) {
-        int pi;
+      // where this lane's block of tokens lies: divided out once per item and stepped from then on; the id of a stage's page is
+      // on its way while the stage before it is issued
+      int pi, off;
+      {
+        const int key = u.kv_begin + (lane << pb_shift);
         if (p.page_shift >= 0) {
           pi = key >> p.page_shift;
           off = key & (p.page_size - 1);
@@ -365,24 +382,28 @@ q8_prefill_kernel(const Params p, const Q8Cache cache) {
           pi = key / p.page_size;
           off = key - pi * p.page_size;
         }
-        return pi;
+      }
+      auto blocks_at = [&](int pos) {
+        const int n = (u.kv_end - pos + pb - 1) >> pb_shift;
+        return n < 0 ? 0 : n > (kBN >> pb_shift) ? kBN >> pb_shift : n;
       };
-      auto page_of = [&](int pi) {
-        int page = __ldg(tab + pi);
+      int id_next = lane < blocks_at(u.kv_begin) ? __ldg(tab + pi) : 0;
+      for (int pos = u.kv_begin; first || pos < u.kv_end; pos += kBN) {
+        const int st = gi % NR;
+        const int nblk = blocks_at(pos);
+        int page = id_next;
         if ((unsigned)page >= (unsigned)p.num_pages) {
           flags |= EJK_RPA_ST_PAGE_ID;
           page = 0;
         }
-        return page;
-      };
-      for (int pos = u.kv_begin; first || pos < u.kv_end; pos += kBN) {
-        const int st = gi % NR;
-        int nblk = (u.kv_end - pos + pb - 1) >> pb_shift;
-        if (nblk > (kBN >> pb_shift)) nblk = kBN >> pb_shift;
-        if (nblk < 0) nblk = 0;
-        // page id of this lane's block of tokens, fetched before the wait so its latency is hidden
-        int page = 0, off = 0;
-        if (lane < nblk) page = page_of(split_key(pos + (lane << pb_shift), off));
+        const int at_off = off;
+        pi += step_pages;
+        off += step_off;
+        if (off >= p.page_size) {
+          off -= p.page_size;
+          ++pi;
+        }
+        id_next = lane < blocks_at(pos + kBN) ? __ldg(tab + pi) : 0;
         if (!mbar_wait(bar_raw_empty(st), ((gi / NR) & 1) ^ 1, abort_flag, wait_ns)) {
           alive = false;
           break;
@@ -406,7 +427,7 @@ q8_prefill_kernel(const Params p, const Q8Cache cache) {
             *items_pub = k + 1;
           }
           // meta.x = ring slot | 0x100 on the first stage of an item | 0x200 when the item has rows for tile 1
-          const bool two = NT == 2 && u.slot > kBM && u.q_len * G > u.row0 + kBM;
+          const bool two = u.slot > kBM && u.q_len * G > u.row0 + kBM;
           raw_metas[st] = make_int2(ring_slot | (first ? 0x100 : 0) | (two ? 0x200 : 0), pos);
           const uint32_t bytes = (uint32_t)nblk * (uint32_t)pb * 2 * D;
           if (withhold) {
@@ -419,7 +440,7 @@ q8_prefill_kernel(const Params p, const Q8Cache cache) {
         __syncwarp();
         if (!withhold) {
           if (lane < nblk) {
-            const uint8_t* src = cache.pages + (((size_t)page * Hkv + h) * 2) * plane_bytes + (size_t)off * D;
+            const uint8_t* src = cache.pages + (((size_t)page * Hkv + h) * 2) * plane_bytes + (size_t)at_off * D;
             const uint32_t dst = sb + C::OFF_RAW + st * C::RAW_BYTES + (uint32_t)(lane << pb_shift) * D;
             bulk_load(dst, src, (uint32_t)pb * D, full);
             bulk_load(dst + kBN * D, src + plane_bytes, (uint32_t)pb * D, full);
@@ -429,13 +450,17 @@ q8_prefill_kernel(const Params p, const Q8Cache cache) {
           const int last = (u.kv_end < pos + kBN ? u.kv_end : pos + kBN) - 1;
           const int n_e = last >= pos ? (last >> sb_shift) - e0 + 1 : 0;
           const uint32_t sdst = sb + C::OFF_RAWSCALE + st * (2 * kBN * 4);
-          for (int e = lane; e < n_e; e += 32) {
-            int eoff;
-            const int key = (e0 + e) << sb_shift;
-            const int pi = split_key(key > pos ? key : pos, eoff);
-            const long long at = (((long long)page_of(pi) * Hkv + h) * 2) * scales_per_page + (eoff >> sb_shift);
-            cp_async4(sdst + e * 4, cache.scales + at);
-            cp_async4(sdst + (kBN + e) * 4, cache.scales + at + scales_per_page);
+          for (int b0 = 0; b0 < n_e; b0 += 32) {
+            const int e = b0 + lane;
+            int rel = ((e0 + e) << sb_shift) - pos;  // the block's first key in the stage; its page is that of a lane's tokens
+            rel = e < n_e && rel > 0 ? rel : 0;
+            const int of_page = __shfl_sync(0xffffffffu, page, rel >> pb_shift);
+            const int eoff = __shfl_sync(0xffffffffu, at_off, rel >> pb_shift) + (rel & (pb - 1));
+            if (e < n_e) {
+              const float* src = cache.scales + (((long long)of_page * Hkv + h) * 2) * scales_per_page + (eoff >> sb_shift);
+              cp_async4(sdst + e * 4, src);
+              cp_async4(sdst + (kBN + e) * 4, src + scales_per_page);
+            }
           }
           cp_async_arrive(full);
         }
@@ -465,7 +490,7 @@ q8_prefill_kernel(const Params p, const Q8Cache cache) {
     // =============================== MMA issuers ===============================
     // Single-thread roles, ordered by the barriers alone: S_x(t+1) needs the S columns back (s_free), P_x.V(t) needs P_x(t)
     // (p_full); both need the stage (kv_full).
-    if (lane == 0 && (warp == 3 || warp - 1 < NT)) {
+    if (lane == 0) {
       const bool is_s = warp < 3;
       const int x = is_s ? warp - 1 : 0;
       constexpr uint32_t idesc_s = instr_desc<__half>(kBN, false);
@@ -487,8 +512,7 @@ q8_prefill_kernel(const Params p, const Q8Cache cache) {
 #pragma unroll
       for (int y = 0; y < NT; ++y) tx[y] = itemsx[y] = 0;
       while (!is_s) {
-        // ---- P.V of all tiles, tile 0 first (the order in which the tiles take their turns at the
-        // exponentials, so P_0(t) is ready before P_1(t), and P_0(t+1) only after that) ----
+        // ---- P.V of all tiles, tile 0 first ----
         const int st = gi % NS;
         if (!mbar_wait_thread(bar_kv_full(st), (gi / NS) & 1, abort_flag, wait_ns)) break;
         const int mx = metas[st].x;
@@ -597,8 +621,8 @@ q8_prefill_kernel(const Params p, const Q8Cache cache) {
     const int ch = ctid % CPT, t0 = ctid / CPT;
     const int half_first = D == 128 ? (ch >> 2) & 1 : 0;
     const uint32_t c_first = (uint32_t)((2 * ch + half_first) & 7), c_second = c_first ^ 1u;
-    const bool coarse = PLAIN || sb_shift >= 3;    // one factor per 8 tokens is enough
-    const float to_log2 = p.cap != 0.f ? p.inv_cap_scale : p.scale_log2;
+    constexpr bool coarse = PLAIN;        // one factor per 8 tokens is enough
+    const float to_log2 = p.cap != 0.f ? p.inv_cap_scale * (2.f * kLog2eP) : p.scale_log2;
     float v_norm = 1.f;
     int lo_min = -1, kv_end = 0;
     int gi = 0;
@@ -640,8 +664,7 @@ q8_prefill_kernel(const Params p, const Q8Cache cache) {
         v_norm = __uint_as_float((254u + kVBits - e) << 23);
       }
       if (!mbar_wait(bar_kv_empty(st), ((gi / NS) & 1) ^ 1, abort_flag, wait_ns)) break;
-      // each token's factor on its logits; where blocks have 8 tokens or more, one per 8 tokens.  Never 0: masked logits are
-      // -inf, and their product with it has to stay that
+      // each token's factor on its logits; in the common kernel one per 8 tokens
       if (ctid < (coarse ? kBN / 8 : kBN)) {
         const int key = pos + (coarse ? ctid * 8 : ctid);
         reinterpret_cast<float*>(smem + C::OFF_KSCALE + st * (kBN * 4))[ctid] = key < kv_end ? ks_s[(key >> sb_shift) - e0] * to_log2 : 1.f;
@@ -698,7 +721,6 @@ q8_prefill_kernel(const Params p, const Q8Cache cache) {
     // warp may touch are fixed by warp % 4), so row maxima and sums need no shuffles.
     constexpr int HB = kBN;
     const int sw = warp - 8;
-    [[maybe_unused]] const bool coarse = PLAIN || cache.block_shift >= 3;
     const int x = sw / C::SM_WARPS;                       // which tile of the CTA
     const int row = (warp & 3) * 32 + lane;               // TMEM lane == row within the tile
     const uint32_t lane_addr = (uint32_t)((warp & 3) * 32) << 16;
@@ -785,7 +807,7 @@ q8_prefill_kernel(const Params p, const Q8Cache cache) {
       if (u.seq < 0) break;
       int n_stages = (u.kv_end - u.kv_begin + kBN - 1) / kBN;
       if (n_stages < 1) n_stages = 1;
-      const bool two = NT == 2 && u.slot > kBM && u.q_len * G > u.row0 + kBM;  // the item has rows for both tiles
+      const bool two = u.slot > kBM && u.q_len * G > u.row0 + kBM;  // the item has rows for both tiles
       const bool active = (x == 0) || two;
       if (!active) {  // the item has no rows for this tile
         __syncwarp();
@@ -835,8 +857,7 @@ q8_prefill_kernel(const Params p, const Q8Cache cache) {
         // Common case: the products stay in the registers, a factor per 8 columns goes into the exponent's FMA and only the
         // groups' maxima are multiplied; a soft cap, finer scales or a scale that is not positive materialise the logits.
         const float v_new = vrefs[st];
-        const float* kf = reinterpret_cast<const float*>(smem + C::OFF_KSCALE + st * (kBN * 4));
-        const float4* kf4 = reinterpret_cast<const float4*>(kf);
+        const float4* kf4 = reinterpret_cast<const float4*>(smem + C::OFF_KSCALE + st * (kBN * 4));
         const bool full_vis = (pos + HB - 1 <= pos_row) && (pos > lo_row);
         float ef[HB / 8];
 #pragma unroll
@@ -853,22 +874,27 @@ q8_prefill_kernel(const Params p, const Q8Cache cache) {
           }
         }
         if constexpr (!PLAIN) {
-          if (coarse) {
+          const uint64_t qf = pack_f32x2(q_fac, q_fac);
 #pragma unroll
-            for (int i = 0; i < HB; ++i) sr[i] = __float_as_uint(__uint_as_float(sr[i]) * (kf[i >> 3] * q_fac));
-          } else {
-#pragma unroll
-            for (int i = 0; i < HB; i += 4) {
-              const float4 f = kf4[i >> 2];
-              sr[i] = __float_as_uint(__uint_as_float(sr[i]) * (f.x * q_fac));
-              sr[i + 1] = __float_as_uint(__uint_as_float(sr[i + 1]) * (f.y * q_fac));
-              sr[i + 2] = __float_as_uint(__uint_as_float(sr[i + 2]) * (f.z * q_fac));
-              sr[i + 3] = __float_as_uint(__uint_as_float(sr[i + 3]) * (f.w * q_fac));
-            }
+          for (int i = 0; i < HB; i += 4) {
+            const float4 f = kf4[i >> 2];
+            const float2 a = unpack_f32x2(mul_f32x2(pack_f32x2(__uint_as_float(sr[i]), __uint_as_float(sr[i + 1])), mul_f32x2(pack_f32x2(f.x, f.y), qf)));
+            const float2 b = unpack_f32x2(mul_f32x2(pack_f32x2(__uint_as_float(sr[i + 2]), __uint_as_float(sr[i + 3])), mul_f32x2(pack_f32x2(f.z, f.w), qf)));
+            sr[i] = __float_as_uint(a.x);
+            sr[i + 1] = __float_as_uint(a.y);
+            sr[i + 2] = __float_as_uint(b.x);
+            sr[i + 3] = __float_as_uint(b.y);
           }
           if (p.cap != 0.f) {
+            // cap * tanh(t) = cap - 2 cap / (2^(2 t log2 e) + 1); the factors hold the 2 log2 e.  An infinite power gives cap
+            const uint64_t one = pack_f32x2(1.f, 1.f), cap = pack_f32x2(p.cap_log2, p.cap_log2), twice = pack_f32x2(-2.f * p.cap_log2, -2.f * p.cap_log2);
 #pragma unroll
-            for (int i = 0; i < HB; ++i) sr[i] = __float_as_uint(p.cap_log2 * soft_cap_tanh(__uint_as_float(sr[i])));
+            for (int i = 0; i < HB; i += 2) {
+              const float2 e = unpack_f32x2(add_f32x2(pack_f32x2(fast_exp2(__uint_as_float(sr[i])), fast_exp2(__uint_as_float(sr[i + 1]))), one));
+              const float2 y = unpack_f32x2(fma_f32x2(pack_f32x2(fast_reciprocal(e.x), fast_reciprocal(e.y)), twice, cap));
+              sr[i] = __float_as_uint(y.x);
+              sr[i + 1] = __float_as_uint(y.y);
+            }
           }
         }
         if (__builtin_expect(!full_vis, 0)) {
