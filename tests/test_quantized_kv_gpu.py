@@ -146,6 +146,44 @@ def test_attention_prompt_chunks(code):
     check(b, run(b))
 
 
+@pytest.mark.parametrize("page, block", [(8, 8), (8, 1), (16, 2), (24, 8), (40, 4), (48, 16), (56, 8), (64, 64), (128, 128), (256, 64)])
+@pytest.mark.parametrize("dim, window", [(64, None), (128, 70)])
+def test_attention_prompt_pages_and_scale_blocks(page, block, dim, window):
+    """Tiles that begin and end inside pages and scale blocks, with a window that begins inside one."""
+    b = make_batch([(100, 333), (70, 70), (1, 200), (130, 517)], Hq=4, Hkv=2, dim=dim, page=page, block=block, code=torch.int8,
+                   half=torch.bfloat16, seed=page + block, any_scale=True)
+    kw = {} if window is None else dict(sliding_window=window)
+    check(b, run(b, **kw), **kw)
+
+
+@pytest.mark.parametrize("cap, scale", [(-3.0, None), (0.01, None), (5.0, 4.0), (50.0, -0.3)])
+@pytest.mark.parametrize("block", [16, 2])
+def test_attention_prompt_soft_caps(block, cap, scale):
+    """Caps of either sign, one that every logit reaches and one that few reach."""
+    b = make_batch([(90, 300), (1, 100), (200, 260)], Hq=4, Hkv=2, dim=64, page=16, block=block, code=torch.float8_e4m3fn, half=torch.float16, seed=8)
+    kw = dict(logits_soft_cap=cap, softmax_scale=scale)
+    check(b, run(b, **kw), **kw)
+
+
+@pytest.mark.parametrize("rows", [1, 90])
+def test_scales_need_no_more_than_their_own_alignment(rows):
+    b = make_batch([(rows, 300), (1, 77)], Hq=4, Hkv=2, dim=128, page=16, block=4, code=torch.int8, half=torch.bfloat16, seed=9)
+    want = run(b)
+    c = {k: v.cuda() if isinstance(v, torch.Tensor) else v for k, v in b.items()}
+    flat = torch.zeros(c["scales"].numel() + 1, device="cuda")
+    scales = flat[1:].view(c["scales"].shape)
+    scales.copy_(c["scales"])
+    assert torch.equal(ej.quantized_ragged_page_attention(c["q"], c["codes"], scales, c["ctx"], c["tab"], c["start"], c["n"]), want)
+    slots = torch.arange(40, dtype=torch.int32, device="cuda")
+    for got, plain in zip(ej.quantized_kv_read(c["codes"], scales, slots), ej.quantized_kv_read(c["codes"], c["scales"], slots)):
+        assert torch.equal(got, plain)
+    x = torch.randn((40, 2, 128), generator=torch.Generator().manual_seed(10)).bfloat16().cuda()
+    kv = c["codes"].clone()
+    ej.quantized_kv_write(x, x, c["codes"], c["scales"], slots)
+    ej.quantized_kv_write(x, x, kv, scales, slots)
+    assert torch.equal(kv, c["codes"]) and torch.equal(scales, c["scales"])
+
+
 @pytest.fixture
 def option():
     old = {}
