@@ -18,10 +18,11 @@
 //     products run on f16 mma.sync with float32 sums.  8-bit operands would halve the mma work, which is not what bounds
 //     the kernel, and would round q and p to 3 bits of mantissa.  (Eight warps in two teams that take the stages in turn
 //     were slower: 0.50 ms against 0.37 for 128 sequences of 8192 keys; the registers go down to 96.)
-//   * k_scale multiplies the finished dot product, v_scale the probability: two multiplications a token and row, none per
-//     element.  p * v_scale has to fit f16: a warp divides v_scale by a power of two, chosen from the largest scale that
-//     it has met so that the product is at most 2^15, and moves it as it moves m.  What is below 2^-24 of that
-//     range is lost: 2^-32 of the largest |V|.
+//   * k_scale multiplies the finished dot product, v_scale the probability: a few multiplications a token and row, none per
+//     element.  p * v_scale has to fit f16: a row divides v_scale by a power of two, chosen from the largest scale that
+//     it has seen so that the product is at most 2^15, and moves it as it moves m.  What is below 2^-24 of that
+//     range is lost: 2^-31 of the largest |V| that the row sees.  (One power of two for all rows of a tile would let a key that
+//     the mask hides from a row push that row's values out of f16.)
 //   * bf16 queries go to f16 by a power of two per row (their largest element to [2^14, 2^15)), undone on the logits.
 //
 // Every wait on an mbarrier is bounded in wall time (option "wait_ms"): on expiry the warp raises
@@ -45,7 +46,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kMergeInFlight = 8;     // parts whose loads a merge keeps in flight per row
 constexpr int kGroup = 16;            // parts that are combined at a time: more go through groups
 constexpr float kLazyRescale = 8.0f;  // rescale the accumulators only when the max grows by 2^8: p <= 2^8
-constexpr int kVBits = 6;             // the largest v_scale met so far is taken to [2^6, 2^7): p * v_scale <= 2^15 < 65504
+constexpr int kVBits = 6;             // the largest v_scale seen so far is taken to [2^6, 2^7): p * v_scale <= 2^15 < 65504
 
 // One piece of work of a CTA: stages of one (row tile, kv head).  Of a pair that several CTAs share, u.n_chunks is the number of
 // parts, u.chunk_idx this part's number and u.merge_idx the CTA of part 0; u.slot is where this part goes, u.pad where part 0 is.
@@ -541,7 +542,8 @@ q8_splitkv_kernel(const __grid_constant__ CUtensorMap tmap, const Params p, cons
     float m_run[NT][2], l_run[NT][2], q_fac[NT][2];
     int pos_r[NT][2], lo_r[NT][2];
     int pos_min = 0, lo_max = 0, lo_min = -1;
-    float v_norm = 1.f;  // power of two that the V scales are multiplied by
+    bool one_token = true;  // the tile's rows are one query token's: they see the same keys
+    float v_norm[NT][2];  // powers of two that the V scales are multiplied by, one per row
     int s = 0;
     uint32_t full_parity = 0, c_parity = 0;
     int pieces = 0;
@@ -575,9 +577,9 @@ q8_splitkv_kernel(const __grid_constant__ CUtensorMap tmap, const Params p, cons
         const float to_log2 = p.cap != 0.f ? p.inv_cap_scale : p.scale_log2;
         const int base = u.kv_len - u.q_len;
         pos_min = base + u.row0 / G;
+        one_token = (u.row0 + n_rows - 1) / G == u.row0 / G;
         lo_max = (p.window > 0) ? (base + (u.row0 + n_rows - 1) / G - p.window) : -1;
         lo_min = (p.window > 0) ? pos_min - p.window : -1;
-        v_norm = __uint_as_float((127u + 125u) << 23);  // no scale met yet: the largest power of two (see below)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           // elements 32kt + 4t .. +3 (first mma of the chunk) and 32kt + 16 + 4t .. +3 (second)
@@ -601,6 +603,7 @@ q8_splitkv_kernel(const __grid_constant__ CUtensorMap tmap, const Params p, cons
             q_fac[nt][j] = qfac[r] * to_log2;
             m_run[nt][j] = -INFINITY;
             l_run[nt][j] = 0.f;
+            v_norm[nt][j] = __uint_as_float((127u + 125u) << 23);  // no scale seen yet: the largest power of two (see below)
           }
 #pragma unroll
           for (int kt = 0; kt < KT; ++kt)
@@ -640,7 +643,7 @@ q8_splitkv_kernel(const __grid_constant__ CUtensorMap tmap, const Params p, cons
             }
           }
         }
-        // ---- scales of this lane's four tokens, and the largest V scale of the warp's 32
+        // ---- scales of this lane's four tokens
         const float* ks_s = reinterpret_cast<const float*>(smem + C::OFF_SCALE + s * (2 * TK * 4));
         const float* vs_s = ks_s + TK;
         const int e0 = pos >> sb_shift;
@@ -653,30 +656,36 @@ q8_splitkv_kernel(const __grid_constant__ CUtensorMap tmap, const Params p, cons
           // no row sees a key from kv_end on, or one that the window of the tile's first row has left behind
           vs[i] = (key < u.kv_end && key > lo_min) ? vs_s[e] : 0.f;
         }
-        {
-          float top = fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3]));
-          const uint32_t tb = __reduce_max_sync(0xffffffffu, __float_as_uint(top));  // positive floats order as integers
-          top = __uint_as_float(tb);
-          if (top * v_norm >= (float)(2 << kVBits)) {
-            // a larger scale than any before: take it to [2^6, 2^7) and the accumulators along
-            uint32_t e = tb >> 23;
-            e = e < 8u ? 8u : e;
-            const float v_new = __uint_as_float((254u + kVBits - e) << 23);
-            const float f = v_new * power_of_two_inverse(v_norm);  // 0 where the old terms are below anything that counts
+        const bool tail = key0 + TW > u.kv_end;  // tokens past the chunk end: stale or unowned bytes
+        const bool edge = tail || key0 <= lo_min;
+        const bool need_mask = tail || (key0 + TW - 1 > pos_min) || (key0 <= lo_max);
+        // takes the rows' accumulators to the power of two that the largest V scale asks for: that one to [2^6, 2^7)
+        auto larger_scale = [&](float top, float& norm) {
+          uint32_t e = __float_as_uint(top) >> 23;
+          e = e < 8u ? 8u : e;
+          const float v_new = __uint_as_float((254u + kVBits - e) << 23);
+          const float f = v_new * power_of_two_inverse(norm);  // 0 where the old terms are below anything that counts
+          norm = v_new;
+          return f;
+        };
+        if (one_token) {
+          // the rows see the same keys: one power of two, by the largest V scale of the warp's 32 (positive floats order as
+          // integers)
+          const float top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3])))));
+          if (top * v_norm[0][0] >= (float)(2 << kVBits)) {
+            const float f = larger_scale(top, v_norm[0][0]);
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+            for (int nt = 0; nt < NT; ++nt) {
+              v_norm[nt][0] = v_norm[nt][1] = v_norm[0][0];
 #pragma unroll
               for (int mt = 0; mt < KT; ++mt)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) acc[nt][mt][i] *= f;
-            v_norm = v_new;
+            }
           }
 #pragma unroll
-          for (int i = 0; i < 4; ++i) vs[i] *= v_norm;
+          for (int i = 0; i < 4; ++i) vs[i] *= v_norm[0][0];
         }
-        const bool tail = key0 + TW > u.kv_end;  // tokens past the chunk end: stale or unowned bytes
-        const bool edge = tail || key0 <= lo_min;
-        const bool need_mask = tail || (key0 + TW - 1 > pos_min) || (key0 <= lo_max);
         bool grow = false;
         float mx[NT][2];
 #pragma unroll
@@ -730,22 +739,57 @@ q8_splitkv_kernel(const __grid_constant__ CUtensorMap tmap, const Params p, cons
         }
         // ---- probabilities; times the V scale to f16, transposed into the B fragments of P.V
         uint32_t pbf[NT][4];
+        auto weights = [&](auto same) {
+          // same: the rows see the same keys and share the power of two, which has gone into vs
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
+          for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-          for (int b = 0; b < 2; ++b) {
+            for (int b = 0; b < 2; ++b) {
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                const float m_use = (m_run[nt][j] == -INFINITY) ? 0.f : m_run[nt][j];
+                const float p0 = fast_exp2(sc[nt][b][j] - m_use);
+                const float p1 = fast_exp2(sc[nt][b][j + 2] - m_use);
+                l_run[nt][j] += p0 + p1;
+                if constexpr (decltype(same)::value) {
+                  sc[nt][b][j] = p0 * vs[b * 2];
+                  sc[nt][b][j + 2] = p1 * vs[b * 2 + 1];
+                } else {
+                  // a key without weight has none whatever its scale: it may be one that the row does not see
+                  sc[nt][b][j] = p0 == 0.f ? 0.f : p0 * (vs[b * 2] * v_norm[nt][j]);
+                  sc[nt][b][j + 2] = p1 == 0.f ? 0.f : p1 * (vs[b * 2 + 1] * v_norm[nt][j]);
+                }
+              }
+              pbf[nt][b * 2] = movmatrix_trans(Mma<__half>::pack(sc[nt][b][0], sc[nt][b][1]));
+              pbf[nt][b * 2 + 1] = movmatrix_trans(Mma<__half>::pack(sc[nt][b][2], sc[nt][b][3]));
+            }
+          }
+        };
+        if (one_token) {
+          weights(std::true_type{});
+        } else {
+          // a power of two for each row, by the largest V scale among the keys that it sees
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-              const float m_use = (m_run[nt][j] == -INFINITY) ? 0.f : m_run[nt][j];
-              const float p0 = fast_exp2(sc[nt][b][j] - m_use);
-              const float p1 = fast_exp2(sc[nt][b][j + 2] - m_use);
-              l_run[nt][j] += p0 + p1;
-              sc[nt][b][j] = p0 * vs[b * 2];
-              sc[nt][b][j + 2] = p1 * vs[b * 2 + 1];
+              float top = 0.f;
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (sc[nt][i >> 1][(i & 1) * 2 + j] != -INFINITY) top = fmaxf(top, vs[i]);
+              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+              if (top * v_norm[nt][j] >= (float)(2 << kVBits)) {
+                const float f = larger_scale(top, v_norm[nt][j]);
+#pragma unroll
+                for (int mt = 0; mt < KT; ++mt) {
+                  acc[nt][mt][j] *= f;
+                  acc[nt][mt][j + 2] *= f;
+                }
+              }
             }
-            pbf[nt][b * 2] = movmatrix_trans(Mma<__half>::pack(sc[nt][b][0], sc[nt][b][1]));
-            pbf[nt][b * 2 + 1] = movmatrix_trans(Mma<__half>::pack(sc[nt][b][2], sc[nt][b][3]));
-          }
+          weights(std::false_type{});
         }
         // ---- V^T fragments: four transposed 8-token matrices of one 16-byte chunk; register j holds, for the two
         // head-dim lanes 2g and 2g+1, tokens 8j + 2t (low half) and 8j + 2t + 1 (high half): rows g and g+8 of the mma
@@ -795,10 +839,9 @@ q8_splitkv_kernel(const __grid_constant__ CUtensorMap tmap, const Params p, cons
             if (lane < 4) ml[warp * RT + nt * 8 + lane * 2 + j] = make_float2(m_run[nt][j], l);
           }
         if (!consumer_sync()) break;
-        // accumulators relative to the rows' common maximum (v_back undoes the power of two that this warp took the V scales
-        // by).  Row r, head-dim lane d of warp w is at [w][r][d], with d's 16-lane block XORed by r / 2 against bank conflicts
+        // accumulators relative to the rows' common maximum, without the power of two that this warp took the row's V scales
+        // by.  Row r, head-dim lane d of warp w is at [w][r][d], with d's 16-lane block XORed by r / 2 against bank conflicts
         float* sum = reinterpret_cast<float*>(smem + s * C::STAGE_BYTES);
-        const float v_back = power_of_two_inverse(v_norm);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -807,7 +850,7 @@ q8_splitkv_kernel(const __grid_constant__ CUtensorMap tmap, const Params p, cons
             float mt = -INFINITY;
 #pragma unroll
             for (int w = 0; w < kConsumerWarps; ++w) mt = fmaxf(mt, ml[w * RT + r].x);
-            const float f = fast_exp2(m_run[nt][j] - ((mt == -INFINITY) ? 0.f : mt)) * v_back;
+            const float f = fast_exp2(m_run[nt][j] - ((mt == -INFINITY) ? 0.f : mt)) * power_of_two_inverse(v_norm[nt][j]);
             // accumulator rows g / g+8 of block mt are head-dim lanes 16mt + 2g / + 1 (see the V fragments)
             float* row = sum + (warp * RT + r) * D + (lane >> 2) * 2;
 #pragma unroll

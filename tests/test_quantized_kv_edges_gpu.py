@@ -1,0 +1,109 @@
+"""The operators around the 8-bit cache at the edges of what a call may hold: scales far apart under a mask, offsets that
+describe no batch, NaN, the largest scale, table sizes around the shared-memory limit, a first call under capture.
+
+Attention is checked row by row: with the bounds of test_quantized_kv_gpu.py, but the last term, what underflows, is taken of the
+largest |V| among the keys that the ROW sees, so that a key which the mask hides from a row cannot excuse an error in it.
+"""
+
+import subprocess
+import sys
+import textwrap
+from pathlib import Path
+
+import numpy as np
+import pytest
+import torch
+
+import ejkernel_b200 as ej
+from ejkernel_b200 import _cabi
+from ejkernel_b200.kernels._cuda.quantized_kv import read_status
+from oracle import q8_oracle
+
+from .test_quantized_kv_gpu import CODES, HALVES, clean_status, make_batch, make_cache, make_requests, check_tables, option, oracle, run  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+ROOT = Path(__file__).resolve().parent.parent
+
+
+def visible_top(b, window=None):
+    """[T, Hq, 1]: the largest |V| among the keys that a row sees."""
+    v = np.abs(q8_oracle.values_of(b["codes"], b["scales"])[:, :, 1]).max(-1)  # [P, Hkv, page]
+    T, Hq, _ = b["q"].shape
+    Hkv = v.shape[1]
+    out = np.zeros((T, Hq, 1))
+    start, tab = b["start"].tolist(), b["tab"].numpy()
+    for s in range(b["n"]):
+        n, kv = start[s + 1] - start[s], int(b["ctx"][s])
+        keys = v[tab[s, : -(-kv // v.shape[2])]].transpose(1, 0, 2).reshape(Hkv, -1)[:, :kv]
+        for r in range(n):
+            pos = kv - n + r
+            seen = keys[:, max(0, pos - window + 1) if window else 0: pos + 1]
+            if seen.shape[1]:
+                out[start[s] + r, :, 0] = np.repeat(seen.max(1), Hq // Hkv)
+    return out
+
+
+def check_rows(b, out, **kw):
+    want, bound = oracle(b, **kw)
+    got = out.double().cpu().numpy()
+    assert np.isfinite(got).all()
+    exact_scales = bool((torch.frexp(b["scales"]).mantissa == 0.5).all())
+    room = (2.0**-10 if exact_scales else 2.0**-9) * bound + torch.finfo(out.dtype).eps / 2 * (1 + 2.0**-6) * np.abs(want) \
+        + 2.0**-24 * visible_top(b, kw.get("sliding_window")) + torch.finfo(out.dtype).tiny
+    worst = (np.abs(got - want) / room).max()
+    assert worst <= 1.0, worst
+
+
+def set_v_scales(b, of):
+    """V scale of the block that token j of every sequence lies in: of(sequence, first token of the block)."""
+    page, per = b["codes"].shape[3], b["scales"].shape[3]
+    block = page // per
+    for s in range(b["n"]):
+        for j in range(0, int(b["ctx"][s]), block):
+            b["scales"][int(b["tab"][s, j // page]), :, 1, j % page // block] = of(s, j)
+
+
+# ------------------------------------------------------------------- a row's result and the scales that it does not see
+
+
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("dim, Hq", [(64, 2), (128, 2), (256, 2), (64, 9), (128, 9), (256, 9)])
+@pytest.mark.parametrize("window", [None, 40])
+def test_split_kv_rows_do_not_feel_scales_that_their_mask_hides(code, dim, Hq, window):
+    """Few tokens share a row tile.  Causally the first ones must not lose what later tokens' large values push out of f16; with
+    a window the last ones must not feel the large values that have left their window."""
+    b = make_batch([(3, 200), (2, 33), (3, 3), (1, 90)], Hq=Hq, Hkv=1, dim=dim, page=16, block=1, code=code, half=torch.bfloat16, seed=dim + Hq)
+    ctx = b["ctx"].tolist()
+    set_v_scales(b, lambda s, j: 2.0**-40 if (j < ctx[s] - 2 if window is None else j > ctx[s] - 42) else 1.0)
+    kw = {} if window is None else dict(sliding_window=window)
+    check_rows(b, run(b, **kw), **kw)
+
+
+# ------------------------------------------------------------------------------------ rows that no sequence serves
+
+
+def poisoned(b, **kw):
+    """The call's output where the memory that it gets was full of NaN."""
+    run(b, **kw)
+    torch.cuda.synchronize()
+    for _ in range(3):  # the allocator gives a freed block of the size to the next call
+        t = torch.full(b["q"].shape, float("nan"), dtype=b["q"].dtype, device="cuda")
+        del t
+        out = run(b, **kw)
+        assert torch.isfinite(out).all()
+    return out
+
+
+# ------------------------------------------------------------------------------------------------------ dispatch
+
+
+def launches():
+    return _cabi.load().ejk_rpa_last_launch_count()
+
+
+@pytest.mark.parametrize("dim, Hq", [(64, 9), (64, 16), (256, 9), (256, 16)])
+@pytest.mark.parametrize("code, half", [(torch.int8, torch.bfloat16), (torch.int8, torch.float16), (torch.float8_e4m3fn, torch.bfloat16), (torch.float8_e4m3fn, torch.float16)])
+def test_more_than_eight_heads_per_kv_head(code, half, dim, Hq):
+    b = make_batch([(1, 300), (2, 77), (1, 9), (1, 2500)], Hq=2 * Hq, Hkv=2, dim=dim, page=16, block=8, code=code, half=half, seed=Hq)
+    check_rows(b, run(b))
