@@ -17,6 +17,10 @@
 //     v_scale / v_ref, v_ref a power of two that keeps the products within f16: the largest v_scale met so far is taken to
 //     [2^6, 2^7), and a power of two times a code is exact down to 2^-24.  When a larger scale comes, v_ref grows and the
 //     softmax threads rescale O, as they do when the maximum grows.
+//   * one v_ref for all rows of an item must not push what some of them see out of f16: where a scale of the stage is
+//     2^-11 and less of the largest one met so far ("far" stages: the mask can hide that one from a row), V goes to shared memory as
+//     codes alone, and each softmax thread puts v_scale into its weights, under a power of two of its own row.  O then is in
+//     units of the row's; the next common stage takes it to v_ref's.
 //   * P is f16.  Its reference sits 2^7 below the maximum it was chosen for, which puts the weights between 2^15 and 2^-24:
 //     what is below 2^-31 of the largest weight is lost.
 //   * registers: 16 warps have 128 registers a thread; the issuing warps and the converters give theirs to the softmax
@@ -58,6 +62,8 @@ constexpr float kLog2eP = 1.4426950408889634f;
 constexpr float kRefBelow = 7.0f;  // P's reference sits this far below the maximum it is chosen for ...
 constexpr float kLazyP = 15.0f;    // ... and is kept until the maximum has passed it by this much: P <= 2^15 < 65504
 constexpr int kVBits = 6;          // the largest v_scale met so far is taken to [2^6, 2^7): 448 * 2^7 < 65504
+constexpr float kFar = 0x1p-5f;    // a stage is far where a scale is below this in those units: its smallest codes leave f16's normals
+constexpr float kFarV = 0x1p7f;    // what a far stage's codes are multiplied by, and its weights divided
 
 // One piece of work of a CTA, as in rpa_prefill_sm100.cu.
 struct ItemDescP {
@@ -91,10 +97,11 @@ struct CfgP {
   static constexpr int OFF_RAW = OFF_KV + NS * STAGE_BYTES;
   static constexpr int OFF_RAWSCALE = OFF_RAW + NR * RAW_BYTES;      // per raw stage: BN scales of K, BN of V (at most)
   static constexpr int OFF_KSCALE = OFF_RAWSCALE + NR * 2 * BN * 4;  // per 16-bit stage: each token's factor on its logits
-  static constexpr int OFF_RING = OFF_KSCALE + NS * BN * 4;
+  static constexpr int OFF_VSCALE = OFF_KSCALE + NS * BN * 4;        // per far stage: each token's V scale
+  static constexpr int OFF_RING = OFF_VSCALE + NS * BN * 4;
   static constexpr int OFF_RMETA = OFF_RING + kRingP * (int)sizeof(ItemDescP);
   static constexpr int OFF_META = OFF_RMETA + NR * 8;
-  static constexpr int OFF_VREF = OFF_META + NS * 8;                 // per 16-bit stage: 1 / v_ref
+  static constexpr int OFF_VREF = OFF_META + NS * 8;                 // per 16-bit stage: 1 / v_ref, negative: a far stage
   static constexpr int OFF_BAR = (OFF_VREF + NS * 4 + 7) / 8 * 8;
   // barriers: kv_full[NS] kv_empty[NS] raw_full[NR] raw_empty[NR], then per tile: s_full s_free p_full[2] pv_done[2]
   // q_full o_free
@@ -167,6 +174,102 @@ __device__ __forceinline__ float fast_reciprocal(float x) {
 __device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, __half2 b) {
   const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), b);
   return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+// A far stage of a softmax thread: what the kernel does with the others' (which see there), but with the tokens' V scales in the
+// weights, under a power of two of the row's own.  Such stages are rare, and the length of the softmax warps' code bounds the
+// kernel (in line, 4 prompt chunks took 543 to 585 us instead of 500), so that this is a call that works on a copy of the logits
+// in local memory.
+struct FarRow {
+  float m, l, v;  // reference of the weights, their sum, the units of O
+  bool ok;        // false: a wait ran out
+};
+template <int D, bool PLAIN>
+__device__ __noinline__ FarRow far_stage(FarRow r, const float* kf, const float* vs, float q_fac, float cap_log2, int hi_i, int lo_i,
+                                         uint32_t tm_s, uint32_t tm_p, uint32_t tm_o, uint32_t bar_s_free, uint32_t bar_p_full,
+                                         uint32_t bar_pv_before, uint32_t bar_pv_last, int ti, bool first, volatile int* abort_flag,
+                                         unsigned long long wait_ns) {
+  constexpr int BN = CfgP<D>::BN;
+  const int lane = threadIdx.x & 31;
+  float y[BN], mx = -INFINITY, top = 0.f;
+#pragma unroll 1
+  for (int c0 = 0; c0 < BN; c0 += 16) {
+    uint32_t s[16];
+    tc_ld16(tm_s + c0, s);
+    tc_wait_ld();
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const int i = c0 + j;
+      // in the common kernel the factor is one per 8 columns, and the soft cap is elsewhere
+      const float f = kf[PLAIN ? i >> 3 : i] * q_fac;
+      float v = __uint_as_float(s[j]) * f;
+      if (!PLAIN && cap_log2 != 0.f) v = fmaf(fast_reciprocal(fast_exp2(v) + 1.f), -2.f * cap_log2, cap_log2);
+      if (i > hi_i || i <= lo_i) v = -INFINITY;
+      else top = fmaxf(top, vs[i]);
+      mx = fmaxf(mx, v);
+      y[i] = v;
+    }
+  }
+  tc_fence_before();
+  __syncwarp();
+  if (lane == 0) mbar_arrive(bar_s_free);
+  r.ok = ti < 2 || mbar_wait(bar_pv_before, ((ti - 2) >> 1) & 1, abort_flag, wait_ns);
+  if (!r.ok) return r;
+  // The row's units: its largest V scale to [2^6, 2^7).  v_ref is never above that, so the next common stage cannot ask for
+  // finer units than these.
+  float v_new = r.v;
+  if (top > 0.f) {
+    if (r.m == -INFINITY) v_new = __uint_as_float((127u + 125u) << 23);  // the row has seen no scale yet
+    if (top * v_new >= (float)(2 << kVBits)) {
+      uint32_t e = __float_as_uint(top) >> 23;
+      e = e < 8u ? 8u : e;
+      v_new = __uint_as_float((254u + kVBits - e) << 23);
+    }
+  }
+  const bool grow = (mx > r.m + kLazyP) || (r.m == -INFINITY && mx > -INFINITY);
+  if (__any_sync(0xffffffffu, grow || v_new != r.v)) {
+    float alpha = r.m > -INFINITY ? v_new * power_of_two_inverse(r.v) : 1.f;
+    if (grow) {
+      const float f = fast_exp2(r.m - (mx - kRefBelow));
+      r.m = mx - kRefBelow;
+      r.l *= f;
+      alpha *= f;
+    }
+    r.v = v_new;
+    if (!first) {
+      r.ok = mbar_wait(bar_pv_last, ((ti - 1) >> 1) & 1, abort_flag, wait_ns);
+      if (!r.ok) return r;
+      tc_fence_after();
+#pragma unroll 1
+      for (int c0 = 0; c0 < D; c0 += 16) {
+        uint32_t o[16];
+        tc_ld16(tm_o + c0, o);
+        tc_wait_ld();
+#pragma unroll
+        for (int c = 0; c < 16; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * alpha);
+        tc_st16(tm_o + c0, o);
+      }
+    }
+  }
+  const float m_use = r.m == -INFINITY ? 0.f : r.m, unit = r.v * (1.f / kFarV);
+#pragma unroll 1
+  for (int c0 = 0; c0 < BN; c0 += 32) {
+    uint32_t pk[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const int i = c0 + 2 * j;
+      const float p0 = fast_exp2(y[i] - m_use), p1 = fast_exp2(y[i + 1] - m_use);
+      r.l += p0 + p1;
+      // a key without weight has none whatever its scale: it may be one that the row does not see
+      pk[j] = Mma<__half>::pack(p0 == 0.f ? 0.f : p0 * (vs[i] * unit), p1 == 0.f ? 0.f : p1 * (vs[i + 1] * unit));
+    }
+    tc_st16(tm_p + (c0 >> 1), pk);
+  }
+  tc_wait_st();
+  tc_fence_before();
+  __syncwarp();
+  if (lane == 0) mbar_arrive(bar_p_full);
+  return r;
 }
 
 // PLAIN: scale blocks of 8 tokens or more, no soft cap, a positive scale
@@ -650,12 +753,17 @@ q8_prefill_kernel(const Params p, const Q8Cache cache) {
         lo_min = (p.window > 0) ? (u.kv_len - u.q_len + u.row0 / G - p.window) : -1;
         v_norm = __uint_as_float((127u + 125u) << 23);  // no scale met yet: the largest power of two
       }
-      // the largest V scale of the stage's keys that some row sees; every warp computes the same
+      // the largest V scale of the stage's keys that some row sees, and this lane's smallest; every warp computes the same
       uint32_t tb = 0;
+      float low = INFINITY;
 #pragma unroll
       for (int i = 0; i < kBN / 32; ++i) {
         const int key = pos + lane + 32 * i;
-        if (key < kv_end && key > lo_min) tb = max(tb, __float_as_uint(vs_s[(key >> sb_shift) - e0]));
+        if (key < kv_end && key > lo_min) {
+          const float v = vs_s[(key >> sb_shift) - e0];
+          tb = max(tb, __float_as_uint(v));
+          low = fminf(low, v);
+        }
       }
       tb = __reduce_max_sync(0xffffffffu, tb);  // positive floats order as integers
       if (__uint_as_float(tb) * v_norm >= (float)(2 << kVBits)) {
@@ -663,15 +771,21 @@ q8_prefill_kernel(const Params p, const Q8Cache cache) {
         e = e < 8u ? 8u : e;
         v_norm = __uint_as_float((254u + kVBits - e) << 23);
       }
+      const bool far = __any_sync(0xffffffffu, low * v_norm < kFar);
+      const float f_scale = far ? 0.f : v_norm, f_plus = far ? kFarV : 0.f;
       if (!mbar_wait(bar_kv_empty(st), ((gi / NS) & 1) ^ 1, abort_flag, wait_ns)) break;
       // each token's factor on its logits; in the common kernel one per 8 tokens
       if (ctid < (coarse ? kBN / 8 : kBN)) {
         const int key = pos + (coarse ? ctid * 8 : ctid);
         reinterpret_cast<float*>(smem + C::OFF_KSCALE + st * (kBN * 4))[ctid] = key < kv_end ? ks_s[(key >> sb_shift) - e0] * to_log2 : 1.f;
       }
+      if (far && ctid < kBN) {
+        const int key = pos + ctid;
+        reinterpret_cast<float*>(smem + C::OFF_VSCALE + st * (kBN * 4))[ctid] = key < kv_end && key > lo_min ? vs_s[(key >> sb_shift) - e0] : 0.f;
+      }
       if (ctid == 0) {
         metas[st] = meta;
-        vrefs[st] = v_norm;
+        vrefs[st] = far ? -v_norm : v_norm;
       }
       const uint8_t* raw = smem + C::OFF_RAW + rs * C::RAW_BYTES + ch * 16;
       uint8_t* out = smem + C::OFF_KV + st * C::STAGE_BYTES + (ch >> 2) * 1024;
@@ -681,7 +795,7 @@ q8_prefill_kernel(const Params p, const Q8Cache cache) {
         const uint4 kc = *reinterpret_cast<const uint4*>(raw + t * D);
         uint4 vc = *reinterpret_cast<const uint4*>(raw + (kBN + t) * D);
         const int key = pos + t;
-        float f = vs_s[(key >> sb_shift) - e0] * v_norm;
+        float f = fmaf(vs_s[(key >> sb_shift) - e0], f_scale, f_plus);
         if (key >= kv_end || key <= lo_min) {  // V of a key that no row sees is zero: those are stale bytes, possibly NaN
           vc = make_uint4(0u, 0u, 0u, 0u);
           f = 0.f;
@@ -835,288 +949,309 @@ q8_prefill_kernel(const Params p, const Q8Cache cache) {
       }
       q_ready = false;
       q_fac = q_fac_next;
-      for (int js = 0; js < n_stages; ++js, ++gi, ++ti) {
-        const int st = gi % NS;
-        const int pos = u.kv_begin + js * kBN;  // first key of the stage
-        const bool first = (js == 0);
-        if (!mbar_wait(bar_s_full(x), ti & 1, abort_flag, wait_ns)) { alive = false; break; }
-        tc_fence_after();
-
-        // ---- the row's logits of the stage into registers; then the S columns are free for the
-        // tile's next S MMA, which runs while this stage's exponentials are computed
-        uint32_t sr[HB];
-#pragma unroll
-        for (int c = 0; c + 32 <= HB; c += 32) tc_ld32(tm_s + c, *reinterpret_cast<uint32_t(*)[32]>(&sr[c]));
-        static_assert(HB % 32 == 0, "S is read 32 columns at a time");
-        tc_wait_ld();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar_s_free(x));
-
-        // ---- logits in the log2 domain: raw dot products times the token's factor (k_scale * scale * log2 e) and the row's.
-        // Common case: the products stay in the registers, a factor per 8 columns goes into the exponent's FMA and only the
-        // groups' maxima are multiplied; a soft cap, finer scales or a scale that is not positive materialise the logits.
-        const float v_new = vrefs[st];
-        const float4* kf4 = reinterpret_cast<const float4*>(smem + C::OFF_KSCALE + st * (kBN * 4));
-        const bool full_vis = (pos + HB - 1 <= pos_row) && (pos > lo_row);
-        float ef[HB / 8];
-#pragma unroll
-        for (int i = 0; i < HB / 8; ++i) ef[i] = 1.f;
-        if constexpr (PLAIN) {
-#pragma unroll
-          for (int i = 0; i < HB / 8; i += 4) {
-            const float4 f = kf4[i >> 2];
-            // not below the smallest normal number: a masked logit, -inf, times 0 would be NaN
-            ef[i] = fmaxf(f.x * q_fac, 1.17549435e-38f);
-            ef[i + 1] = fmaxf(f.y * q_fac, 1.17549435e-38f);
-            ef[i + 2] = fmaxf(f.z * q_fac, 1.17549435e-38f);
-            ef[i + 3] = fmaxf(f.w * q_fac, 1.17549435e-38f);
-          }
-        }
-        if constexpr (!PLAIN) {
-          const uint64_t qf = pack_f32x2(q_fac, q_fac);
-#pragma unroll
-          for (int i = 0; i < HB; i += 4) {
-            const float4 f = kf4[i >> 2];
-            const float2 a = unpack_f32x2(mul_f32x2(pack_f32x2(__uint_as_float(sr[i]), __uint_as_float(sr[i + 1])), mul_f32x2(pack_f32x2(f.x, f.y), qf)));
-            const float2 b = unpack_f32x2(mul_f32x2(pack_f32x2(__uint_as_float(sr[i + 2]), __uint_as_float(sr[i + 3])), mul_f32x2(pack_f32x2(f.z, f.w), qf)));
-            sr[i] = __float_as_uint(a.x);
-            sr[i + 1] = __float_as_uint(a.y);
-            sr[i + 2] = __float_as_uint(b.x);
-            sr[i + 3] = __float_as_uint(b.y);
-          }
-          if (p.cap != 0.f) {
-            // cap * tanh(t) = cap - 2 cap / (2^(2 t log2 e) + 1); the factors hold the 2 log2 e.  An infinite power gives cap
-            const uint64_t one = pack_f32x2(1.f, 1.f), cap = pack_f32x2(p.cap_log2, p.cap_log2), twice = pack_f32x2(-2.f * p.cap_log2, -2.f * p.cap_log2);
-#pragma unroll
-            for (int i = 0; i < HB; i += 2) {
-              const float2 e = unpack_f32x2(add_f32x2(pack_f32x2(fast_exp2(__uint_as_float(sr[i])), fast_exp2(__uint_as_float(sr[i + 1]))), one));
-              const float2 y = unpack_f32x2(fma_f32x2(pack_f32x2(fast_reciprocal(e.x), fast_reciprocal(e.y)), twice, cap));
-              sr[i] = __float_as_uint(y.x);
-              sr[i + 1] = __float_as_uint(y.y);
-            }
-          }
-        }
-        if (__builtin_expect(!full_vis, 0)) {
-          const int hi_i = pos_row - pos;  // last visible column of the stage
-          const int lo_i = lo_row - pos;   // columns up to here are left of the window
-#pragma unroll
-          for (int i = 0; i < HB; ++i)
-            if (i > hi_i || i <= lo_i) sr[i] = __float_as_uint(-INFINITY);
-        }
-        float mx = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < HB; i += 8) {
-          float a = fmaxf(__uint_as_float(sr[i]), __uint_as_float(sr[i + 1]));
-          float b = fmaxf(__uint_as_float(sr[i + 2]), __uint_as_float(sr[i + 3]));
-          a = fmax3(a, __uint_as_float(sr[i + 4]), __uint_as_float(sr[i + 5]));
-          b = fmax3(b, __uint_as_float(sr[i + 6]), __uint_as_float(sr[i + 7]));
-          mx = fmaxf(mx, fmaxf(a, b) * ef[i >> 3]);
-        }
-        // P_x has two buffers: this stage's goes where the stage before the previous one's was, whose
-        // P.V must have read it (it has, normally long ago)
-        if (ti >= 2) {
-          if (!mbar_wait(bar_pv_done(x, ti & 1), ((ti - 2) >> 1) & 1, abort_flag, wait_ns)) { alive = false; break; }
-        }
-        const uint32_t tm_p = tm_p0 + (ti & 1) * C::P_COLS;
-        // the row's maximum has outgrown its reference, or V comes under a larger reference than O's
-        const bool grow = (mx > m_run + kLazyP) || (m_run == -INFINITY && mx > -INFINITY);
-        if (__any_sync(0xffffffffu, grow || v_new != v_norm)) {
-          float alpha = 1.f;
-          if (grow) {
-            alpha = fast_exp2(m_run - (mx - kRefBelow));  // 0 on the first finite maximum
-            m_run = mx - kRefBelow;
-            l_run *= alpha;
-          }
-          if (!first) alpha *= v_new * power_of_two_inverse(v_norm);
-          v_norm = v_new;
-          if (!first) {
-            // O holds the sum over the earlier stages of this item: rescale the row, once the tile's
-            // previous P.V has completed (O is only touched between P.Vs)
-            if (!mbar_wait(bar_pv_done(x, (ti - 1) & 1), ((ti - 1) >> 1) & 1, abort_flag, wait_ns)) { alive = false; break; }
-            tc_fence_after();
-#pragma unroll 1
-            for (int c0 = 0; c0 < D; c0 += 16) {
-              uint32_t o[16];
-              tc_ld16(tm_o + c0, o);
-              tc_wait_ld();
-#pragma unroll
-              for (int c = 0; c < 16; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * alpha);
-              tc_st16(tm_o + c0, o);
-            }
-          }
-        }
-        const float m_use = (m_run == -INFINITY) ? 0.f : m_run;
-        // probabilities, packed as 16-bit pairs, into the tile's P buffer of this stage
-        // (pairs of columns in one instruction where there is one: this loop's length bounds the kernel)
-        const uint64_t neg_m = pack_f32x2(-m_use, -m_use);
-        uint64_t lsum[2] = {0ull, 0ull};
-#pragma unroll
-        for (int c = 0; c < HB; c += 32) {
-          uint32_t pk[16];
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const float f = ef[(c + 2 * j) >> 3];
-            const uint64_t y = fma_f32x2(pack_f32x2(__uint_as_float(sr[c + 2 * j]), __uint_as_float(sr[c + 2 * j + 1])), pack_f32x2(f, f), neg_m);
-            const float2 e = unpack_f32x2(y);
-            const float p0 = fast_exp2(e.x), p1 = fast_exp2(e.y);
-            lsum[j & 1] = add_f32x2(lsum[j & 1], pack_f32x2(p0, p1));
-            pk[j] = Mma<__half>::pack(p0, p1);
-          }
-          tc_st16(tm_p + (c >> 1), pk);
-        }
-        const float2 lsum_pair = unpack_f32x2(add_f32x2(lsum[0], lsum[1]));
-        l_run += lsum_pair.x + lsum_pair.y;
-        tc_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar_p_full(x, ti & 1));
-
-        if (pos + kBN >= u.kv_end) {
-          // ---- last stage of the piece.  All S of the item completed long ago, so the tile's query buffer is free: fetch
-          // the next item's query row (if the producer has published that item already; it normally has, it runs stages
-          // ahead), then wait for the last P.V, normalise and store, or (a part of a split item) publish the unnormalised
-          // part and, if it is the last to arrive, combine ----
-          bool q_pending = *items_pub > k;
-          q_pending = __all_sync(0xffffffffu, q_pending);
-          if (q_pending) {
-            __threadfence_block();
-            const Unit un = ring[k % kRingP].u;
-            q_pending = un.seq >= 0 && (x == 0 || (un.slot > kBM && un.q_len * G > un.row0 + kBM));
-            if (q_pending) {
-              q_fetch(un, ring[k % kRingP].h);
-              q_ready = true;
-            }
-          }
-          if (!mbar_wait(bar_pv_done(x, ti & 1), (ti >> 1) & 1, abort_flag, wait_ns)) { alive = false; break; }
+      // runs of common stages, and the far ones between them
+      int js = 0;
+      while (true) {
+        bool far = false;
+        for (; js < n_stages; ++js, ++gi, ++ti) {
+          const int st = gi % NS;
+          const int pos = u.kv_begin + js * kBN;  // first key of the stage
+          const bool first = (js == 0);
+          if (!mbar_wait(bar_s_full(x), ti & 1, abort_flag, wait_ns)) { alive = false; break; }
           tc_fence_after();
-          const float v_back = power_of_two_inverse(v_norm);  // O is in units of v_ref
-          if (u.n_chunks > 1) {
-            // Slot of the part CTA c holds of this (item, head): a CTA has at most two parts, the item
-            // its quota begins in (slot 2c) and the item its quota ends in (slot 2c + 1).
-            auto slot_of = [&](int c) { return ((long long)first_stage <= (long long)c * quota) ? 2 * c : 2 * c + 1; };
-            const size_t mine = ((size_t)slot_of((int)blockIdx.x) * NT + x) * kBM + row;
-            if (row_ok) p.ppart_ml[mine] = make_float2(m_run, l_run);
-#pragma unroll 1
-            for (int c0 = 0; c0 < D; c0 += 32) {
-              uint32_t o[32];
-              tc_ld32(tm_o + c0, o);
-              tc_wait_ld();
-              if (row_ok) {
-                float4* dst = reinterpret_cast<float4*>(p.ppart_o + mine * D + c0);
+          // ---- the row's logits of the stage into registers; then the S columns are free for the
+          // tile's next S MMA, which runs while this stage's exponentials are computed
+          uint32_t sr[HB];
 #pragma unroll
-                for (int c = 0; c < 32; c += 4)
-                  dst[c >> 2] = make_float4(__uint_as_float(o[c]) * v_back, __uint_as_float(o[c + 1]) * v_back,
-                                            __uint_as_float(o[c + 2]) * v_back, __uint_as_float(o[c + 3]) * v_back);
-              }
-            }
-            tc_fence_before();
-            __threadfence();
-            __syncwarp();
-            int old = 0;
-            if (lane == 0) {
-              mbar_arrive(bar_o_free(x));
-              // one counter per 32-row quarter of the tile: the warps of a group never wait for each other
-              old = atomicAdd(&p.ptickets[((size_t)u.merge_idx * NT + x) * 4 + (warp & 3)], 1);
-            }
-            old = __shfl_sync(0xffffffffu, old, 0);
-            if (old == u.n_chunks - 1 && row_ok) {
-              // last part to arrive: combine the parts of this row, in part order (so the result does not
-              // depend on which part arrived last)
-              __threadfence();
-              const int c_first = first_stage / quota;
-              float m_tot = -INFINITY;
-              for (int pi = 0; pi < u.n_chunks; ++pi)
-                m_tot = fmaxf(m_tot, __ldcg(&p.ppart_ml[((size_t)slot_of(c_first + pi) * NT + x) * kBM + row]).x);
-              const float mu = (m_tot == -INFINITY) ? 0.f : m_tot;
-              float l_tot = 0.f;
-              for (int pi = 0; pi < u.n_chunks; ++pi) {
-                const float2 ml = __ldcg(&p.ppart_ml[((size_t)slot_of(c_first + pi) * NT + x) * kBM + row]);
-                l_tot += ml.y * fast_exp2(ml.x - mu);
-              }
-              float scl = 1.f, l_fin = l_tot;
-              if (p.num_sinks > 0) {
-                const int srow = (p.sink_rows == p.Hq) ? out_head : (p.sink_rows == Hkv ? h : 0);
-                const float* sk = p.sinks + (size_t)srow * p.num_sinks;
-                float sm = -INFINITY;
-                for (int i = 0; i < p.num_sinks; ++i) sm = fmaxf(sm, sk[i] * kLog2eP);
-                const float m_fin = fmaxf(m_tot, sm);
-                const float mf = (m_fin == -INFINITY) ? 0.f : m_fin;
-                scl = fast_exp2(m_tot - mf);
-                l_fin = l_tot * scl;
-                for (int i = 0; i < p.num_sinks; ++i) l_fin += fast_exp2(sk[i] * kLog2eP - mf);
-              }
-              scl = (l_fin > 0.f) ? scl / l_fin : 0.f;
-              T* orow = reinterpret_cast<T*>(p.out) + ((size_t)out_row_q * p.Hq + out_head) * D;
-#pragma unroll 1
-              for (int c0 = 0; c0 < D; c0 += 32) {
-                float acc[32];
-#pragma unroll
-                for (int c = 0; c < 32; ++c) acc[c] = 0.f;
-                for (int pi = 0; pi < u.n_chunks; ++pi) {
-                  const size_t at = ((size_t)slot_of(c_first + pi) * NT + x) * kBM + row;
-                  const float f = fast_exp2(__ldcg(&p.ppart_ml[at]).x - mu);
-                  const float4* src = reinterpret_cast<const float4*>(p.ppart_o + at * D + c0);
-#pragma unroll
-                  for (int c = 0; c < 32; c += 4) {
-                    const float4 v = __ldcg(src + (c >> 2));
-                    acc[c] += v.x * f;
-                    acc[c + 1] += v.y * f;
-                    acc[c + 2] += v.z * f;
-                    acc[c + 3] += v.w * f;
-                  }
-                }
-#pragma unroll
-                for (int c = 0; c < 32; c += 8) {
-                  uint4 v;
-                  v.x = Mma<T>::pack(acc[c] * scl, acc[c + 1] * scl);
-                  v.y = Mma<T>::pack(acc[c + 2] * scl, acc[c + 3] * scl);
-                  v.z = Mma<T>::pack(acc[c + 4] * scl, acc[c + 5] * scl);
-                  v.w = Mma<T>::pack(acc[c + 6] * scl, acc[c + 7] * scl);
-                  *reinterpret_cast<uint4*>(orow + c0 + c) = v;
-                }
-              }
-            }
-            continue;  // next stage = first stage of the next piece
+          for (int c = 0; c + 32 <= HB; c += 32) tc_ld32(tm_s + c, *reinterpret_cast<uint32_t(*)[32]>(&sr[c]));
+          static_assert(HB % 32 == 0, "S is read 32 columns at a time");
+          const float v_stage = vrefs[st];  // on its way with S
+          const float4* kf4 = reinterpret_cast<const float4*>(smem + C::OFF_KSCALE + st * (kBN * 4));
+          tc_wait_ld();
+          if (__builtin_expect(v_stage < 0.f, 0)) {
+            far = true;
+            break;
           }
-          const float l_row = l_run;
-          float scl = 1.f, l_fin = l_row;
-          if (p.num_sinks > 0 && row_ok) {
-            // attention sinks join the denominator only
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar_s_free(x));
+
+          // ---- logits in the log2 domain: raw dot products times the token's factor (k_scale * scale * log2 e) and the row's.
+          // Common case: the products stay in the registers, a factor per 8 columns goes into the exponent's FMA and only the
+          // groups' maxima are multiplied; a soft cap, finer scales or a scale that is not positive materialise the logits.
+          const bool full_vis = (pos + HB - 1 <= pos_row) && (pos > lo_row);
+          float ef[HB / 8];
+#pragma unroll
+          for (int i = 0; i < HB / 8; ++i) ef[i] = 1.f;
+          if constexpr (PLAIN) {
+#pragma unroll
+            for (int i = 0; i < HB / 8; i += 4) {
+              const float4 f = kf4[i >> 2];
+              // not below the smallest normal number: a masked logit, -inf, times 0 would be NaN
+              ef[i] = fmaxf(f.x * q_fac, 1.17549435e-38f);
+              ef[i + 1] = fmaxf(f.y * q_fac, 1.17549435e-38f);
+              ef[i + 2] = fmaxf(f.z * q_fac, 1.17549435e-38f);
+              ef[i + 3] = fmaxf(f.w * q_fac, 1.17549435e-38f);
+            }
+          }
+          if constexpr (!PLAIN) {
+            const uint64_t qf = pack_f32x2(q_fac, q_fac);
+#pragma unroll
+            for (int i = 0; i < HB; i += 4) {
+              const float4 f = kf4[i >> 2];
+              const float2 a = unpack_f32x2(mul_f32x2(pack_f32x2(__uint_as_float(sr[i]), __uint_as_float(sr[i + 1])), mul_f32x2(pack_f32x2(f.x, f.y), qf)));
+              const float2 b = unpack_f32x2(mul_f32x2(pack_f32x2(__uint_as_float(sr[i + 2]), __uint_as_float(sr[i + 3])), mul_f32x2(pack_f32x2(f.z, f.w), qf)));
+              sr[i] = __float_as_uint(a.x);
+              sr[i + 1] = __float_as_uint(a.y);
+              sr[i + 2] = __float_as_uint(b.x);
+              sr[i + 3] = __float_as_uint(b.y);
+            }
+            if (p.cap != 0.f) {
+              // cap * tanh(t) = cap - 2 cap / (2^(2 t log2 e) + 1); the factors hold the 2 log2 e.  An infinite power gives cap
+              const uint64_t one = pack_f32x2(1.f, 1.f), cap = pack_f32x2(p.cap_log2, p.cap_log2), twice = pack_f32x2(-2.f * p.cap_log2, -2.f * p.cap_log2);
+#pragma unroll
+              for (int i = 0; i < HB; i += 2) {
+                const float2 e = unpack_f32x2(add_f32x2(pack_f32x2(fast_exp2(__uint_as_float(sr[i])), fast_exp2(__uint_as_float(sr[i + 1]))), one));
+                const float2 y = unpack_f32x2(fma_f32x2(pack_f32x2(fast_reciprocal(e.x), fast_reciprocal(e.y)), twice, cap));
+                sr[i] = __float_as_uint(y.x);
+                sr[i + 1] = __float_as_uint(y.y);
+              }
+            }
+          }
+          if (__builtin_expect(!full_vis, 0)) {
+            const int hi_i = pos_row - pos;  // last visible column of the stage
+            const int lo_i = lo_row - pos;   // columns up to here are left of the window
+#pragma unroll
+            for (int i = 0; i < HB; ++i)
+              if (i > hi_i || i <= lo_i) sr[i] = __float_as_uint(-INFINITY);
+          }
+          float mx = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < HB; i += 8) {
+            float a = fmaxf(__uint_as_float(sr[i]), __uint_as_float(sr[i + 1]));
+            float b = fmaxf(__uint_as_float(sr[i + 2]), __uint_as_float(sr[i + 3]));
+            a = fmax3(a, __uint_as_float(sr[i + 4]), __uint_as_float(sr[i + 5]));
+            b = fmax3(b, __uint_as_float(sr[i + 6]), __uint_as_float(sr[i + 7]));
+            mx = fmaxf(mx, fmaxf(a, b) * ef[i >> 3]);
+          }
+          // P_x has two buffers: this stage's goes where the stage before the previous one's was, whose
+          // P.V must have read it (it has, normally long ago)
+          if (ti >= 2) {
+            if (!mbar_wait(bar_pv_done(x, ti & 1), ((ti - 2) >> 1) & 1, abort_flag, wait_ns)) { alive = false; break; }
+          }
+          const uint32_t tm_p = tm_p0 + (ti & 1) * C::P_COLS;
+          // O comes into the stage's units if the row sees a key of it; they never grow finer over an item
+          const float v_new = mx > -INFINITY ? v_stage : v_norm;
+          // the row's maximum has outgrown its reference, or V comes in other units than O's
+          const bool grow = (mx > m_run + kLazyP) || (m_run == -INFINITY && mx > -INFINITY);
+          if (__any_sync(0xffffffffu, grow || v_new != v_norm)) {
+            float alpha = 1.f;
+            if (m_run > -INFINITY) alpha = v_new * power_of_two_inverse(v_norm);  // O is zero otherwise
+            if (grow) {
+              const float f = fast_exp2(m_run - (mx - kRefBelow));  // 0 on the first finite maximum
+              m_run = mx - kRefBelow;
+              l_run *= f;
+              alpha *= f;
+            }
+            v_norm = v_new;
+            if (!first) {
+              // O holds the sum over the earlier stages of this item: rescale the row, once the tile's
+              // previous P.V has completed (O is only touched between P.Vs)
+              if (!mbar_wait(bar_pv_done(x, (ti - 1) & 1), ((ti - 1) >> 1) & 1, abort_flag, wait_ns)) { alive = false; break; }
+              tc_fence_after();
+#pragma unroll 1
+              for (int c0 = 0; c0 < D; c0 += 16) {
+                uint32_t o[16];
+                tc_ld16(tm_o + c0, o);
+                tc_wait_ld();
+#pragma unroll
+                for (int c = 0; c < 16; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * alpha);
+                tc_st16(tm_o + c0, o);
+              }
+            }
+          }
+          const float m_use = (m_run == -INFINITY) ? 0.f : m_run;
+          // probabilities, packed as 16-bit pairs, into the tile's P buffer of this stage
+          // (pairs of columns in one instruction where there is one: this loop's length bounds the kernel)
+          const uint64_t neg_m = pack_f32x2(-m_use, -m_use);
+          uint64_t lsum[2] = {0ull, 0ull};
+#pragma unroll
+          for (int c = 0; c < HB; c += 32) {
+            uint32_t pk[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              const float f = ef[(c + 2 * j) >> 3];
+              const uint64_t y = fma_f32x2(pack_f32x2(__uint_as_float(sr[c + 2 * j]), __uint_as_float(sr[c + 2 * j + 1])), pack_f32x2(f, f), neg_m);
+              const float2 e = unpack_f32x2(y);
+              const float p0 = fast_exp2(e.x), p1 = fast_exp2(e.y);
+              lsum[j & 1] = add_f32x2(lsum[j & 1], pack_f32x2(p0, p1));
+              pk[j] = Mma<__half>::pack(p0, p1);
+            }
+            tc_st16(tm_p + (c >> 1), pk);
+          }
+          const float2 lsum_pair = unpack_f32x2(add_f32x2(lsum[0], lsum[1]));
+          l_run += lsum_pair.x + lsum_pair.y;
+          tc_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar_p_full(x, ti & 1));
+        }
+        if (!far) break;
+        const int st = gi % NS;
+        const FarRow r = far_stage<D, PLAIN>(
+            {m_run, l_run, v_norm, true}, reinterpret_cast<const float*>(smem + C::OFF_KSCALE + st * (kBN * 4)),
+            reinterpret_cast<const float*>(smem + C::OFF_VSCALE + st * (kBN * 4)), q_fac, p.cap_log2, pos_row - (u.kv_begin + js * kBN),
+            lo_row - (u.kv_begin + js * kBN), tm_s, tm_p0 + (ti & 1) * C::P_COLS, tm_o, bar_s_free(x), bar_p_full(x, ti & 1),
+            bar_pv_done(x, ti & 1), bar_pv_done(x, (ti - 1) & 1), ti, js == 0, abort_flag, wait_ns);
+        if (!r.ok) { alive = false; break; }
+        m_run = r.m;
+        l_run = r.l;
+        v_norm = r.v;
+        ++js, ++gi, ++ti;
+      }
+      if (!alive) break;
+      // ---- last stage of the piece.  All S of the item completed long ago, so the tile's query buffer is free: fetch
+      // the next item's query row (if the producer has published that item already; it normally has, it runs stages
+      // ahead), then wait for the last P.V, normalise and store, or (a part of a split item) publish the unnormalised
+      // part and, if it is the last to arrive, combine ----
+      bool q_pending = *items_pub > k;
+      q_pending = __all_sync(0xffffffffu, q_pending);
+      if (q_pending) {
+        __threadfence_block();
+        const Unit un = ring[k % kRingP].u;
+        q_pending = un.seq >= 0 && (x == 0 || (un.slot > kBM && un.q_len * G > un.row0 + kBM));
+        if (q_pending) {
+          q_fetch(un, ring[k % kRingP].h);
+          q_ready = true;
+        }
+      }
+      if (!mbar_wait(bar_pv_done(x, (ti - 1) & 1), ((ti - 1) >> 1) & 1, abort_flag, wait_ns)) { alive = false; break; }
+      tc_fence_after();
+      const float v_back = power_of_two_inverse(v_norm);  // O is in units of v_ref
+      if (u.n_chunks > 1) {
+        // Slot of the part CTA c holds of this (item, head): a CTA has at most two parts, the item
+        // its quota begins in (slot 2c) and the item its quota ends in (slot 2c + 1).
+        auto slot_of = [&](int c) { return ((long long)first_stage <= (long long)c * quota) ? 2 * c : 2 * c + 1; };
+        const size_t mine = ((size_t)slot_of((int)blockIdx.x) * NT + x) * kBM + row;
+        if (row_ok) p.ppart_ml[mine] = make_float2(m_run, l_run);
+#pragma unroll 1
+        for (int c0 = 0; c0 < D; c0 += 32) {
+          uint32_t o[32];
+          tc_ld32(tm_o + c0, o);
+          tc_wait_ld();
+          if (row_ok) {
+            float4* dst = reinterpret_cast<float4*>(p.ppart_o + mine * D + c0);
+#pragma unroll
+            for (int c = 0; c < 32; c += 4)
+              dst[c >> 2] = make_float4(__uint_as_float(o[c]) * v_back, __uint_as_float(o[c + 1]) * v_back,
+                                        __uint_as_float(o[c + 2]) * v_back, __uint_as_float(o[c + 3]) * v_back);
+          }
+        }
+        tc_fence_before();
+        __threadfence();
+        __syncwarp();
+        int old = 0;
+        if (lane == 0) {
+          mbar_arrive(bar_o_free(x));
+          // one counter per 32-row quarter of the tile: the warps of a group never wait for each other
+          old = atomicAdd(&p.ptickets[((size_t)u.merge_idx * NT + x) * 4 + (warp & 3)], 1);
+        }
+        old = __shfl_sync(0xffffffffu, old, 0);
+        if (old == u.n_chunks - 1 && row_ok) {
+          // last part to arrive: combine the parts of this row, in part order (so the result does not
+          // depend on which part arrived last)
+          __threadfence();
+          const int c_first = first_stage / quota;
+          float m_tot = -INFINITY;
+          for (int pi = 0; pi < u.n_chunks; ++pi)
+            m_tot = fmaxf(m_tot, __ldcg(&p.ppart_ml[((size_t)slot_of(c_first + pi) * NT + x) * kBM + row]).x);
+          const float mu = (m_tot == -INFINITY) ? 0.f : m_tot;
+          float l_tot = 0.f;
+          for (int pi = 0; pi < u.n_chunks; ++pi) {
+            const float2 ml = __ldcg(&p.ppart_ml[((size_t)slot_of(c_first + pi) * NT + x) * kBM + row]);
+            l_tot += ml.y * fast_exp2(ml.x - mu);
+          }
+          float scl = 1.f, l_fin = l_tot;
+          if (p.num_sinks > 0) {
             const int srow = (p.sink_rows == p.Hq) ? out_head : (p.sink_rows == Hkv ? h : 0);
             const float* sk = p.sinks + (size_t)srow * p.num_sinks;
             float sm = -INFINITY;
             for (int i = 0; i < p.num_sinks; ++i) sm = fmaxf(sm, sk[i] * kLog2eP);
-            const float m_fin = fmaxf(m_run, sm);
+            const float m_fin = fmaxf(m_tot, sm);
             const float mf = (m_fin == -INFINITY) ? 0.f : m_fin;
-            scl = fast_exp2(m_run - mf);
-            l_fin = l_row * scl;
+            scl = fast_exp2(m_tot - mf);
+            l_fin = l_tot * scl;
             for (int i = 0; i < p.num_sinks; ++i) l_fin += fast_exp2(sk[i] * kLog2eP - mf);
           }
-          scl = (l_fin > 0.f) ? scl / l_fin * v_back : 0.f;
+          scl = (l_fin > 0.f) ? scl / l_fin : 0.f;
           T* orow = reinterpret_cast<T*>(p.out) + ((size_t)out_row_q * p.Hq + out_head) * D;
 #pragma unroll 1
           for (int c0 = 0; c0 < D; c0 += 32) {
-            uint32_t o[32];
-            tc_ld32(tm_o + c0, o);
-            tc_wait_ld();
-            if (row_ok) {
+            float acc[32];
 #pragma unroll
-              for (int c = 0; c < 32; c += 8) {
-                uint4 v;
-                v.x = Mma<T>::pack(__uint_as_float(o[c]) * scl, __uint_as_float(o[c + 1]) * scl);
-                v.y = Mma<T>::pack(__uint_as_float(o[c + 2]) * scl, __uint_as_float(o[c + 3]) * scl);
-                v.z = Mma<T>::pack(__uint_as_float(o[c + 4]) * scl, __uint_as_float(o[c + 5]) * scl);
-                v.w = Mma<T>::pack(__uint_as_float(o[c + 6]) * scl, __uint_as_float(o[c + 7]) * scl);
-                *reinterpret_cast<uint4*>(orow + c0 + c) = v;
+            for (int c = 0; c < 32; ++c) acc[c] = 0.f;
+            for (int pi = 0; pi < u.n_chunks; ++pi) {
+              const size_t at = ((size_t)slot_of(c_first + pi) * NT + x) * kBM + row;
+              const float f = fast_exp2(__ldcg(&p.ppart_ml[at]).x - mu);
+              const float4* src = reinterpret_cast<const float4*>(p.ppart_o + at * D + c0);
+#pragma unroll
+              for (int c = 0; c < 32; c += 4) {
+                const float4 v = __ldcg(src + (c >> 2));
+                acc[c] += v.x * f;
+                acc[c + 1] += v.y * f;
+                acc[c + 2] += v.z * f;
+                acc[c + 3] += v.w * f;
               }
             }
+#pragma unroll
+            for (int c = 0; c < 32; c += 8) {
+              uint4 v;
+              v.x = Mma<T>::pack(acc[c] * scl, acc[c + 1] * scl);
+              v.y = Mma<T>::pack(acc[c + 2] * scl, acc[c + 3] * scl);
+              v.z = Mma<T>::pack(acc[c + 4] * scl, acc[c + 5] * scl);
+              v.w = Mma<T>::pack(acc[c + 6] * scl, acc[c + 7] * scl);
+              *reinterpret_cast<uint4*>(orow + c0 + c) = v;
+            }
           }
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(bar_o_free(x));
+        }
+        continue;  // on to the next piece
+      }
+      const float l_row = l_run;
+      float scl = 1.f, l_fin = l_row;
+      if (p.num_sinks > 0 && row_ok) {
+        // attention sinks join the denominator only
+        const int srow = (p.sink_rows == p.Hq) ? out_head : (p.sink_rows == Hkv ? h : 0);
+        const float* sk = p.sinks + (size_t)srow * p.num_sinks;
+        float sm = -INFINITY;
+        for (int i = 0; i < p.num_sinks; ++i) sm = fmaxf(sm, sk[i] * kLog2eP);
+        const float m_fin = fmaxf(m_run, sm);
+        const float mf = (m_fin == -INFINITY) ? 0.f : m_fin;
+        scl = fast_exp2(m_run - mf);
+        l_fin = l_row * scl;
+        for (int i = 0; i < p.num_sinks; ++i) l_fin += fast_exp2(sk[i] * kLog2eP - mf);
+      }
+      scl = (l_fin > 0.f) ? scl / l_fin * v_back : 0.f;
+      T* orow = reinterpret_cast<T*>(p.out) + ((size_t)out_row_q * p.Hq + out_head) * D;
+#pragma unroll 1
+      for (int c0 = 0; c0 < D; c0 += 32) {
+        uint32_t o[32];
+        tc_ld32(tm_o + c0, o);
+        tc_wait_ld();
+        if (row_ok) {
+#pragma unroll
+          for (int c = 0; c < 32; c += 8) {
+            uint4 v;
+            v.x = Mma<T>::pack(__uint_as_float(o[c]) * scl, __uint_as_float(o[c + 1]) * scl);
+            v.y = Mma<T>::pack(__uint_as_float(o[c + 2]) * scl, __uint_as_float(o[c + 3]) * scl);
+            v.z = Mma<T>::pack(__uint_as_float(o[c + 4]) * scl, __uint_as_float(o[c + 5]) * scl);
+            v.w = Mma<T>::pack(__uint_as_float(o[c + 6]) * scl, __uint_as_float(o[c + 7]) * scl);
+            *reinterpret_cast<uint4*>(orow + c0 + c) = v;
+          }
         }
       }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar_o_free(x));
     }
   }
   if (*abort_flag) flags |= EJK_RPA_ST_TIMEOUT;

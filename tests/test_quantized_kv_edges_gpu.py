@@ -80,6 +80,41 @@ def test_split_kv_rows_do_not_feel_scales_that_their_mask_hides(code, dim, Hq, w
     check_rows(b, run(b, **kw), **kw)
 
 
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("block, kw", [(1, {}), (8, {}), (16, {}), (8, dict(logits_soft_cap=5.0)), (2, dict(softmax_scale=-0.1))])
+def test_prompt_rows_do_not_feel_scales_that_the_causal_mask_hides(code, dim, block, kw):
+    """A prefix of small values, then large ones in the same 64-token stage and in later ones."""
+    b = make_batch([(200, 200), (90, 333), (40, 40)], Hq=4, Hkv=2, dim=dim, page=16, block=block, code=code, half=torch.bfloat16, seed=dim + block)
+    ctx = b["ctx"].tolist()
+    set_v_scales(b, lambda s, j: 2.0**-40 if j < (48, ctx[1] - 48, 16)[s] else 1.0)
+    check_rows(b, run(b, **kw), **kw)
+
+
+@pytest.mark.parametrize("split", [0, 2])
+@pytest.mark.parametrize("dim, block", [(64, 4), (128, 16)])
+def test_prompt_rows_do_not_feel_scales_that_left_their_window(option, dim, block, split):
+    """Large values first: rows whose window has passed them see small ones alone, in the same stage and in later ones."""
+    option("prefill_split", split)
+    b = make_batch([(300, 700), (250, 250)], Hq=4, Hkv=2, dim=dim, page=16, block=block, code=torch.int8, half=torch.bfloat16, seed=dim)
+    first = [400, 0]
+    set_v_scales(b, lambda s, j: 1.0 if j < first[s] + 16 else 2.0**-40)
+    check_rows(b, run(b, sliding_window=50), sliding_window=50)
+
+
+@pytest.mark.parametrize("rows", [3, 100])
+@pytest.mark.parametrize("half", HALVES)
+@pytest.mark.parametrize("any_scale", [False, True])
+def test_scales_far_apart_row_by_row(rows, half, any_scale):
+    far = 30 if half == torch.bfloat16 else 6
+    b = make_batch([(rows, 260), (1, 150), (rows, rows)], Hq=4, Hkv=1, dim=64, page=16, block=8, code=torch.float8_e4m3fn, half=half, seed=rows, any_scale=any_scale)
+    b["scales"][:, :, 1] *= torch.exp2(torch.randint(-far, far - 2, b["scales"][:, :, 1].shape, generator=torch.Generator().manual_seed(2)).float())
+    sinks = torch.randn((4, 2), generator=torch.Generator().manual_seed(1))
+    check_rows(b, run(b))
+    check_rows(b, run(b, sliding_window=37), sliding_window=37)
+    check_rows(b, run(b, sinks=sinks), sinks=sinks)
+
+
 # ------------------------------------------------------------------------------------ rows that no sequence serves
 
 
