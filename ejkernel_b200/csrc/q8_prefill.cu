@@ -1230,7 +1230,9 @@ q8_prefill_kernel(const Params p, const Q8Cache cache) {
         l_fin = l_row * scl;
         for (int i = 0; i < p.num_sinks; ++i) l_fin += fast_exp2(sk[i] * kLog2eP - mf);
       }
-      scl = (l_fin > 0.f) ? scl / l_fin * v_back : 0.f;
+      scl = (l_fin > 0.f) ? scl / l_fin : 0.f;
+      // two factors: their product can lie below what float32 holds, where the scales are tiny and the keys many
+      auto finish = [&](uint32_t o) { return __uint_as_float(o) * scl * v_back; };
       T* orow = reinterpret_cast<T*>(p.out) + ((size_t)out_row_q * p.Hq + out_head) * D;
 #pragma unroll 1
       for (int c0 = 0; c0 < D; c0 += 32) {
@@ -1241,10 +1243,10 @@ q8_prefill_kernel(const Params p, const Q8Cache cache) {
 #pragma unroll
           for (int c = 0; c < 32; c += 8) {
             uint4 v;
-            v.x = Mma<T>::pack(__uint_as_float(o[c]) * scl, __uint_as_float(o[c + 1]) * scl);
-            v.y = Mma<T>::pack(__uint_as_float(o[c + 2]) * scl, __uint_as_float(o[c + 3]) * scl);
-            v.z = Mma<T>::pack(__uint_as_float(o[c + 4]) * scl, __uint_as_float(o[c + 5]) * scl);
-            v.w = Mma<T>::pack(__uint_as_float(o[c + 6]) * scl, __uint_as_float(o[c + 7]) * scl);
+            v.x = Mma<T>::pack(finish(o[c]), finish(o[c + 1]));
+            v.y = Mma<T>::pack(finish(o[c + 2]), finish(o[c + 3]));
+            v.z = Mma<T>::pack(finish(o[c + 4]), finish(o[c + 5]));
+            v.w = Mma<T>::pack(finish(o[c + 6]), finish(o[c + 7]));
             *reinterpret_cast<uint4*>(orow + c0 + c) = v;
           }
         }

@@ -115,6 +115,18 @@ def test_scales_far_apart_row_by_row(rows, half, any_scale):
     check_rows(b, run(b, sinks=sinks), sinks=sinks)
 
 
+@pytest.mark.parametrize("rows, split", [(1, 1), (100, 0), (100, 2)])
+def test_values_near_the_smallest_normal_number(option, rows, split):
+    """Scales of 2^-120 over many keys of equal weight: the sum is undone by the scales' power of two and by the weights' sum, one
+    after the other; their product alone would be below what float32 holds."""
+    option("prefill_split", split)
+    b = make_batch([(rows, 4000)], Hq=2, Hkv=1, dim=64, page=16, block=16, code=torch.int8, half=torch.bfloat16, seed=5)
+    b["codes"][:, :, 1] = torch.randint(60, 128, b["codes"][:, :, 1].shape, generator=torch.Generator().manual_seed(3)).to(torch.int8)
+    b["scales"][:, :, 1] = 2.0**-120
+    b["q"] = b["q"] * 0.01
+    check_rows(b, run(b))
+
+
 # ------------------------------------------------------------------------------------ rows that no sequence serves
 
 
