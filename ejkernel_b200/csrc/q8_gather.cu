@@ -53,7 +53,8 @@ __global__ void __launch_bounds__(kThreads) q8_gather_kernel(const Params p, con
     else hi = mid;
   }
   const int q0 = S > 0 ? p.query_start_loc[lo] : 0, q1 = S > 0 ? p.query_start_loc[lo + 1] : 0;
-  if (S <= 0 || t < q0 || t >= q1) {  // a row of no sequence
+  if (S > 0 && bad_rows(q0, q1, p.T)) flags |= EJK_RPA_ST_QLEN;
+  if (S <= 0 || t < q0 || t >= q1 || bad_rows(q0, q1, p.T)) {  // a row of no sequence, or of one whose offsets are refused
     for (int d = tid; d < D; d += kThreads) out[d] = Mma<T>::from_float(0.f);
     if (flags && tid == 0 && p.status) atomicOr(reinterpret_cast<unsigned*>(p.status), flags);
     return;
@@ -64,7 +65,7 @@ __global__ void __launch_bounds__(kThreads) q8_gather_kernel(const Params p, con
     flags |= EJK_RPA_ST_KVLEN;
     kv_len = kv_len < 0 ? 0 : kv_cap;
   }
-  if (q0 < 0 || q1 > p.T || q1 - q0 > kv_len) flags |= EJK_RPA_ST_QLEN;
+  if (q1 - q0 > kv_len) flags |= EJK_RPA_ST_QLEN;
   const int pos = kv_len - (q1 - q0) + (t - q0);
   const int key0 = (p.window > 0 && pos - p.window + 1 > 0) ? pos - p.window + 1 : 0;
   const int key1 = pos + 1 < kv_len ? pos + 1 : kv_len;

@@ -29,7 +29,7 @@ __device__ __forceinline__ SeqTiles load_seq(const Params& p, int s, unsigned& f
     kv = kv < 0 ? 0 : kv_cap;
   }
   int ql = q1 - q0;
-  if (ql < 0 || q0 < 0 || q1 > p.T) {
+  if (bad_rows(q0, q1, p.T)) {
     flags |= EJK_RPA_ST_QLEN;
     ql = 0;
   }
@@ -118,7 +118,17 @@ __global__ void __launch_bounds__(kThreads) q8_plan_kernel(const Params p, int n
   const int item_rows = half ? kPrefillRows : 2 * kPrefillRows;
   const int n_items = half ? s_items[1] : s_items[0];
   const bool fits = n_items <= p.max_punits;
-  if (!fits) flags |= EJK_RPA_ST_INTERNAL;
+  if (!fits) {
+    // only where sequences overlap: nothing is listed, and the rows that the list would have served are zero
+    flags |= EJK_RPA_ST_INTERNAL;
+    for (int s = 0; s < S; ++s) {
+      const SeqTiles q = load_seq(p, s, flags);
+      if (!q.tiles) continue;
+      uint4* dst = reinterpret_cast<uint4*>(p.out) + (size_t)q.q_start * p.Hq * (p.D / 8);
+      const size_t n16 = (size_t)q.q_len * p.Hq * (p.D / 8);
+      for (size_t i = tid; i < n16; i += kThreads) dst[i] = make_uint4(0u, 0u, 0u, 0u);
+    }
+  }
   const bool sorted = n_items <= kSortItems;
   int n_sort = 1;
   while (n_sort < n_items) n_sort <<= 1;

@@ -84,6 +84,7 @@ struct Cfg {
   static constexpr int OFF_BAR = OFF_META + NS * 8;  // full[NS], empty[NS], cbar
   static constexpr int OFF_SHARE = OFF_BAR + (2 * NS + 1) * 8;
   static constexpr int OFF_ABORT = OFF_SHARE + (int)sizeof(Share);
+  static constexpr int OFF_BAD = OFF_ABORT + 4;
   static constexpr int SMEM_BYTES = OFF_ABORT + 16 + 1024;  // + alignment slack
   static constexpr int CTAS = SMEM_BYTES <= 112 * 1024 ? 2 : 1;
   static_assert(SMEM_BYTES <= 227 * 1024, "shared memory budget");
@@ -132,7 +133,7 @@ __device__ __forceinline__ Seq load_seq(const Params& p, int s, int rows_per_til
     kv = kv < 0 ? 0 : kv_cap;
   }
   int ql = q1 - q0;
-  if (ql < 0 || q0 < 0 || q1 > p.T) {
+  if (bad_rows(q0, q1, p.T)) {
     flags |= EJK_RPA_ST_QLEN;
     ql = 0;
   }
@@ -195,6 +196,7 @@ q8_splitkv_kernel(const __grid_constant__ CUtensorMap tmap, const Params p, cons
   ItemDesc* ring = reinterpret_cast<ItemDesc*>(smem + C::OFF_RING);
   int2* metas = reinterpret_cast<int2*>(smem + C::OFF_META);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::OFF_ABORT);
+  volatile int* bad_offsets = reinterpret_cast<volatile int*>(smem + C::OFF_BAD);
   Share* share = reinterpret_cast<Share*>(smem + C::OFF_SHARE);
   const uint32_t bar_full = smem_base + C::OFF_BAR;
   const uint32_t bar_empty = bar_full + NS * 8;
@@ -215,6 +217,7 @@ q8_splitkv_kernel(const __grid_constant__ CUtensorMap tmap, const Params p, cons
     }
     mbar_init(bar_c, kConsumerWarps);
     *abort_flag = 0;
+    *bad_offsets = 0;
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
   }
@@ -239,6 +242,7 @@ q8_splitkv_kernel(const __grid_constant__ CUtensorMap tmap, const Params p, cons
     const int a = min(tid * per, S), b = min(a + per, S);
     long long mine = 0;
     for (int i = a; i < b; ++i) mine += seq_stages(p, load_seq(p, i, RT, flags), RT);
+    if (flags & EJK_RPA_ST_QLEN) *bad_offsets = 1;
     if (blockIdx.x != 0) flags = 0;  // one CTA reports
     long long incl = mine;
 #pragma unroll
@@ -1025,8 +1029,18 @@ q8_splitkv_kernel(const __grid_constant__ CUtensorMap tmap, const Params p, cons
   }
   if (flags && p.status) atomicOr(reinterpret_cast<unsigned*>(p.status), flags);
   {
-    const int tail = S > 0 ? __ldg(p.query_start_loc + S) : __ldg(p.query_start_loc);
-    zero_tail_rows(p.out, min(max(tail, 0), p.T), p.T, (size_t)p.Hq * D * sizeof(T));
+    // rows of no sequence: in front of the first, behind the last, and those of sequences whose offsets are refused.  Between
+    // the first offset and the last every row lies between two neighbouring offsets, whatever their order: none is left out
+    const size_t row_bytes = (size_t)p.Hq * D * sizeof(T);
+    const int head = __ldg(p.query_start_loc), tail = __ldg(p.query_start_loc + S);
+    zero_tail_rows(p.out, 0, min(max(head, 0), p.T), row_bytes);
+    zero_tail_rows(p.out, min(max(tail, 0), p.T), p.T, row_bytes);
+    if (*bad_offsets) {
+      for (int i = 0; i < S; ++i) {
+        const int q0 = __ldg(p.query_start_loc + i), q1 = __ldg(p.query_start_loc + i + 1);
+        if (bad_rows(q0, q1, p.T)) zero_tail_rows(p.out, max(q0, 0), min(q1, p.T), row_bytes);
+      }
+    }
   }
   // In a mixed batch this grid is a programmatic dependent of the prefill-tile grid and never waited for it
   // (the two write different rows).  Whatever follows in the stream, though, is only ordered after THIS grid:

@@ -106,6 +106,9 @@ __device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 x) { retu
 template <>
 __device__ __forceinline__ float to_float<__half>(__half x) { return __half2float(x); }
 
+// Offsets of a sequence that no kernel serves (they report it): its rows that there are, are zero.
+__device__ __forceinline__ bool bad_rows(int q0, int q1, int T) { return q1 < q0 || q0 < 0 || q1 > T; }
+
 // host side, shared by the entry points (defined in rpa_api.cu)
 struct LaunchOptions {
   int min_chunk, prefill_rows, prefill_share, prefill_split, overlap, wait_ms, path, test_withhold;

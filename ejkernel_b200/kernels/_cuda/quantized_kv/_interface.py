@@ -279,7 +279,7 @@ def quantized_ragged_page_attention(
                 queries, kv_pages, kv_scales, context_lens, block_tables, query_start_loc, num_seqs, softmax_scale=softmax_scale,
                 logits_soft_cap=logits_soft_cap, sliding_window=sliding_window, softmax_aux=softmax_aux,
                 num_kv_pages_per_block=num_kv_pages_per_block, num_queries_per_block=num_queries_per_block)
-    out = torch.empty_like(queries)  # every row is written: sequences by their tiles, the rest zero-filled
+    out = torch.empty_like(queries)  # every row is written: sequences by their tiles, rows of no sequence or of a refused one with zeros
     aux = None
     if softmax_aux is not None and attrs.num_sinks:
         aux = softmax_aux.to(torch.float32).contiguous()

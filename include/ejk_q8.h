@@ -52,7 +52,9 @@ EJK_RPA_API size_t ejk_q8_workspace_bytes(const ejk_q8_shape* shape);
 
 /* Ragged attention over the 8-bit cache.  Operands, masks, sinks and zero rows as ejk_rpa_launch; `attrs.q_scale` and
  * `attrs.out_scale` must be 0.  With x = softmax_scale * k_scale[j] * sum_d q[d] * k_code[j, d], soft cap and masks on
- * x, the output is sum_j softmax(x)[j] * v_scale[j] * v_code[j]. */
+ * x, the output is sum_j softmax(x)[j] * v_scale[j] * v_code[j].  Every row of `out` is written: rows of no sequence, and of
+ * sequences whose offsets are refused (EJK_RPA_ST_QLEN: they decrease, or lie outside [0, total_tokens]), are zero.  Where
+ * offsets decrease, sequences can claim the same rows: whose such a row is, or whether it is zero, is open. */
 EJK_RPA_API int ejk_q8_attention_launch(const void* queries, const void* kv_pages, const float* kv_scales,
                                         const int32_t* context_lens, const int32_t* block_tables,
                                         const int32_t* query_start_loc, const int32_t* num_seqs, const float* softmax_aux,

@@ -142,6 +142,34 @@ def poisoned(b, **kw):
     return out
 
 
+@pytest.mark.parametrize("page", [16, 5])
+@pytest.mark.parametrize("start, served", [([0, 1, 900], {0}), ([2, 3, 5], {2, 3, 4}), ([-3, 2, 4], {2, 3}), ([0, 3, 3000], {0, 1, 2}), ([7, 7, 7], set()), ([0, 0, -4], set())])
+def test_rows_under_bad_offsets_are_zero(page, start, served):
+    b = make_batch([(1, 40), (6, 30)], Hq=4, Hkv=2, dim=64, page=page, block=1, code=torch.int8, half=torch.bfloat16, seed=12)
+    out = poisoned(b | dict(start=torch.tensor(start, dtype=torch.int32)))
+    read_status()
+    for t in range(7):
+        assert bool(out[t].any()) == (t in served), t
+
+
+@pytest.mark.parametrize("page", [16, 5])
+def test_prompt_rows_under_bad_offsets_are_zero(page):
+    b = make_batch([(100, 140), (120, 130)], Hq=4, Hkv=2, dim=64, page=page, block=1, code=torch.int8, half=torch.bfloat16, seed=13)
+    out = poisoned(b | dict(start=torch.tensor([0, 100, 221], dtype=torch.int32)))
+    assert read_status() & _cabi.ST_QLEN
+    assert bool(out[:100].any(-1).all()) and not bool(out[100:].any())
+
+
+def test_rows_are_zero_where_overlapping_offsets_need_more_items_than_there_are():
+    """Each of five sequences claims all 1000 rows: more 128-row items than 1000 tokens can make."""
+    b = make_batch([(1000, 1000)], Hq=4, Hkv=1, dim=64, page=16, block=16, code=torch.int8, half=torch.bfloat16, seed=14)
+    b["tab"], b["ctx"] = b["tab"].repeat(9, 1), b["ctx"].repeat(9)
+    b["start"], b["n"] = torch.tensor([0, 1000] * 5, dtype=torch.int32), 9
+    out = poisoned(b)
+    assert read_status() & _cabi.ST_INTERNAL
+    assert not bool(out.any())
+
+
 # ------------------------------------------------------------------------------------------------------ dispatch
 
 
