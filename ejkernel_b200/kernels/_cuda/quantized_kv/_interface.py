@@ -399,7 +399,7 @@ def quantized_kv_read(
 ) -> tuple[Array, Array]:
     """The cache's rows at ``slot_mapping`` in 16 bits: ``(keys, values)``, each ``[rows, num_kv_heads, head_dim]``.
 
-    A value beyond the range of ``dtype`` saturates; a negative slot gives a row of zeros.
+    A value beyond the range of ``dtype`` saturates, a code that is a NaN gives a NaN; a negative slot gives a row of zeros.
     """
     try:
         key = (kv_pages.shape, kv_pages.dtype, kv_pages.is_contiguous(), kv_pages.get_device(),

@@ -77,7 +77,7 @@ EJK_RPA_API int ejk_q8_write_launch(const void* keys, const void* values, int64_
                                     const ejk_q8_shape* shape, void* stream);
 
 /* The rows at `slots` as 16-bit keys / values [total_tokens, num_kv_heads, head_dim]: code * scale, rounded, saturated at
- * the largest finite value.  A negative slot gives zeros. */
+ * the largest finite value; a code that is a NaN gives a NaN.  A negative slot gives zeros. */
 EJK_RPA_API int ejk_q8_read_launch(const void* kv_pages, const float* kv_scales, const int32_t* slots, void* keys,
                                    void* values, int32_t* status, const ejk_q8_shape* shape, void* stream);
 

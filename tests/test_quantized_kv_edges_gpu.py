@@ -170,6 +170,22 @@ def test_rows_are_zero_where_overlapping_offsets_need_more_items_than_there_are(
     assert not bool(out.any())
 
 
+# ------------------------------------------------------------------------------------------------ write and read
+
+
+@pytest.mark.parametrize("half", HALVES)
+def test_read_gives_a_nan_back_as_a_nan(half):
+    g = torch.Generator().manual_seed(6)
+    kv, scales = make_cache(g, 2, 1, 16, 64, torch.float8_e4m3fn, 16)
+    codes = kv.view(torch.uint8).clone()
+    codes[0, 0, 0, 3, 7], codes[1, 0, 1, 2, 0] = 0x7F, 0xFF
+    kv, scales = codes.view(torch.float8_e4m3fn).cuda(), scales.cuda()
+    slots = torch.arange(32, dtype=torch.int32, device="cuda")
+    for which, got in enumerate(ej.quantized_kv_read(kv, scales, slots, dtype=half)):
+        want = (kv.float() * scales.repeat_interleave(16, 3)[..., None])[:, 0, which].reshape(32, 1, 64)
+        assert torch.equal(torch.isnan(got), torch.isnan(want)) and int(torch.isnan(got).sum()) == 1
+
+
 # ------------------------------------------------------------------------------------------------------ dispatch
 
 
