@@ -112,9 +112,9 @@ __device__ __forceinline__ unsigned write_block(const T* __restrict__ src, long 
   }
   __syncwarp();  // every lane has read the old scale
   if (lane == 0) *scale_at = scale;
-  // a scale that this kernel wrote is a power of two, and the product with its inverse is the quotient; one that a
-  // caller put there need not be
-  const bool exact = (__float_as_uint(scale) & 0x7fffffu) == 0;
+  // a scale that this kernel wrote is a power of two up to 2^122, and the product with its inverse is the quotient; one that a
+  // caller put there need not be, or be 2^127, whose inverse is no normal number
+  const bool exact = (__float_as_uint(scale) & 0x7fffffu) == 0 && __float_as_uint(scale) < (254u << 23);
   const float inv = exact ? power_of_two_inverse(scale) : 0.f;
   auto put = [&](const uint4& v, int r) {
     const uint32_t x[4] = {v.x, v.y, v.z, v.w};

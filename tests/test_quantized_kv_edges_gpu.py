@@ -186,6 +186,44 @@ def test_read_gives_a_nan_back_as_a_nan(half):
         assert torch.equal(torch.isnan(got), torch.isnan(want)) and int(torch.isnan(got).sum()) == 1
 
 
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("exponent", [127, 126, 125])
+def test_write_behind_rows_of_the_largest_scales(code, exponent):
+    """Kept rows stand under a scale of 2^127, the largest power of two there is: its inverse is no normal number."""
+    g = torch.Generator().manual_seed(exponent)
+    kv, scales = make_cache(g, 2, 1, 16, 64, code, 16)
+    kv.view(torch.uint8).zero_()
+    scales[:] = 2.0**exponent
+    x = torch.randn((3, 1, 64), generator=g, dtype=torch.float64).mul(2.0**124).clamp(-3e38, 3e38).to(torch.bfloat16)
+    x[0, 0, 0], x[0, 0, 1] = 3e38, -3e38
+    slots = torch.tensor([17, 18, 19], dtype=torch.int32)
+    want_c, want_s = q8_oracle.write(x, x, kv, scales, slots)
+    kv, scales = kv.cuda(), scales.cuda()
+    ej.quantized_kv_write(x.cuda(), x.cuda(), kv, scales, slots.cuda())
+    assert np.array_equal(scales.cpu().double().numpy(), want_s)
+    assert np.array_equal(kv.cpu().float().double().numpy(), want_c) and want_c.any()
+
+
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("dim, page, block", [(64, 16, 16), (128, 16, 4), (256, 24, 8), (64, 5, 1)])
+def test_write_to_pages_in_any_order(code, dim, page, block):
+    """Rows that go on in a lower or a distant page."""
+    g = torch.Generator().manual_seed(dim + page)
+    kv, scales = make_cache(g, 40, 2, page, dim, code, block)
+    order, at, slots = torch.randperm(40, generator=g), 0, []
+    for c, n in ((3, 2 * page), (page - 1, 3 * page + 2), (0, 1), (page // 2, 4 * page)):
+        held = -(-(c + n) // page)
+        pos = torch.arange(c, c + n)
+        slots.append(order[at: at + held][pos // page] * page + pos % page)
+        at += held
+    slots = torch.cat(slots).to(torch.int32)
+    x = (torch.randn((slots.numel(), 2, dim), generator=g) * torch.exp2(torch.randint(-9, 4, (slots.numel(), 2, 1), generator=g).float())).to(torch.float16)
+    want_c, want_s = q8_oracle.write(x, -x, kv, scales, slots)
+    kv, scales = kv.cuda(), scales.cuda()
+    ej.quantized_kv_write(x.cuda(), (-x).cuda(), kv, scales, slots.cuda())
+    assert np.array_equal(scales.cpu().double().numpy(), want_s) and np.array_equal(kv.cpu().float().double().numpy(), want_c)
+
+
 # ------------------------------------------------------------------------------------------------------ dispatch
 
 
