@@ -244,8 +244,9 @@ cudaError_t launch_page_tables(const int32_t* query_lens, const int32_t* context
   const TableArgs a = {query_lens, context_lens, tables, free_pages, num_free, num_seqs, finished, new_lens, starts,
                        slots, new_free, status, S, pps, page, capacity, T};
   const size_t smem = (size_t)S * 3 * sizeof(unsigned);
-  if (smem > 48 * 1024) {
-    // the limit of the kernel on the current device, set whenever it is needed: two words of host work
+  if (smem > 32 * 1024) {
+    // The limit of the kernel on the current device, set whenever it may be needed: two words of host work.  Without it a block
+    // gets 48 KB, of which the kernel's own few hundred bytes take a part
     if (cudaError_t e = cudaFuncSetAttribute(page_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPageTableMaxRows * 12); e != cudaSuccess)
       return e;
   }

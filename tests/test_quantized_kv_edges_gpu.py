@@ -224,6 +224,20 @@ def test_write_to_pages_in_any_order(code, dim, page, block):
     assert np.array_equal(scales.cpu().double().numpy(), want_s) and np.array_equal(kv.cpu().float().double().numpy(), want_c)
 
 
+# -------------------------------------------------------------------------------------------------- page tables
+
+
+@pytest.mark.parametrize("rows", [2731, 4050, 4063, 4064, 4096, 4097, 16384])
+def test_tables_of_rows_around_the_plain_shared_memory_limit(rows):
+    """In a process of its own: once a larger table has raised the kernel's limit, the sizes below are served too."""
+    code = f"""
+        from tests.test_quantized_kv_gpu import check_tables, make_requests
+        check_tables(make_requests([1, 0, 20, 3], [0, 17, 5, 16], page=16, pps=8, seed=1, rows={rows}), 16, 30)
+    """
+    r = subprocess.run([sys.executable, "-c", textwrap.dedent(code)], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+
+
 # ------------------------------------------------------------------------------------------------------ dispatch
 
 
