@@ -225,9 +225,9 @@ def _plan_attention(
     nbytes = 0
     if T:
         with torch.cuda.device(queries.device):
-            nbytes = int(_cabi.load().ejk_q8_workspace_bytes(ctypes.byref(shape)))
+            nbytes = int(_cabi.load().ejk_q8_attention_workspace_bytes(ctypes.byref(shape), ctypes.byref(attrs)))
         if nbytes == 0:
-            raise ValueError("ejk_q8_workspace_bytes rejected the shape")
+            raise ValueError("ejk_q8_attention_workspace_bytes rejected the shape")
     return shape, attrs, nbytes, ctypes.byref(shape), ctypes.byref(attrs), queries.device
 
 
@@ -252,6 +252,10 @@ def quantized_ragged_page_attention(
 
     Products run on the codes as 16-bit floats (exact) and accumulate in float32; ``softmax_scale`` defaults to
     ``head_dim ** -0.5``.  Returns a tensor of the shape and dtype of ``queries``.
+
+    ``num_queries_per_block``: from how many query tokens on a sequence is served by tensor tiles (head_dim 64 and 128).  Without
+    it that is decided for batches with more tokens than ``block_tables`` has rows; a table padded with idle rows hides from the
+    host whether there is a prompt in the batch, so give it where chunks of prompts come in such tables.
     """
     try:
         key = (queries.shape, queries.dtype, queries.is_contiguous(), queries.get_device(),

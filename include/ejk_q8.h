@@ -46,13 +46,19 @@ typedef struct ejk_q8_shape {
  * call leaves them zero, one whose waits ran out (EJK_RPA_ST_TIMEOUT) included; the rest needs no initialisation. */
 #define EJK_Q8_TICKET_BYTES 16384
 
-/* Scratch that ejk_q8_attention_launch needs for this static shape on the current device (0: invalid shape).  One workspace
- * serves any number of calls that are ordered on the device, of any shapes that fit. */
+/* Scratch that ejk_q8_attention_launch needs for this static shape on the current device (0: invalid shape), in calls with
+ * these attributes (of which num_queries_per_block counts; null: without it).  One workspace serves any number of calls that are
+ * ordered on the device, of any shapes that fit. */
+EJK_RPA_API size_t ejk_q8_attention_workspace_bytes(const ejk_q8_shape* shape, const ejk_rpa_attrs* attrs);
+/* The same without attributes. */
 EJK_RPA_API size_t ejk_q8_workspace_bytes(const ejk_q8_shape* shape);
 
 /* Ragged attention over the 8-bit cache.  Operands, masks, sinks and zero rows as ejk_rpa_launch; `attrs.q_scale` and
  * `attrs.out_scale` must be 0.  With x = softmax_scale * k_scale[j] * sum_d q[d] * k_code[j, d], soft cap and masks on
- * x, the output is sum_j softmax(x)[j] * v_scale[j] * v_code[j].  Every row of `out` is written: rows of no sequence, and of
+ * x, the output is sum_j softmax(x)[j] * v_scale[j] * v_code[j].
+ * Sequences with many query rows are served by tensor tiles (head_dim 64 and 128): those of num_queries_per_block tokens and more
+ * where the caller gives it, otherwise those of 32 rows and more in batches with more tokens than block_tables has rows.  In a
+ * table with idle rows only the hint tells a chunk of a prompt from decode rows.  Every row of `out` is written: rows of no sequence, and of
  * sequences whose offsets are refused (EJK_RPA_ST_QLEN: they decrease, or lie outside [0, total_tokens]), are zero.  Where
  * offsets decrease, sequences can claim the same rows: whose such a row is, or whether it is zero, is open. */
 EJK_RPA_API int ejk_q8_attention_launch(const void* queries, const void* kv_pages, const float* kv_scales,

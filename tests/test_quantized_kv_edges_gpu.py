@@ -245,6 +245,20 @@ def launches():
     return _cabi.load().ejk_rpa_last_launch_count()
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+def test_the_query_hint_counts_in_a_padded_table_too(dim):
+    """One chunk in a table of more rows than the batch has tokens: with the hint it is served by tensor tiles (three launches)."""
+    b = make_batch([(200, 333), (1, 50), (3, 60)], Hq=4, Hkv=2, dim=dim, page=16, block=16, code=torch.int8, half=torch.bfloat16, seed=21, rows=256)
+    check_rows(b, run(b))
+    assert launches() == 1
+    out = run(b, cfg=ej.RaggedPageAttentionConfig(num_kv_pages_per_block=None, num_queries_per_block=64))
+    assert launches() == 3
+    check_rows(b, out)
+    # a hint that no sequence of the batch can reach spares the plan
+    check_rows(b, run(b, cfg=ej.RaggedPageAttentionConfig(num_kv_pages_per_block=None, num_queries_per_block=205)))
+    assert launches() == 1
+
+
 @pytest.mark.parametrize("dim, Hq", [(64, 9), (64, 16), (256, 9), (256, 16)])
 @pytest.mark.parametrize("code, half", [(torch.int8, torch.bfloat16), (torch.int8, torch.float16), (torch.float8_e4m3fn, torch.bfloat16), (torch.float8_e4m3fn, torch.float16)])
 def test_more_than_eight_heads_per_kv_head(code, half, dim, Hq):
