@@ -53,6 +53,7 @@ Q8_TICKET_BYTES = 16384
 Q8_EXPORTS = (
     "ejk_q8_workspace_bytes",
     "ejk_q8_attention_workspace_bytes",
+    "ejk_q8_status_word",
     "ejk_q8_attention_launch",
     "ejk_q8_write_launch",
     "ejk_q8_read_launch",
@@ -195,6 +196,8 @@ def load() -> ctypes.CDLL:
     lib.ejk_rpa_stream_probe.argtypes = [c_void_p, c_size_t, c_void_p, c_void_p]
     lib.ejk_q8_workspace_bytes.restype = c_size_t
     lib.ejk_q8_workspace_bytes.argtypes = [POINTER(Q8Shape)]
+    lib.ejk_q8_status_word.restype = c_int
+    lib.ejk_q8_status_word.argtypes = [POINTER(c_void_p)]
     lib.ejk_q8_attention_workspace_bytes.restype = c_size_t
     lib.ejk_q8_attention_workspace_bytes.argtypes = [POINTER(Q8Shape), POINTER(Attrs)]
     lib.ejk_q8_attention_launch.restype = c_int

@@ -7,6 +7,8 @@
 namespace ejk {
 namespace {
 
+__device__ int32_t g_status;  // zero when the library is loaded, one on each device
+
 int log2_exact(int x) {
   if (x <= 0 || (x & (x - 1))) return -1;
   int s = 0;
@@ -107,6 +109,21 @@ size_t ejk_q8_attention_workspace_bytes(const ejk_q8_shape* shape, const ejk_rpa
   if (!n_sm) return 0;
   if (kQ8TicketsPerCta * 2 * n_sm * sizeof(int32_t) > EJK_Q8_TICKET_BYTES) return 0;
   return q8_workspace(*shape, n_sm, tiles_possible(*shape, attrs ? attrs->num_queries_per_block : 0)).total;
+}
+
+int ejk_q8_status_word(int32_t** word) {
+  if (!word) return EJK_RPA_E_NULL;
+  *word = nullptr;
+  if (!sm100_sm_count()) return EJK_RPA_E_DEVICE;
+  // loading the library's image, should this be its first use, is refused to a thread that is capturing in the strict mode
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  if (cudaError_t e = cudaThreadExchangeStreamCaptureMode(&mode); e != cudaSuccess) return static_cast<int>(e);
+  void* at = nullptr;
+  const cudaError_t e = cudaGetSymbolAddress(&at, g_status);
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  *word = static_cast<int32_t*>(at);
+  return 0;
 }
 
 int ejk_q8_attention_launch(const void* queries, const void* kv_pages, const float* kv_scales,

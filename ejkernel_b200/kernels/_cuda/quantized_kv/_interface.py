@@ -37,7 +37,7 @@ CODE_DTYPES = {FP8: _cabi.E4M3, torch.int8: _cabi.I8}
 
 _MAX_REMEMBERED = 4096
 _plans: dict[tuple, object] = {}
-_status: dict[int, torch.Tensor] = {}  # one word per device: bits are only OR-ed in, so streams can share it
+_status: dict[int, int] = {}  # address of the device's word, in the library's image: bits are only OR-ed in, so streams can share it
 _scratch: dict[tuple[int, int], torch.Tensor] = {}  # (device, stream) -> workspace; a stream's calls are ordered
 _MAX_STREAMS = 16
 
@@ -107,26 +107,34 @@ def _check_cache(kv_pages, kv_scales) -> int:
     return page_size // blocks
 
 
-def _status_word(device: torch.device):
-    """Address of the device's status word, or None."""
-    word = _status.get(device.index)
-    if word is None:
-        if _capturing():
-            return None  # a word made here would be the graph's, and zeroed by every replay
-        word = torch.zeros(1, dtype=torch.int32, device=device)
-        torch.cuda.current_stream(device).synchronize()  # once: other streams may use it from now on
-        _status[device.index] = word
-    return word.data_ptr()
+def _status_word(device: torch.device) -> int:
+    """Address of the status word of a device, which is the current one.  Memory of the allocator would not do: a word that is
+    made while a stream is captured would be the graph's, and zeroed by every replay."""
+    at = _status.get(device.index)
+    if at is None:
+        word = ctypes.c_void_p()
+        _cabi.check(_function("ejk_q8_status_word")(ctypes.byref(word)), "ejk_q8_status_word")
+        at = _status[device.index] = word.value
+    return at
+
+
+class _Word:
+    def __init__(self, at: int):
+        self.__cuda_array_interface__ = dict(shape=(1,), typestr="<i4", data=(at, False), version=3)
+
+
+def _status_tensor(index: int) -> torch.Tensor:
+    return torch.as_tensor(_Word(_status[index]), device=torch.device("cuda", index))
 
 
 def read_status(device: torch.device | str | int | None = None, clear: bool = True) -> int:
     """The status word of these operators on a device (forces a synchronisation): bits of ``_cabi.STATUS_TEXT``."""
     device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device("cuda", device) if isinstance(device, int) else torch.device(device)
     index = torch.cuda.current_device() if device.index is None else device.index
-    word = _status.get(index)
-    if word is None:
+    if index not in _status:
         return 0
     torch.cuda.synchronize(index)
+    word = _status_tensor(index)
     value = int(word.item())
     if clear:
         word.zero_()
@@ -138,9 +146,10 @@ def _after(device: torch.device, what: str) -> None:
     """Opt-in (``EJKERNEL_B200_CHECK_STATUS=1``): read the status word after the call and raise when an output is invalid."""
     if os.environ.get("EJKERNEL_B200_CHECK_STATUS", "0") in ("", "0") or device.index not in _status or _capturing():
         return
-    word = int(_status[device.index].item())
+    tensor = _status_tensor(device.index)
+    word = int(tensor.item())
     if word & (_cabi.ST_TIMEOUT | _cabi.ST_INTERNAL):
-        _status[device.index].zero_()
+        tensor.zero_()
         raise _cabi.RpaLibraryError(f"{what}: status word {word:#x}: " + "; ".join(_cabi.decode_status(word)))
 
 

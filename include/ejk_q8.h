@@ -42,6 +42,10 @@ typedef struct ejk_q8_shape {
   int32_t scale_block;   /* tokens that share a scale: a power of two that divides page_size */
 } ejk_q8_shape;
 
+/* A status word for `status` of the calls below that lives as long as the library, one on each device (that of the current
+ * device is given): zero at first, the caller clears it.  It can be had while a stream is being captured. */
+EJK_RPA_API int ejk_q8_status_word(int32_t** word);
+
 /* The first bytes of an attention workspace: counters that have to be zero when a workspace is used for the first time.  Every
  * call leaves them zero, one whose waits ran out (EJK_RPA_ST_TIMEOUT) included; the rest needs no initialisation. */
 #define EJK_Q8_TICKET_BYTES 16384

@@ -264,3 +264,37 @@ def test_the_query_hint_counts_in_a_padded_table_too(dim):
 def test_more_than_eight_heads_per_kv_head(code, half, dim, Hq):
     b = make_batch([(1, 300), (2, 77), (1, 9), (1, 2500)], Hq=2 * Hq, Hkv=2, dim=dim, page=16, block=8, code=code, half=half, seed=Hq)
     check_rows(b, run(b))
+
+
+# ------------------------------------------------------------------------------------------------------- capture
+
+
+def test_the_first_call_of_a_process_is_captured():
+    """The status word outlives the graph, and reports what its replays meet."""
+    code = """
+        import torch
+        import ejkernel_b200 as ej
+        from ejkernel_b200 import _cabi
+        from ejkernel_b200.kernels._cuda.quantized_kv import read_status
+
+        kv, scales = ej.allocate_quantized_kv(4, 1, 16, 64, dtype=torch.int8)
+        x = torch.ones((3, 1, 64), dtype=torch.bfloat16, device="cuda")
+        slots = torch.tensor([5, 6, 7], dtype=torch.int32, device="cuda")
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            ej.quantized_kv_write(x, x, kv, scales, slots)
+        graph.replay()
+        assert read_status() == 0
+        assert bool(kv[0, 0, :, 5:8].any(-1).all())
+        slots.fill_(1 << 20)
+        graph.replay()
+        assert read_status() == _cabi.ST_PAGE_ID
+        slots.copy_(torch.tensor([5, 6, 7]))
+        x[1, 0, 3] = float("nan")
+        for _ in range(2):
+            graph.replay()
+        assert read_status(clear=False) == _cabi.ST_NONFINITE and read_status() == _cabi.ST_NONFINITE and read_status() == 0
+    """
+    r = subprocess.run([sys.executable, "-c", textwrap.dedent(code)], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
