@@ -173,6 +173,10 @@ def _count(num_seqs, device: torch.device) -> torch.Tensor:
     """The number of sequences as an int32 on the device."""
     if isinstance(num_seqs, torch.Tensor) and num_seqs.dtype is torch.int32 and num_seqs.device == device and num_seqs.numel() == 1:
         return num_seqs
+    if _capturing() and not (isinstance(num_seqs, torch.Tensor) and num_seqs.is_cuda):
+        # a step of the graph: copying from the host cannot be captured, and a constant that is kept for eager calls can be
+        # dropped while the graph lives
+        return torch.full((1,), int(num_seqs), dtype=torch.int32, device=device)
     return _num_seqs_tensor(num_seqs, device)
 
 

@@ -298,3 +298,25 @@ def test_the_first_call_of_a_process_is_captured():
     """
     r = subprocess.run([sys.executable, "-c", textwrap.dedent(code)], cwd=ROOT, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stderr[-2000:]
+
+
+@pytest.mark.parametrize("kind", ["int", "host"])
+def test_a_number_of_sequences_that_the_host_holds_is_captured(kind):
+    """A count that no call has used before is part of the graph, and stays what it was when the process forgets old counts."""
+    from ejkernel_b200.kernels._cuda.ragged_page_attention import _interface
+
+    b = make_batch([(1, 100), (2, 40), (1, 70)], Hq=4, Hkv=1, dim=64, page=16, block=16, code=torch.int8, half=torch.bfloat16, seed=23, rows=5)
+    gpu = {k: v.cuda() if isinstance(v, torch.Tensor) else v for k, v in b.items()}
+    want = run(gpu)
+    _interface._num_seqs_consts.clear()
+    if kind == "host":
+        gpu["n"] = torch.tensor([3])
+    args = (gpu["q"], gpu["codes"], gpu["scales"], gpu["ctx"], gpu["tab"], gpu["start"], gpu["n"])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ej.quantized_ragged_page_attention(*args)
+    _interface._num_seqs_consts.clear()
+    keep = [torch.zeros(1, dtype=torch.int32, device="cuda") for _ in range(64)]
+    graph.replay()
+    assert torch.equal(out, want) and keep
