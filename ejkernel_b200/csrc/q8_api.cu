@@ -92,6 +92,8 @@ bool tiles_possible(const ejk_q8_shape& s, int num_queries_per_block) {
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+template <typename... P>
+bool aligned4(P... p) { return ((reinterpret_cast<uintptr_t>(p) | ...) & 3) == 0; }
 bool finite(float x) { return x == x && !std::isinf(x); }
 
 }  // namespace
@@ -142,7 +144,8 @@ int ejk_q8_attention_launch(const void* queries, const void* kv_pages, const flo
   if (a.q_scale != 0.f || a.out_scale != 0.f) return EJK_RPA_E_ARG;
   if (a.num_sinks < 0 || (a.num_sinks > 0 && !softmax_aux)) return EJK_RPA_E_ARG;
   if (a.num_sinks > 0 && a.sink_rows != s.num_q_heads && a.sink_rows != s.num_kv_heads && a.sink_rows != 1) return EJK_RPA_E_ARG;
-  if (!aligned16(queries) || !aligned16(kv_pages) || (reinterpret_cast<uintptr_t>(kv_scales) & 3) || !aligned16(out)) return EJK_RPA_E_ALIGN;
+  if (!aligned16(queries) || !aligned16(kv_pages) || !aligned16(out)) return EJK_RPA_E_ALIGN;
+  if (!aligned4(kv_scales, context_lens, block_tables, query_start_loc, num_seqs, softmax_aux, status)) return EJK_RPA_E_ALIGN;
   const int n_sm = sm100_sm_count();
   if (!n_sm) return EJK_RPA_E_DEVICE;
   if (kQ8TicketsPerCta * 2 * n_sm * sizeof(int32_t) > EJK_Q8_TICKET_BYTES) return EJK_RPA_E_DEVICE;
@@ -264,6 +267,7 @@ int ejk_q8_write_launch(const void* keys, const void* values, int64_t key_stride
   const int64_t row = (int64_t)s.num_kv_heads * s.head_dim;
   if (key_stride < row || value_stride < row) return EJK_RPA_E_SHAPE;
   if (!aligned16(keys) || !aligned16(values) || !aligned16(kv_pages) || key_stride % 8 || value_stride % 8) return EJK_RPA_E_ALIGN;
+  if (!aligned4(kv_scales, slots, status)) return EJK_RPA_E_ALIGN;
   if (!sm100_sm_count()) return EJK_RPA_E_DEVICE;
   cudaError_t e = launch_q8_write(keys, values, key_stride, value_stride, cache_of(kv_pages, kv_scales, s), slots, status,
                                   s.total_tokens, s.dtype, s.code_dtype, static_cast<cudaStream_t>(stream));
@@ -280,7 +284,7 @@ int ejk_q8_read_launch(const void* kv_pages, const float* kv_scales, const int32
   const ejk_q8_shape& s = *shape;
   // the kernel counts 8-element chunks of K in 32 bits
   if (s.total_tokens <= 0 || (long long)s.total_tokens * s.num_kv_heads * (s.head_dim / 8) > 0x7fffffffLL) return EJK_RPA_E_SHAPE;
-  if (!aligned16(keys) || !aligned16(values) || !aligned16(kv_pages)) return EJK_RPA_E_ALIGN;
+  if (!aligned16(keys) || !aligned16(values) || !aligned16(kv_pages) || !aligned4(kv_scales, slots, status)) return EJK_RPA_E_ALIGN;
   if (!sm100_sm_count()) return EJK_RPA_E_DEVICE;
   cudaError_t e = launch_q8_read(cache_of(kv_pages, kv_scales, s), slots, keys, values, status, s.total_tokens, s.dtype,
                                  s.code_dtype, static_cast<cudaStream_t>(stream));
@@ -301,6 +305,8 @@ int ejk_page_tables_launch(const int32_t* query_lens, const int32_t* context_len
   if (max_num_seqs <= 0 || max_num_seqs > kPageTableMaxRows || pages_per_seq <= 0 || page_size <= 0 || capacity <= 0 || total_tokens < 0)
     return EJK_RPA_E_SHAPE;
   if ((long long)pages_per_seq * page_size > 0x3fffffffLL || total_tokens > 0x3fffffff) return EJK_RPA_E_SHAPE;
+  if (!aligned4(query_lens, context_lens, block_tables, free_pages, num_free, num_seqs, new_context_lens, query_start_loc, slots, new_num_free, status))
+    return EJK_RPA_E_ALIGN;
   if (!sm100_sm_count()) return EJK_RPA_E_DEVICE;
   cudaError_t e = launch_page_tables(query_lens, context_lens, block_tables, free_pages, num_free, num_seqs, finished,
                                      new_context_lens, query_start_loc, slots, new_num_free, status, max_num_seqs,

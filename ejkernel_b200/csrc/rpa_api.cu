@@ -174,7 +174,7 @@ const char* ejk_rpa_error_string(int code) {
     case EJK_RPA_E_WORKSPACE: return "workspace too small or not 256-byte aligned";
     case EJK_RPA_E_ARG: return "invalid attribute (sliding_window, logits_soft_cap, softmax_aux or option name)";
     case EJK_RPA_E_DEVICE: return "current CUDA device is not an sm_100-class GPU";
-    case EJK_RPA_E_ALIGN: return "queries, kv_pages and out must be 16-byte aligned";
+    case EJK_RPA_E_ALIGN: return "queries, kv_pages and out must be 16-byte aligned, other operands as their type";
     case EJK_RPA_E_SCRATCH:
       return "this shape needs more scratch than the library's built-in static buffer holds "
              "(EJK_RPA_STATIC_SCRATCH_BYTES); use ejk_rpa_launch with a caller-provided workspace";
