@@ -140,7 +140,11 @@ int ejk_q8_attention_launch(const void* queries, const void* kv_pages, const flo
   if (int e = check_attention(*shape)) return e;
   const ejk_q8_shape& s = *shape;
   const ejk_rpa_attrs& a = *attrs;
-  if (!finite(a.softmax_scale) || !finite(a.logits_soft_cap)) return EJK_RPA_E_ARG;
+  // with what the kernels multiply by: the scale and the cap in units of log2, and the scale in units of the cap
+  const float log2e = 1.4426950408889634f;
+  const float in_caps = a.logits_soft_cap != 0.f ? a.softmax_scale / a.logits_soft_cap : 0.f;
+  if (!finite(a.softmax_scale * log2e) || !finite(a.logits_soft_cap) || !finite(in_caps * (2.f * log2e))) return EJK_RPA_E_ARG;
+  if (std::fabs(a.logits_soft_cap) > 0x1p100f) return EJK_RPA_E_ARG;
   if (a.q_scale != 0.f || a.out_scale != 0.f) return EJK_RPA_E_ARG;
   if (a.num_sinks < 0 || (a.num_sinks > 0 && !softmax_aux)) return EJK_RPA_E_ARG;
   if (a.num_sinks > 0 && a.sink_rows != s.num_q_heads && a.sink_rows != s.num_kv_heads && a.sink_rows != 1) return EJK_RPA_E_ARG;
@@ -180,13 +184,12 @@ int ejk_q8_attention_launch(const void* queries, const void* kv_pages, const flo
   p.window = a.sliding_window > 0 ? a.sliding_window : 0;
   p.num_sinks = a.num_sinks;
   p.sink_rows = a.sink_rows;
-  const float log2e = 1.4426950408889634f;
   p.out_scale = 1.f;
   p.scale = a.softmax_scale;
   p.scale_log2 = a.softmax_scale * log2e;
   p.cap = a.logits_soft_cap;
   p.cap_log2 = a.logits_soft_cap * log2e;
-  p.inv_cap_scale = a.logits_soft_cap != 0.f ? a.softmax_scale / a.logits_soft_cap : 0.f;
+  p.inv_cap_scale = in_caps;
   const Q8Cache c = cache_of(kv_pages, kv_scales, s);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (!use_tma) {

@@ -36,6 +36,8 @@ from ..ragged_page_attention._interface import _DTYPE_CODE, FP8, _num_seqs_tenso
 CODE_DTYPES = {FP8: _cabi.E4M3, torch.int8: _cabi.I8}
 
 _MAX_REMEMBERED = 4096
+_MAX_FACTOR, _MAX_CAP = 2.0**126, 2.0**100
+_MAX_INT = 0x7FFFFFFF
 _plans: dict[tuple, object] = {}
 _status: dict[int, int] = {}  # address of the device's word, in the library's image: bits are only OR-ed in, so streams can share it
 _scratch: dict[tuple[int, int], torch.Tensor] = {}  # (device, stream) -> workspace; a stream's calls are ordered
@@ -219,6 +221,11 @@ def _plan_attention(
     scale = D**-0.5 if softmax_scale is None else float(softmax_scale)
     if not math.isfinite(scale):
         raise ValueError(f"{softmax_scale=} must be finite")
+    # the kernels hold these numbers in float32, times 2 log2(e) at most
+    if abs(scale) > _MAX_FACTOR:
+        raise ValueError(f"{softmax_scale=} is beyond the range of float32")
+    if logits_soft_cap is not None and not (1 / _MAX_CAP <= abs(logits_soft_cap) <= _MAX_CAP and abs(scale) / abs(logits_soft_cap) <= _MAX_CAP):
+        raise ValueError(f"{logits_soft_cap=} or its quotient with the softmax scale is beyond the range of float32")
     if num_kv_pages_per_block is not None and not 0 < num_kv_pages_per_block <= pps:
         raise ValueError(f"{num_kv_pages_per_block=} must be in range (0, {pps}].")
     if num_queries_per_block is not None and num_queries_per_block <= 0:
@@ -233,8 +240,9 @@ def _plan_attention(
                    block_tables=block_tables, query_start_loc=query_start_loc, softmax_aux=softmax_aux)
     _need_cuda("quantized_ragged_page_attention", queries)
     shape = _cabi.Q8Shape(T, S, pps, P, page_size, Hq, Hkv, D, _DTYPE_CODE[queries.dtype], CODE_DTYPES[kv_pages.dtype], block)
-    attrs = _cabi.Attrs(scale, float(logits_soft_cap or 0.0), int(sliding_window or 0), sinks, rows,
-                        int(num_kv_pages_per_block or 0), int(num_queries_per_block or 0), 0.0, 0.0)
+    # a window, or a threshold, beyond 32 bits is beyond every length
+    attrs = _cabi.Attrs(scale, float(logits_soft_cap or 0.0), min(int(sliding_window or 0), _MAX_INT), sinks, rows,
+                        int(num_kv_pages_per_block or 0), min(int(num_queries_per_block or 0), _MAX_INT), 0.0, 0.0)
     nbytes = 0
     if T:
         with torch.cuda.device(queries.device):

@@ -55,6 +55,10 @@ def check_rows(b, out, **kw):
     assert worst <= 1.0, worst
 
 
+def launches():
+    return _cabi.load().ejk_rpa_last_launch_count()
+
+
 def set_v_scales(b, of):
     """V scale of the block that token j of every sequence lies in: of(sequence, first token of the block)."""
     page, per = b["codes"].shape[3], b["scales"].shape[3]
@@ -125,6 +129,27 @@ def test_values_near_the_smallest_normal_number(option, rows, split):
     b["scales"][:, :, 1] = 2.0**-120
     b["q"] = b["q"] * 0.01
     check_rows(b, run(b))
+
+
+# ---------------------------------------------------------------------------------- numbers at the end of their types
+
+
+@pytest.mark.parametrize("rows", [1, 90])
+def test_windows_beyond_32_bits_hide_nothing(rows):
+    b = make_batch([(rows, 200), (1, 33)], Hq=4, Hkv=2, dim=64, page=16, block=16, code=torch.int8, half=torch.bfloat16, seed=24)
+    want = run(b)
+    for window in (2**31 - 1, 2**31, 2**32 + 5):
+        assert torch.equal(run(b, sliding_window=window), want)
+    hint = ej.RaggedPageAttentionConfig(num_kv_pages_per_block=None, num_queries_per_block=2**32 + 1)
+    check_rows(b, run(b, cfg=hint))
+    assert launches() == 1
+
+
+@pytest.mark.parametrize("rows", [1, 90])
+@pytest.mark.parametrize("kw", [dict(logits_soft_cap=2.0**-90, softmax_scale=1.0), dict(softmax_scale=2.0**-140)])
+def test_caps_and_scales_at_the_ends_of_float32(rows, kw):
+    b = make_batch([(rows, 200), (1, 33)], Hq=4, Hkv=2, dim=64, page=16, block=16, code=torch.int8, half=torch.bfloat16, seed=25)
+    check_rows(b, run(b, **kw), **kw)
 
 
 # ------------------------------------------------------------------------------------ rows that no sequence serves
@@ -239,10 +264,6 @@ def test_tables_of_rows_around_the_plain_shared_memory_limit(rows):
 
 
 # ------------------------------------------------------------------------------------------------------ dispatch
-
-
-def launches():
-    return _cabi.load().ejk_rpa_last_launch_count()
 
 
 @pytest.mark.parametrize("dim", [64, 128])

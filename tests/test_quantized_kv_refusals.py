@@ -40,3 +40,18 @@ def test_page_tables_refuse_operands_off_their_boundary(rpa_lib, which):
     at = [ONE] * 12
     at[which] += 2
     assert rpa_lib.ejk_page_tables_launch(*at, 2, 2, 16, 8, 4, None) == -8
+
+
+@pytest.mark.parametrize("kw", [dict(logits_soft_cap=1e-60), dict(logits_soft_cap=-1e-44), dict(logits_soft_cap=1e60), dict(logits_soft_cap=3e30),
+                                dict(softmax_scale=1e60), dict(softmax_scale=-3e38), dict(logits_soft_cap=1e-30, softmax_scale=1e30)])
+def test_attention_refuses_numbers_that_float32_does_not_hold(kw):
+    """A cap that rounds to zero would be no cap; one whose quotient overflows makes NaN of a logit of zero."""
+    with pytest.raises(ValueError, match="float32"):
+        attend(make(), **kw)
+
+
+@pytest.mark.parametrize("scale, cap", [(3e38, 0.0), (1.0, 3e30), (1.0, 1e-44), (1e30, 1e-30)])
+def test_the_c_entry_refuses_factors_that_overflow(rpa_lib, scale, cap):
+    attrs = _cabi.Attrs(scale, cap, 0, 0, 0, 0, 0, 0.0, 0.0)
+    rc = rpa_lib.ejk_q8_attention_launch(*[ONE] * 7, None, ONE, ONE, 1 << 30, None, ctypes.byref(_cabi.Q8Shape(**SHAPE)), ctypes.byref(attrs), None)
+    assert rc == -6
