@@ -102,7 +102,7 @@ __global__ void __launch_bounds__(kThreads) q8_gather_kernel(const Params p, con
         for (int i = 0; i < 16; ++i) dot = fmaf(Code::decode((uint8_t)(ww[i >> 2] >> (8 * (i & 3)))), s_q[d + i], dot);
       }
       dot *= ks;
-      y = p.cap != 0.f ? p.cap_log2 * soft_cap_tanh(dot * p.inv_cap_scale) : dot * p.scale_log2;
+      y = p.cap != 0.f ? soft_cap_large(p.cap_log2, dot * p.inv_cap_scale) : dot * p.scale_log2;
     }
     const float m_new = fmaxf(m, block_reduce(y, true, s_red));
     const float mu = m_new == -INFINITY ? 0.f : m_new;

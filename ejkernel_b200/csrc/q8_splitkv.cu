@@ -694,13 +694,21 @@ q8_splitkv_kernel(const __grid_constant__ CUtensorMap tmap, const Params p, cons
         float mx[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
+          auto each = [&](auto f) {
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) sc[nt][b][e] = f(sc[nt][b][e] * (q_fac[nt][e & 1] * ks[b * 2 + (e >> 1)]));
+          };
+          if (p.cap == 0.f) each([](float x) { return x; });
+          else if (fabsf(p.cap) <= kPlainCap) each([&](float x) { return p.cap_log2 * soft_cap_tanh(x); });
+          else each([&](float x) { return soft_cap_large(p.cap_log2, x); });
 #pragma unroll
           for (int b = 0; b < 2; ++b)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const int j = e & 1;
-              float x = sc[nt][b][e] * (q_fac[nt][j] * ks[b * 2 + (e >> 1)]);
-              if (p.cap != 0.f) x = p.cap_log2 * soft_cap_tanh(x);
+              float x = sc[nt][b][e];
               if (need_mask) {
                 // a 128-token stage can straddle the end of a chunk (chunks are cut at multiples of 64): keys from
                 // kv_end on belong to the next chunk, or to nobody

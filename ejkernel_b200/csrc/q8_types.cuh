@@ -106,6 +106,16 @@ __device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 x) { retu
 template <>
 __device__ __forceinline__ float to_float<__half>(__half x) { return __half2float(x); }
 
+// cap_log2 * tanh(t) as cap_log2 * (1 - 2 / (e^2t + 1)) is off by up to cap * 2^-22, which is an error of the logit: up to this cap it
+// stays below 2^-12.  Beyond it small t go through tanh's series, t - t^3/3 + 2t^5/15 - 17t^7/315 + 62t^9/2835, whose next term is
+// 1e-8 of the value at 1/4; the tensor tiles do not have that form and leave such calls to the other kernels.
+constexpr float kPlainCap = 1024.f;
+__device__ __forceinline__ float soft_cap_large(float cap_log2, float t) {
+  const float s = t * t;
+  const float y = t + t * s * (-1.f / 3.f + s * (2.f / 15.f + s * (-17.f / 315.f + s * (62.f / 2835.f))));
+  return cap_log2 * (fabsf(t) < 0.25f ? y : soft_cap_tanh(t));
+}
+
 // Offsets of a sequence that no kernel serves (they report it): its rows that there are, are zero.
 __device__ __forceinline__ bool bad_rows(int q0, int q1, int T) { return q1 < q0 || q0 < 0 || q1 > T; }
 

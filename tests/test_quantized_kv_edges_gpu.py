@@ -145,6 +145,16 @@ def test_windows_beyond_32_bits_hide_nothing(rows):
     assert launches() == 1
 
 
+@pytest.mark.parametrize("rows, page", [(1, 16), (90, 16), (3, 5)])
+@pytest.mark.parametrize("cap", [1000.0, 5e3, -2e5, 1e9, 2.0**100])
+def test_large_soft_caps(rows, page, cap):
+    """cap * tanh(x / cap) of logits far below the cap: 1 - 2 / (e^2t + 1) would lose them, cap * 2^-22 each."""
+    b = make_batch([(rows, 200), (1, 33)], Hq=4, Hkv=2, dim=64, page=page, block=1, code=torch.int8, half=torch.float16, seed=26)
+    check_rows(b, run(b, logits_soft_cap=cap), logits_soft_cap=cap)
+    b["q"] = b["q"] * 30
+    check_rows(b, run(b, logits_soft_cap=cap, softmax_scale=0.02), logits_soft_cap=cap, softmax_scale=0.02)
+
+
 @pytest.mark.parametrize("rows", [1, 90])
 @pytest.mark.parametrize("kw", [dict(logits_soft_cap=2.0**-90, softmax_scale=1.0), dict(softmax_scale=2.0**-140)])
 def test_caps_and_scales_at_the_ends_of_float32(rows, kw):
