@@ -153,12 +153,12 @@ int ejk_q8_attention_launch(const void* queries, const void* kv_pages, const flo
   const int n_sm = sm100_sm_count();
   if (!n_sm) return EJK_RPA_E_DEVICE;
   if (kQ8TicketsPerCta * 2 * n_sm * sizeof(int32_t) > EJK_Q8_TICKET_BYTES) return EJK_RPA_E_DEVICE;
-  const bool tiles = tiles_possible(s, a.num_queries_per_block) && std::fabs(a.logits_soft_cap) <= kPlainCap;
+  const bool tiles = tiles_possible(s, a.num_queries_per_block);
   const Q8Workspace W = q8_workspace(s, n_sm, tiles);
   if (workspace_bytes < W.total || (reinterpret_cast<uintptr_t>(workspace) & 255)) return EJK_RPA_E_WORKSPACE;
 
   const LaunchOptions opt = launch_options();
-  const bool use_tma = opt.path != 1 && q8_tma_supported(s.page_size);
+  const bool use_tma = opt.path != 1 && q8_tma_supported(s.page_size) && std::fabs(a.logits_soft_cap) <= kPlainCap;
   if (opt.path == 2 && !use_tma) return EJK_RPA_E_ARG;
 
   Params p;

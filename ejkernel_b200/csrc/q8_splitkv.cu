@@ -18,11 +18,11 @@
 //     products run on f16 mma.sync with float32 sums.  8-bit operands would halve the mma work, which is not what bounds
 //     the kernel, and would round q and p to 3 bits of mantissa.  (Eight warps in two teams that take the stages in turn
 //     were slower: 0.50 ms against 0.37 for 128 sequences of 8192 keys; the registers go down to 96.)
-//   * k_scale multiplies the finished dot product, v_scale the probability: a few multiplications a token and row, none per
-//     element.  p * v_scale has to fit f16: a row divides v_scale by a power of two, chosen from the largest scale that
-//     it has seen so that the product is at most 2^15, and moves it as it moves m.  What is below 2^-24 of that
-//     range is lost: 2^-31 of the largest |V| that the row sees.  (One power of two for all rows of a tile would let a key that
-//     the mask hides from a row push that row's values out of f16.)
+//   * k_scale multiplies the finished dot product, v_scale the probability: two multiplications a token and row, none per
+//     element.  p * v_scale has to fit f16: a warp divides v_scale by a power of two, chosen from the largest scale that
+//     it has met so that the product is at most 2^15, and moves it as it moves m.  What is below 2^-24 of that range is lost:
+//     2^-31 of the largest |V| that the row sees.  In a tile of several tokens the largest scale met can be one that the mask hides
+//     from a row; where scales lie 2^11 and more apart there, the piece's rows are computed one by one at its end (far_row).
 //   * bf16 queries go to f16 by a power of two per row (their largest element to [2^14, 2^15)), undone on the logits.
 //
 // Every wait on an mbarrier is bounded in wall time (option "wait_ms"): on expiry the warp raises
@@ -46,7 +46,8 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kMergeInFlight = 8;     // parts whose loads a merge keeps in flight per row
 constexpr int kGroup = 16;            // parts that are combined at a time: more go through groups
 constexpr float kLazyRescale = 8.0f;  // rescale the accumulators only when the max grows by 2^8: p <= 2^8
-constexpr int kVBits = 6;             // the largest v_scale seen so far is taken to [2^6, 2^7): p * v_scale <= 2^15 < 65504
+constexpr float kFar = 0x1p-5f;       // a scale below this in those units lies far from the largest: see far_row
+constexpr int kVBits = 6;             // the largest v_scale met so far is taken to [2^6, 2^7): p * v_scale <= 2^15 < 65504
 
 // One piece of work of a CTA: stages of one (row tile, kv head).  Of a pair that several CTAs share, u.n_chunks is the number of
 // parts, u.chunk_idx this part's number and u.merge_idx the CTA of part 0; u.slot is where this part goes, u.pad where part 0 is.
@@ -180,6 +181,87 @@ __device__ __forceinline__ Arrival arrive_group(int* tickets, int n_cta, int c0,
   const int groups = (n_parts + kGroup - 1) / kGroup;
   const unsigned old = atomicInc(reinterpret_cast<unsigned*>(tickets + 2 * n_cta + c0), (unsigned)groups - 1u);
   return {old == (unsigned)groups - 1u ? groups : 0, kGroup, 0, true};
+}
+
+// The power of two that takes the largest V scale met to [2^6, 2^7)
+__device__ __forceinline__ float scale_unit(float top) {
+  uint32_t e = __float_as_uint(top) >> 23;
+  e = e < 8u ? 8u : e;
+  return __uint_as_float((254u + kVBits - e) << 23);
+}
+
+// One query row of a piece by one warp, everything in float32: a lane computes one key's logit, then the lanes share out head_dim.
+// It is for tiles of several tokens where a scale of V that some row does not see lies far above one that it does: one power of
+// two for the tile's rows would push what the latter multiplies out of f16.  A call, at the end of the piece: the code of such
+// cases in line cost decode batches 2 to 7 % and prompts at head_dim 256 up to 20 %.
+struct FarRow {
+  const void* q;
+  const int32_t* table;
+  const uint8_t* pages;
+  const float* scales;
+  int32_t num_pages, page_size, Hkv, h, block_shift, key0, key1;
+  float scale_log2, cap_log2, inv_cap_scale;  // cap_log2 == 0: no cap
+  float m, l, o[8];                           // out: maximum, sum, this lane's columns
+};
+template <typename T, typename Code, int D>
+__device__ __noinline__ void far_row(FarRow* r) {
+  constexpr int VPL = D / 32;
+  const int lane = threadIdx.x & 31, bpp = r->page_size >> r->block_shift;
+  const T* q = static_cast<const T*>(r->q);
+  float m = -INFINITY, l = 0.f, o[VPL];
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) o[i] = 0.f;
+#pragma unroll 1
+  for (int base = r->key0; base < r->key1; base += 32) {
+    const int key = base + lane;
+    float y = -INFINITY, vs = 0.f;
+    long long v_row = 0;
+    if (key < r->key1) {
+      const int pi = key / r->page_size, off = key - pi * r->page_size;
+      int page = r->table[pi];
+      if ((unsigned)page >= (unsigned)r->num_pages) page = 0;  // reported by the producer
+      const long long plane = ((long long)page * r->Hkv + r->h) * 2;
+      const uint8_t* k = r->pages + (plane * r->page_size + off) * D;
+      const float ks = r->scales[plane * bpp + (off >> r->block_shift)];
+      vs = r->scales[(plane + 1) * bpp + (off >> r->block_shift)];
+      v_row = ((plane + 1) * r->page_size + off) * D;
+      float dot = 0.f;
+#pragma unroll 1
+      for (int d = 0; d < D; d += 16) {
+        const uint4 c = *reinterpret_cast<const uint4*>(k + d);
+        const uint32_t cw[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+        for (int i = 0; i < 16; ++i) dot = fmaf(Code::decode((uint8_t)(cw[i >> 2] >> (8 * (i & 3)))), to_float(q[d + i]), dot);
+      }
+      dot *= ks;
+      y = r->cap_log2 != 0.f ? r->cap_log2 * soft_cap_tanh(dot * r->inv_cap_scale) : dot * r->scale_log2;
+    }
+    float top = y;
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
+    const float m_new = fmaxf(m, top), mu = m_new == -INFINITY ? 0.f : m_new;
+    const float f = fast_exp2(m - mu), e = fast_exp2(y - mu);
+    m = m_new;
+    float sum = e;
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
+    l = l * f + sum;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) o[i] *= f;
+    const float w = key < r->key1 ? e * vs : 0.f;
+    const int n = min(r->key1 - base, 32);
+#pragma unroll 1
+    for (int j = 0; j < n; ++j) {
+      const float wj = __shfl_sync(0xffffffffu, w, j);
+      const uint8_t* v = r->pages + __shfl_sync(0xffffffffu, v_row, j) + lane * VPL;
+#pragma unroll
+      for (int i = 0; i < VPL; ++i) o[i] = fmaf(wj, Code::decode(v[i]), o[i]);
+    }
+  }
+  r->m = m;
+  r->l = l;
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) r->o[i] = o[i];
 }
 
 template <typename T, typename Code, int D, int NT, int NS>
@@ -547,7 +629,9 @@ q8_splitkv_kernel(const __grid_constant__ CUtensorMap tmap, const Params p, cons
     int pos_r[NT][2], lo_r[NT][2];
     int pos_min = 0, lo_max = 0, lo_min = -1;
     bool one_token = true;  // the tile's rows are one query token's: they see the same keys
-    float v_norm[NT][2];  // powers of two that the V scales are multiplied by, one per row
+    float v_norm = 1.f;  // power of two that the V scales are multiplied by
+    bool mixed = false;  // some row has not seen a key that another has
+    bool far = false;    // ... and scales lie far apart: the piece's rows are computed one by one at its end
     int s = 0;
     uint32_t full_parity = 0, c_parity = 0;
     int pieces = 0;
@@ -561,279 +645,270 @@ q8_splitkv_kernel(const __grid_constant__ CUtensorMap tmap, const Params p, cons
       return ok;
     };
 
+    // some row of the tile does not see all of the warp's keys
+    auto masked = [&](int key0, int kv_end) { return key0 + TW > kv_end || (key0 + TW - 1 > pos_min) || (key0 <= lo_max); };
+    // is some V scale of the warp's keys far below the largest that any row has seen?
+    auto far_scales = [&](int pos, int kv_end) {
+      const int key = pos + warp * TW + lane;
+      const float* vs = reinterpret_cast<const float*>(smem + C::OFF_SCALE + s * (2 * TK * 4)) + TK;
+      const bool seen = key < kv_end && key > lo_min;
+      const float v = seen ? vs[(key >> sb_shift) - (pos >> sb_shift)] : 0.f;
+      const float top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v)));
+      const float unit = top * v_norm >= (float)(2 << kVBits) ? scale_unit(top) : v_norm;
+      return __any_sync(0xffffffffu, seen && v * unit < kFar) != 0;
+    };
+    // The warp's 32 keys of a stage
+    auto stage = [&](int pos, int kv_end) {
+      const int key0 = pos + warp * TW;
+      const uint32_t sbase = smem_base + s * C::STAGE_BYTES;
+      // ---- S^T[32 tokens x rows] = K . Q^T as two 16-token blocks
+      float sc[NT][2][4];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[nt][b][e] = 0.f;
+#pragma unroll
+      for (int kt = 0; kt < D / 32; ++kt) {
+        const int c16 = kt * 2;  // 16-byte chunk of the token's row; + k_dhalf at run time
+        const uint32_t coff = (uint32_t)(c16 / CH) * dc_stride + ((((uint32_t)(c16 % CH) | (uint32_t)k_dhalf) << 4) ^ swz);
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          // a[0] = (token g, bytes 4t..4t+3 of the chunk), a[1] = token g+8, a[2] / a[3] = the next chunk.  The low two
+          // bytes of a register become k slots 2t, 2t+1, the high two k slots 8+2t, 8+2t+1 of one f16 mma -- the
+          // query fragments were loaded in the same order
+          uint32_t a[4];
+          ldmatrix_x4(a, sbase + (b ? k_off1 : k_off0) + coff);
+          uint32_t lo[4], hi[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) Code::widen(a[i], lo[i], hi[i]);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            mma_f16(sc[nt][b], lo[0], lo[1], hi[0], hi[1], qf[nt][kt][0], qf[nt][kt][1]);
+            mma_f16(sc[nt][b], lo[2], lo[3], hi[2], hi[3], qf[nt][kt][2], qf[nt][kt][3]);
+          }
+        }
+      }
+      // ---- scales of this lane's four tokens
+      const float* ks_s = reinterpret_cast<const float*>(smem + C::OFF_SCALE + s * (2 * TK * 4));
+      const float* vs_s = ks_s + TK;
+      const int e0 = pos >> sb_shift;
+      float ks[4], vs[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int key = key0 + (lane >> 2) + i * 8;
+        const int e = (key >> sb_shift) - e0;
+        ks[i] = ks_s[e];
+        // no row sees a key from kv_end on, or one that the window of the tile's first row has left behind
+        vs[i] = (key < kv_end && key > lo_min) ? vs_s[e] : 0.f;
+      }
+      const bool tail = key0 + TW > kv_end;  // tokens past the chunk end: stale or unowned bytes
+      const bool edge = tail || key0 <= lo_min;
+      const bool need_mask = masked(key0, kv_end);
+      // the power of two by the largest V scale of the warp's 32 keys (positive floats order as integers)
+      const float top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3])))));
+      if (top * v_norm >= (float)(2 << kVBits)) {
+        // a larger scale than any before: the accumulators go along
+        const float v_new = scale_unit(top);
+        const float f = v_new * power_of_two_inverse(v_norm);  // 0 where the old terms are below anything that counts
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int mt = 0; mt < KT; ++mt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[nt][mt][i] *= f;
+        v_norm = v_new;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) vs[i] *= v_norm;
+      bool grow = false;
+      float mx[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int j = e & 1;
+            float x = sc[nt][b][e] * (q_fac[nt][j] * ks[b * 2 + (e >> 1)]);
+            if (p.cap != 0.f) x = p.cap_log2 * soft_cap_tanh(x);
+            if (need_mask) {
+              // a 128-token stage can straddle the end of a chunk (chunks are cut at multiples of 64): keys from
+              // kv_end on belong to the next chunk, or to nobody
+              const int key = key0 + b * 16 + (lane >> 2) + (e >> 1) * 8;
+              if (key > pos_r[nt][j] || key <= lo_r[nt][j] || key >= kv_end) x = -INFINITY;
+            }
+            sc[nt][b][e] = x;
+          }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float v = fmaxf(fmaxf(sc[nt][0][j], sc[nt][0][j + 2]), fmaxf(sc[nt][1][j], sc[nt][1][j + 2]));
+          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
+          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
+          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
+          mx[nt][j] = v;
+          // lazy rescaling: keep the old reference maximum unless the new one is 2^8 larger
+          grow |= (v > m_run[nt][j] + kLazyRescale) || (m_run[nt][j] == -INFINITY && v > -INFINITY);
+        }
+      }
+      if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float alpha[2];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const bool g = (mx[nt][j] > m_run[nt][j] + kLazyRescale) || (m_run[nt][j] == -INFINITY && mx[nt][j] > -INFINITY);
+            const float m_new = g ? mx[nt][j] : m_run[nt][j];
+            alpha[j] = g ? fast_exp2(m_run[nt][j] - m_new) : 1.f;  // exp2(-inf) = 0 on the first tile
+            m_run[nt][j] = m_new;
+            l_run[nt][j] *= alpha[j];
+          }
+#pragma unroll
+          for (int mt = 0; mt < KT; ++mt) {
+            acc[nt][mt][0] *= alpha[0];
+            acc[nt][mt][1] *= alpha[1];
+            acc[nt][mt][2] *= alpha[0];
+            acc[nt][mt][3] *= alpha[1];
+          }
+        }
+      }
+      // ---- probabilities; times the V scale to f16, transposed into the B fragments of P.V
+      uint32_t pbf[NT][4];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float m_use = (m_run[nt][j] == -INFINITY) ? 0.f : m_run[nt][j];
+            const float p0 = fast_exp2(sc[nt][b][j] - m_use);
+            const float p1 = fast_exp2(sc[nt][b][j + 2] - m_use);
+            l_run[nt][j] += p0 + p1;
+            sc[nt][b][j] = p0 * vs[b * 2];
+            sc[nt][b][j + 2] = p1 * vs[b * 2 + 1];
+          }
+          pbf[nt][b * 2] = movmatrix_trans(Mma<__half>::pack(sc[nt][b][0], sc[nt][b][1]));
+          pbf[nt][b * 2 + 1] = movmatrix_trans(Mma<__half>::pack(sc[nt][b][2], sc[nt][b][3]));
+        }
+      }
+      // ---- V^T fragments: four transposed 8-token matrices of one 16-byte chunk; register j holds, for the two
+      // head-dim lanes 2g and 2g+1, tokens 8j + 2t (low half) and 8j + 2t + 1 (high half): rows g and g+8 of the mma
+      // stand for lanes 16mt + 2g and + 1.  The bytes of keys that no row sees are cleared, so that 0 * (stale
+      // NaN) cannot reach the accumulators.
+      uint32_t vmask[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
+      if (edge) {
+        const int t0 = key0 + (lane & 3) * 2;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int a = t0 + 8 * j;
+          vmask[j] = (a < kv_end && a > lo_min ? 0x0000ffffu : 0u) | (a + 1 < kv_end && a + 1 > lo_min ? 0xffff0000u : 0u);
+        }
+      }
+#pragma unroll
+      for (int mt = 0; mt < KT; ++mt) {
+        uint32_t r[4];
+        ldmatrix_x4_trans(r, sbase + v_off + (uint32_t)(mt / CH) * dc_stride + (((uint32_t)(mt % CH) << 4) ^ swz));
+        if (edge) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) r[j] &= vmask[j];
+        }
+        uint32_t even[4], odd[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) Code::widen_interleaved(r[j], even[j], odd[j]);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          mma_f16(acc[nt][mt], even[0], odd[0], even[1], odd[1], pbf[nt][0], pbf[nt][1]);
+          mma_f16(acc[nt][mt], even[2], odd[2], even[3], odd[3], pbf[nt][2], pbf[nt][3]);
+        }
+      }
+    };
+
     while (true) {
-      if (!mbar_wait(bar_full + s * 8, full_parity, abort_flag, wait_ns)) break;
-      const int2 meta = metas[s];
-      if (meta.x < 0) break;
+      // the stages of a piece
+      int2 meta;
+      bool end = false;
+      while (true) {
+        if (!mbar_wait(bar_full + s * 8, full_parity, abort_flag, wait_ns)) {
+          end = true;
+          break;
+        }
+        meta = metas[s];
+        end = meta.x < 0;
+        if (end) break;
+        const Unit u = ring[meta.x].u;
+        const int pos = meta.y;
+        const int rows_total = u.q_len * G;
+        int n_rows = rows_total - u.row0;
+        if (n_rows > RT) n_rows = RT;
+
+        if (pos == u.kv_begin) {
+          const uint8_t* qs = smem + C::OFF_Q + s * C::Q_BYTES;
+          const float* qfac = reinterpret_cast<const float*>(smem + C::OFF_QFAC + s * RT * 4);
+          const float to_log2 = p.cap != 0.f ? p.inv_cap_scale : p.scale_log2;
+          const int base = u.kv_len - u.q_len;
+          pos_min = base + u.row0 / G;
+          one_token = (u.row0 + n_rows - 1) / G == u.row0 / G;
+          v_norm = __uint_as_float((127u + 125u) << 23);  // no scale met yet: the largest power of two (see below)
+          mixed = far = false;
+          lo_max = (p.window > 0) ? (base + (u.row0 + n_rows - 1) / G - p.window) : -1;
+          lo_min = (p.window > 0) ? pos_min - p.window : -1;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            // elements 32kt + 4t .. +3 (first mma of the chunk) and 32kt + 16 + 4t .. +3 (second)
+            const uint8_t* qrow = qs + (nt * 8 + (lane >> 2)) * C::Q_ROW_BYTES + (lane & 3) * 8;
+#pragma unroll
+            for (int kt = 0; kt < D / 32; ++kt) {
+              const uint2 a = *reinterpret_cast<const uint2*>(qrow + kt * 64);
+              const uint2 b = *reinterpret_cast<const uint2*>(qrow + kt * 64 + 32);
+              qf[nt][kt][0] = a.x;
+              qf[nt][kt][1] = a.y;
+              qf[nt][kt][2] = b.x;
+              qf[nt][kt][3] = b.y;
+            }
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const int r = nt * 8 + (lane & 3) * 2 + j;
+              const int R = u.row0 + r;
+              const int ps = (R < rows_total) ? base + R / G : -1;
+              pos_r[nt][j] = ps;
+              lo_r[nt][j] = (p.window > 0) ? ps - p.window : -1;
+              q_fac[nt][j] = qfac[r] * to_log2;
+              m_run[nt][j] = -INFINITY;
+              l_run[nt][j] = 0.f;
+            }
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) acc[nt][kt][e] = 0.f;
+          }
+        }
+
+        const int key0 = pos + warp * TW;
+        if (key0 < u.kv_end) {
+          if (!one_token) {
+            mixed |= masked(key0, u.kv_end);
+            if (mixed) far |= far_scales(pos, u.kv_end);
+          }
+          stage(pos, u.kv_end);
+        }
+        if (pos + TK >= u.kv_end) break;
+        // this warp is done with the stage's bytes (query fragments are in registers by now)
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_empty + s * 8);
+        if (++s == NS) {
+          s = 0;
+          full_parity ^= 1u;
+        }
+      }
+      if (end) break;
       const ItemDesc& it = ring[meta.x];
       const Unit u = it.u;
       const int h = it.h;
       const bool first_piece = it.first != 0;
       const int pos = meta.y;
-      const uint32_t sbase = smem_base + s * C::STAGE_BYTES;
-      const int rows_total = u.q_len * G;
-      int n_rows = rows_total - u.row0;
+      int n_rows = u.q_len * G - u.row0;
       if (n_rows > RT) n_rows = RT;
-
-      if (pos == u.kv_begin) {
-        const uint8_t* qs = smem + C::OFF_Q + s * C::Q_BYTES;
-        const float* qfac = reinterpret_cast<const float*>(smem + C::OFF_QFAC + s * RT * 4);
-        const float to_log2 = p.cap != 0.f ? p.inv_cap_scale : p.scale_log2;
-        const int base = u.kv_len - u.q_len;
-        pos_min = base + u.row0 / G;
-        one_token = (u.row0 + n_rows - 1) / G == u.row0 / G;
-        lo_max = (p.window > 0) ? (base + (u.row0 + n_rows - 1) / G - p.window) : -1;
-        lo_min = (p.window > 0) ? pos_min - p.window : -1;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          // elements 32kt + 4t .. +3 (first mma of the chunk) and 32kt + 16 + 4t .. +3 (second)
-          const uint8_t* qrow = qs + (nt * 8 + (lane >> 2)) * C::Q_ROW_BYTES + (lane & 3) * 8;
-#pragma unroll
-          for (int kt = 0; kt < D / 32; ++kt) {
-            const uint2 a = *reinterpret_cast<const uint2*>(qrow + kt * 64);
-            const uint2 b = *reinterpret_cast<const uint2*>(qrow + kt * 64 + 32);
-            qf[nt][kt][0] = a.x;
-            qf[nt][kt][1] = a.y;
-            qf[nt][kt][2] = b.x;
-            qf[nt][kt][3] = b.y;
-          }
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const int r = nt * 8 + (lane & 3) * 2 + j;
-            const int R = u.row0 + r;
-            const int ps = (R < rows_total) ? base + R / G : -1;
-            pos_r[nt][j] = ps;
-            lo_r[nt][j] = (p.window > 0) ? ps - p.window : -1;
-            q_fac[nt][j] = qfac[r] * to_log2;
-            m_run[nt][j] = -INFINITY;
-            l_run[nt][j] = 0.f;
-            v_norm[nt][j] = __uint_as_float((127u + 125u) << 23);  // no scale seen yet: the largest power of two (see below)
-          }
-#pragma unroll
-          for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[nt][kt][e] = 0.f;
-        }
-      }
-
-      const int key0 = pos + warp * TW;
-      if (key0 < u.kv_end) {
-        // ---- S^T[32 tokens x rows] = K . Q^T as two 16-token blocks
-        float sc[NT][2][4];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int b = 0; b < 2; ++b)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) sc[nt][b][e] = 0.f;
-#pragma unroll
-        for (int kt = 0; kt < D / 32; ++kt) {
-          const int c16 = kt * 2;  // 16-byte chunk of the token's row; + k_dhalf at run time
-          const uint32_t coff = (uint32_t)(c16 / CH) * dc_stride + ((((uint32_t)(c16 % CH) | (uint32_t)k_dhalf) << 4) ^ swz);
-#pragma unroll
-          for (int b = 0; b < 2; ++b) {
-            // a[0] = (token g, bytes 4t..4t+3 of the chunk), a[1] = token g+8, a[2] / a[3] = the next chunk.  The low two
-            // bytes of a register become k slots 2t, 2t+1, the high two k slots 8+2t, 8+2t+1 of one f16 mma -- the
-            // query fragments were loaded in the same order
-            uint32_t a[4];
-            ldmatrix_x4(a, sbase + (b ? k_off1 : k_off0) + coff);
-            uint32_t lo[4], hi[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) Code::widen(a[i], lo[i], hi[i]);
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              mma_f16(sc[nt][b], lo[0], lo[1], hi[0], hi[1], qf[nt][kt][0], qf[nt][kt][1]);
-              mma_f16(sc[nt][b], lo[2], lo[3], hi[2], hi[3], qf[nt][kt][2], qf[nt][kt][3]);
-            }
-          }
-        }
-        // ---- scales of this lane's four tokens
-        const float* ks_s = reinterpret_cast<const float*>(smem + C::OFF_SCALE + s * (2 * TK * 4));
-        const float* vs_s = ks_s + TK;
-        const int e0 = pos >> sb_shift;
-        float ks[4], vs[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int key = key0 + (lane >> 2) + i * 8;
-          const int e = (key >> sb_shift) - e0;
-          ks[i] = ks_s[e];
-          // no row sees a key from kv_end on, or one that the window of the tile's first row has left behind
-          vs[i] = (key < u.kv_end && key > lo_min) ? vs_s[e] : 0.f;
-        }
-        const bool tail = key0 + TW > u.kv_end;  // tokens past the chunk end: stale or unowned bytes
-        const bool edge = tail || key0 <= lo_min;
-        const bool need_mask = tail || (key0 + TW - 1 > pos_min) || (key0 <= lo_max);
-        // takes the rows' accumulators to the power of two that the largest V scale asks for: that one to [2^6, 2^7)
-        auto larger_scale = [&](float top, float& norm) {
-          uint32_t e = __float_as_uint(top) >> 23;
-          e = e < 8u ? 8u : e;
-          const float v_new = __uint_as_float((254u + kVBits - e) << 23);
-          const float f = v_new * power_of_two_inverse(norm);  // 0 where the old terms are below anything that counts
-          norm = v_new;
-          return f;
-        };
-        if (one_token) {
-          // the rows see the same keys: one power of two, by the largest V scale of the warp's 32 (positive floats order as
-          // integers)
-          const float top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3])))));
-          if (top * v_norm[0][0] >= (float)(2 << kVBits)) {
-            const float f = larger_scale(top, v_norm[0][0]);
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              v_norm[nt][0] = v_norm[nt][1] = v_norm[0][0];
-#pragma unroll
-              for (int mt = 0; mt < KT; ++mt)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) acc[nt][mt][i] *= f;
-            }
-          }
-#pragma unroll
-          for (int i = 0; i < 4; ++i) vs[i] *= v_norm[0][0];
-        }
-        bool grow = false;
-        float mx[NT][2];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          auto each = [&](auto f) {
-#pragma unroll
-            for (int b = 0; b < 2; ++b)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) sc[nt][b][e] = f(sc[nt][b][e] * (q_fac[nt][e & 1] * ks[b * 2 + (e >> 1)]));
-          };
-          if (p.cap == 0.f) each([](float x) { return x; });
-          else if (fabsf(p.cap) <= kPlainCap) each([&](float x) { return p.cap_log2 * soft_cap_tanh(x); });
-          else each([&](float x) { return soft_cap_large(p.cap_log2, x); });
-#pragma unroll
-          for (int b = 0; b < 2; ++b)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int j = e & 1;
-              float x = sc[nt][b][e];
-              if (need_mask) {
-                // a 128-token stage can straddle the end of a chunk (chunks are cut at multiples of 64): keys from
-                // kv_end on belong to the next chunk, or to nobody
-                const int key = key0 + b * 16 + (lane >> 2) + (e >> 1) * 8;
-                if (key > pos_r[nt][j] || key <= lo_r[nt][j] || key >= u.kv_end) x = -INFINITY;
-              }
-              sc[nt][b][e] = x;
-            }
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            float v = fmaxf(fmaxf(sc[nt][0][j], sc[nt][0][j + 2]), fmaxf(sc[nt][1][j], sc[nt][1][j + 2]));
-            v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
-            v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
-            v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
-            mx[nt][j] = v;
-            // lazy rescaling: keep the old reference maximum unless the new one is 2^8 larger
-            grow |= (v > m_run[nt][j] + kLazyRescale) || (m_run[nt][j] == -INFINITY && v > -INFINITY);
-          }
-        }
-        if (__any_sync(0xffffffffu, grow)) {
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            float alpha[2];
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              const bool g = (mx[nt][j] > m_run[nt][j] + kLazyRescale) || (m_run[nt][j] == -INFINITY && mx[nt][j] > -INFINITY);
-              const float m_new = g ? mx[nt][j] : m_run[nt][j];
-              alpha[j] = g ? fast_exp2(m_run[nt][j] - m_new) : 1.f;  // exp2(-inf) = 0 on the first tile
-              m_run[nt][j] = m_new;
-              l_run[nt][j] *= alpha[j];
-            }
-#pragma unroll
-            for (int mt = 0; mt < KT; ++mt) {
-              acc[nt][mt][0] *= alpha[0];
-              acc[nt][mt][1] *= alpha[1];
-              acc[nt][mt][2] *= alpha[0];
-              acc[nt][mt][3] *= alpha[1];
-            }
-          }
-        }
-        // ---- probabilities; times the V scale to f16, transposed into the B fragments of P.V
-        uint32_t pbf[NT][4];
-        auto weights = [&](auto same) {
-          // same: the rows see the same keys and share the power of two, which has gone into vs
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-            for (int b = 0; b < 2; ++b) {
-#pragma unroll
-              for (int j = 0; j < 2; ++j) {
-                const float m_use = (m_run[nt][j] == -INFINITY) ? 0.f : m_run[nt][j];
-                const float p0 = fast_exp2(sc[nt][b][j] - m_use);
-                const float p1 = fast_exp2(sc[nt][b][j + 2] - m_use);
-                l_run[nt][j] += p0 + p1;
-                if constexpr (decltype(same)::value) {
-                  sc[nt][b][j] = p0 * vs[b * 2];
-                  sc[nt][b][j + 2] = p1 * vs[b * 2 + 1];
-                } else {
-                  // a key without weight has none whatever its scale: it may be one that the row does not see
-                  sc[nt][b][j] = p0 == 0.f ? 0.f : p0 * (vs[b * 2] * v_norm[nt][j]);
-                  sc[nt][b][j + 2] = p1 == 0.f ? 0.f : p1 * (vs[b * 2 + 1] * v_norm[nt][j]);
-                }
-              }
-              pbf[nt][b * 2] = movmatrix_trans(Mma<__half>::pack(sc[nt][b][0], sc[nt][b][1]));
-              pbf[nt][b * 2 + 1] = movmatrix_trans(Mma<__half>::pack(sc[nt][b][2], sc[nt][b][3]));
-            }
-          }
-        };
-        if (one_token) {
-          weights(std::true_type{});
-        } else {
-          // a power of two for each row, by the largest V scale among the keys that it sees
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              float top = 0.f;
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                if (sc[nt][i >> 1][(i & 1) * 2 + j] != -INFINITY) top = fmaxf(top, vs[i]);
-              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-              if (top * v_norm[nt][j] >= (float)(2 << kVBits)) {
-                const float f = larger_scale(top, v_norm[nt][j]);
-#pragma unroll
-                for (int mt = 0; mt < KT; ++mt) {
-                  acc[nt][mt][j] *= f;
-                  acc[nt][mt][j + 2] *= f;
-                }
-              }
-            }
-          weights(std::false_type{});
-        }
-        // ---- V^T fragments: four transposed 8-token matrices of one 16-byte chunk; register j holds, for the two
-        // head-dim lanes 2g and 2g+1, tokens 8j + 2t (low half) and 8j + 2t + 1 (high half): rows g and g+8 of the mma
-        // stand for lanes 16mt + 2g and + 1.  The bytes of keys that no row sees are cleared, so that 0 * (stale
-        // NaN) cannot reach the accumulators.
-        uint32_t vmask[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
-        if (edge) {
-          const int t0 = key0 + (lane & 3) * 2;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int a = t0 + 8 * j;
-            vmask[j] = (a < u.kv_end && a > lo_min ? 0x0000ffffu : 0u) | (a + 1 < u.kv_end && a + 1 > lo_min ? 0xffff0000u : 0u);
-          }
-        }
-#pragma unroll
-        for (int mt = 0; mt < KT; ++mt) {
-          uint32_t r[4];
-          ldmatrix_x4_trans(r, sbase + v_off + (uint32_t)(mt / CH) * dc_stride + (((uint32_t)(mt % CH) << 4) ^ swz));
-          if (edge) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) r[j] &= vmask[j];
-          }
-          uint32_t even[4], odd[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) Code::widen_interleaved(r[j], even[j], odd[j]);
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            mma_f16(acc[nt][mt], even[0], odd[0], even[1], odd[1], pbf[nt][0], pbf[nt][1]);
-            mma_f16(acc[nt][mt], even[2], odd[2], even[3], odd[3], pbf[nt][2], pbf[nt][3]);
-          }
-        }
-      }
       if (pos + TK >= u.kv_end) {
         // ---- end of the piece.  The warps' accumulators meet in the memory of its last stage: with the first barrier every
         // warp is done with the stage and has published its rows' (m, l), with the second all accumulators are there; from
@@ -848,7 +923,8 @@ q8_splitkv_kernel(const __grid_constant__ CUtensorMap tmap, const Params p, cons
             l += __shfl_xor_sync(0xffffffffu, l, 4);
             l += __shfl_xor_sync(0xffffffffu, l, 8);
             l += __shfl_xor_sync(0xffffffffu, l, 16);
-            if (lane < 4) ml[warp * RT + nt * 8 + lane * 2 + j] = make_float2(m_run[nt][j], l);
+            // (the sum's sign: the rows have to be computed one by one)
+            if (lane < 4) ml[warp * RT + nt * 8 + lane * 2 + j] = make_float2(m_run[nt][j], far ? -l : l);
           }
         if (!consumer_sync()) break;
         // accumulators relative to the rows' common maximum, without the power of two that this warp took the row's V scales
@@ -862,7 +938,7 @@ q8_splitkv_kernel(const __grid_constant__ CUtensorMap tmap, const Params p, cons
             float mt = -INFINITY;
 #pragma unroll
             for (int w = 0; w < kConsumerWarps; ++w) mt = fmaxf(mt, ml[w * RT + r].x);
-            const float f = fast_exp2(m_run[nt][j] - ((mt == -INFINITY) ? 0.f : mt)) * power_of_two_inverse(v_norm[nt][j]);
+            const float f = fast_exp2(m_run[nt][j] - ((mt == -INFINITY) ? 0.f : mt)) * power_of_two_inverse(v_norm);
             // accumulator rows g / g+8 of block mt are head-dim lanes 16mt + 2g / + 1 (see the V fragments)
             float* row = sum + (warp * RT + r) * D + (lane >> 2) * 2;
 #pragma unroll
@@ -905,11 +981,16 @@ q8_splitkv_kernel(const __grid_constant__ CUtensorMap tmap, const Params p, cons
         for (int ri = 0; ri < RPW; ++ri) {
           const int r = warp + ri * kConsumerWarps;
           float m_tot = -INFINITY, l_tot = 0.f;
+          uint32_t any_far = 0;
 #pragma unroll
           for (int w = 0; w < kConsumerWarps; ++w) m_tot = fmaxf(m_tot, ml[w * RT + r].x);
           const float mu = (m_tot == -INFINITY) ? 0.f : m_tot;
 #pragma unroll
-          for (int w = 0; w < kConsumerWarps; ++w) l_tot += ml[w * RT + r].y * fast_exp2(ml[w * RT + r].x - mu);
+          for (int w = 0; w < kConsumerWarps; ++w) {
+            const float l = ml[w * RT + r].y;
+            any_far |= __float_as_uint(l) >> 31;
+            l_tot += fabsf(l) * fast_exp2(ml[w * RT + r].x - mu);
+          }
           const int col = lane * VPL;
           const float* src = sum + r * D + (((col >> 4) ^ ((r >> 1) & 3)) << 4) + (col & 15);
           float o[VPL];
@@ -924,6 +1005,30 @@ q8_splitkv_kernel(const __grid_constant__ CUtensorMap tmap, const Params p, cons
               o[i + 1] += v.y;
             }
           if (r >= n_rows) continue;
+          if (__builtin_expect(any_far != 0, 0)) {
+            const int R = u.row0 + r, qt = R / G;
+            const int at = u.kv_len - u.q_len + qt;  // the row's position
+            FarRow f;
+            f.q = reinterpret_cast<const T*>(p.q) + ((size_t)(u.q_start + qt) * p.Hq + h * G + (R - qt * G)) * D;
+            f.table = p.block_tables + (size_t)u.seq * p.pages_per_seq;
+            f.pages = cache.pages;
+            f.scales = cache.scales;
+            f.num_pages = p.num_pages;
+            f.page_size = p.page_size;
+            f.Hkv = Hkv;
+            f.h = h;
+            f.block_shift = cache.block_shift;
+            f.key0 = max(u.kv_begin, p.window > 0 ? at - p.window + 1 : 0);
+            f.key1 = min(u.kv_end, at + 1);
+            f.scale_log2 = p.scale_log2;
+            f.cap_log2 = p.cap_log2;
+            f.inv_cap_scale = p.inv_cap_scale;
+            far_row<T, Code, D>(&f);
+            m_tot = f.m;
+            l_tot = f.l;
+#pragma unroll
+            for (int i = 0; i < VPL; ++i) o[i] = f.o[i];
+          }
           if (u.slot < 0) store_row(r, m_tot, l_tot, o);
           else store_part(u.slot, r, m_tot, l_tot, o);
         }
@@ -996,7 +1101,6 @@ q8_splitkv_kernel(const __grid_constant__ CUtensorMap tmap, const Params p, cons
           }
         }
       } else {
-        // this warp is done with the stage's bytes (query fragments are in registers by now)
         __syncwarp();
         if (lane == 0) mbar_arrive(bar_empty + s * 8);
       }

@@ -108,7 +108,8 @@ __device__ __forceinline__ float to_float<__half>(__half x) { return __half2floa
 
 // cap_log2 * tanh(t) as cap_log2 * (1 - 2 / (e^2t + 1)) is off by up to cap * 2^-22, which is an error of the logit: up to this cap it
 // stays below 2^-12.  Beyond it small t go through tanh's series, t - t^3/3 + 2t^5/15 - 17t^7/315 + 62t^9/2835, whose next term is
-// 1e-8 of the value at 1/4; the tensor tiles do not have that form and leave such calls to the other kernels.
+// 1e-8 of the value at 1/4.  The pipelined kernels do not have that form (in line it cost every decode batch 1 to 7 %): such calls
+// go to the simple one.
 constexpr float kPlainCap = 1024.f;
 __device__ __forceinline__ float soft_cap_large(float cap_log2, float t) {
   const float s = t * t;
