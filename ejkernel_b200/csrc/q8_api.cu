@@ -217,8 +217,11 @@ int ejk_q8_attention_launch(const void* queries, const void* kv_pages, const flo
   p.tma_block_shift = log2_exact(p.tma_block_tokens);
   p.wait_timeout_ms = opt.wait_ms;
   p.test_withhold = opt.test_withhold;
-  // Batches that can hold a sequence with many query rows also get the tensor-tile kernel; whether one qualifies is
-  // decided by the planner on the device.
+  // Batches that can hold a sequence with many query rows also get the tensor-tile kernel; whether one qualifies is decided by the
+  // planner on the device.  From 32 rows on (8 tokens at 4 heads per kv head): 64 requests of 6 tokens over 2000 keys take 160 us in
+  // row tiles and 229 in tensor tiles, of 8 tokens 205 and 217, of 16 tokens 373 and 217; 8 requests over 8000 keys 92 and 125,
+  // 109 and 125, 190 and 133; 128 over 500 keys 121 and 154, 139 and 137, 266 and 139.  Few short requests would gain from a higher
+  // threshold (8 of 8 tokens over 2000 keys 45 and 70): num_queries_per_block is theirs.
   int prefill_rows = opt.prefill_rows;
   if (a.num_queries_per_block > 0) {  // per-call hint: query tokens from which on a sequence is served by tensor tiles
     const long long r = (long long)a.num_queries_per_block * p.G;

@@ -26,15 +26,16 @@
 //   * registers: 16 warps have 128 registers a thread; the issuing warps and the converters give theirs to the softmax
 //     warps (setmaxnreg: 72 + 72 + 2 * 184 = 4 * 128).
 //
-// What bounds it: neither the tensor pipe nor the exponentials (each about a third busy) but the softmax threads' instructions
-// and the instruction cache that five roles share; a stage of two tiles takes 3200 cycles where the 16-bit kernel takes 2500.
-// 4 sequences x 2048 rows over 8192 keys, 32 heads over 8 kv heads of 128: 1.34 ms = 716 TFLOP/s (16-bit operator 1.05 ms); on the
-// way there: all of a stage unrolled in the converters 2.57, a rolled loop 1.73, no rare paths in the common kernel and paired
-// float32 instructions 1.49, no turns between the tiles at the exponentials (which the 16-bit kernel gains from) 1.39, a planner
-// of its own 1.34.  With blocks of 4 tokens 4 chunks of up to 2048 rows (504 us) take 565 us, with a soft cap 804: 664 and 898 before
-// the factors and tanh went two columns to an instruction.  An item of one tile is bound by how long a stage takes to come through:
-// 24 mixed requests with pages of 24 tokens 82 us while the producer divided for each page and scale, 65 with the stepped indexes.
-// Tried and dropped: two threads per row with half of the columns each (1.73), eight converter warps (1.46).
+// What bounds it: neither the tensor pipe nor the exponentials (0.37 busy each; float and integer instructions 0.45, issue slots 0.53)
+// but the softmax threads' instructions and the instruction cache that five roles share.  4 chunks of 1740 to 1995 rows over 2136
+// to 6000 keys, 32 heads over 8 kv heads of 128 (360 GFLOP): 498 us = 0.72 PFLOP/s; int8 codes 526, scale blocks of 4 tokens 560, pages
+// of 24 tokens 517, a soft cap 808, head_dim 64 412, all stages far 1490.  4 sequences of 2048 rows over 8192 keys each: 1.11 ms.
+// On the way there (a batch of that kind, ms): all of a stage unrolled in the converters 2.57, a rolled loop 1.73, no rare paths in
+// the common kernel and paired float32 instructions 1.49, no turns between the tiles at the exponentials (which the 16-bit kernel gains
+// from) 1.39, a planner of its own 1.34; the end of an item out of the loop of its stages another 2 to 6 %.  An item of one tile is
+// bound by how long a stage takes to come through: 24 mixed requests with pages of 24 tokens 82 us while the producer divided for
+// each page and scale, 15 to 20 % less with the stepped indexes.  Tried and dropped: two threads per row with half of the columns
+// each (1.73), eight converter warps (1.46).
 //
 // Warp roles (512 threads, one CTA per SM, persistent over the items of q8_plan.cu):
 //   warp 0 producer, warp 1 S of tile 0 (and the TMEM allocation), warp 2 S of tile 1, warp 3 P.V of all tiles,
@@ -360,7 +361,9 @@ q8_prefill_kernel(const Params p, const Q8Cache cache) {
   if ((p.pdl & 1) && p.prefill_share > 0) {
     const float stages = (float)p.header[kHdrPrefillStages] * (float)Hkv;           // (item, head) stages of 64 tokens
     const float dec_bytes = (float)p.header[kHdrTotalKeys] * (float)Hkv * (float)(2 * D);
-    // one stage of two 128-row tiles, and what a soft cap's tanh adds
+    // One stage of two 128-row tiles (also taken for items of one), and what a soft cap's tanh adds; the rate is an upper estimate
+    // of the split-KV kernel's (4.8 to 6.3 TB/s), which the share above 100 makes good: 96 decode rows of 6000 keys beside 4 chunks of 512 tokens
+    // 399 us at 125, 479 at 100, 569 at 75, 408 with no share taken; batches with less to decode do not depend on it
     const float kStageUs = (D == 64 ? 1.15f : 1.25f) * (p.cap != 0.f ? 1.6f : 1.f);
     constexpr float kDecodeBpUs = 6.6e6f;  // bytes per microsecond the split-KV kernel streams
     const float t_p = stages * kStageUs / (float)gridDim.x, t_d = dec_bytes / kDecodeBpUs;

@@ -40,7 +40,6 @@ struct CodeE4M3 {
     widen(prmt(w, w, 0x3120u), even, odd);
   }
 
-  static constexpr int kId = EJK_RPA_E4M3;
   static constexpr float kMax = 448.f;
   static __device__ __forceinline__ float decode(uint8_t c) {
     uint32_t h;
@@ -76,7 +75,6 @@ struct CodeI8 {
     odd = less_1152(prmt(w, 0x64646464u, 0x4341u));
   }
 
-  static constexpr int kId = EJK_Q8_I8;
   static constexpr float kMax = 127.f;
   static __device__ __forceinline__ float decode(uint8_t c) { return (float)(int8_t)c; }
   static __device__ __forceinline__ uint32_t encode2(float a, float b) {

@@ -504,7 +504,9 @@ def build_page_tables(
     can be given to a new request with the next call.  ``slot_mapping`` has ``total_tokens`` entries,
     ``page * page_size + offset`` each, -1 behind the last sequence and for rows that could not be served (the stack ran
     out, the row's table is too short, the batch exceeds ``total_tokens``): such a row keeps its length and takes no page,
-    and ``read_status`` says so.  Nothing is read back by the host, so the call can be captured into a graph.
+    and ``read_status`` says so.  What attention returns for its query rows is to be dropped (they count in
+    ``query_start_loc``, and are taken as the last tokens of the old length); its new length is its old one.  Nothing is read
+    back by the host, so the call can be captured into a graph.
     """
     try:
         key = (query_lens.shape, query_lens.dtype, query_lens.is_contiguous(), query_lens.get_device(),

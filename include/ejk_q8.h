@@ -6,7 +6,10 @@
  * The cache
  *   kv_pages   [num_pages, num_kv_heads, 2, page_size, head_dim]            codes, one byte each (e4m3 or int8); 2 = K, V
  *   kv_scales  [num_pages, num_kv_heads, 2, page_size / scale_block]         float32, positive and finite
- * A value is its code times the scale of its block of `scale_block` tokens.  The page of one head is contiguous (the
+ * A value is its code times the scale of its block of `scale_block` tokens.  A write makes no NaN codes; e4m3 codes that are NaN
+ * (a cache that was filled otherwise) make NaN of the rows that see them, and where they are V's also of rows that the mask keeps
+ * from them but not from the other keys of the same tile.  Behind a sequence's end and before the window of all its rows any bytes
+ * may lie, scales included.  The page of one head is contiguous (the
  * pool of ejk_rpa_launch interleaves the heads of a token): the attention kernel fetches runs of page_size * head_dim
  * bytes, where one token of one head is 64 to 256 bytes of an 8-bit cache -- shorter than what DRAM serves well.
  *
@@ -60,6 +63,8 @@ EJK_RPA_API size_t ejk_q8_workspace_bytes(const ejk_q8_shape* shape);
 /* Ragged attention over the 8-bit cache.  Operands, masks, sinks and zero rows as ejk_rpa_launch; `attrs.q_scale` and
  * `attrs.out_scale` must be 0.  With x = softmax_scale * k_scale[j] * sum_d q[d] * k_code[j, d], soft cap and masks on
  * x, the output is sum_j softmax(x)[j] * v_scale[j] * v_code[j].
+ * Accuracy, per row, with p the softmax weights and the sums over the keys that the row sees: within 2^-10 sum p |v| (2^-9 where
+ * scales are no powers of two) + 2^-24 max |v| + the output's rounding, for logits of a few units.
  * Sequences with many query rows are served by tensor tiles (head_dim 64 and 128): those of num_queries_per_block tokens and more
  * where the caller gives it, otherwise those of 32 rows and more in batches with more tokens than block_tables has rows.  In a
  * table with idle rows only the hint tells a chunk of a prompt from decode rows.  Every row of `out` is written: rows of no sequence, and of
@@ -99,7 +104,9 @@ EJK_RPA_API int ejk_q8_read_launch(const void* kv_pages, const float* kv_scales,
  * First the pages of finished rows go on top of the stack, in row and page order (such a row takes no tokens in this
  * call).  Then every row that lacks pages for its context_len + query_len tokens takes them from the top, rows in
  * order.  A row that cannot be served -- the stack is empty, the row's table too short, the batch longer than
- * total_tokens -- takes no page, keeps its context length, gets slots of -1 and sets a status bit.
+ * total_tokens -- takes no page, keeps its context length, gets slots of -1 and sets a status bit.  Its tokens still count in
+ * query_start_loc: a write skips them, and attention takes them as the LAST tokens of the old context length and returns numbers for
+ * them.  Whoever lets a step go on without reading the status has to drop such rows' results (their new length is the old one).
  * slots[t] = page * page_size + offset of token t; -1 behind the last sequence.  max_num_seqs is 16384 at most.
  * No output may overlap an input other than as named above. */
 EJK_RPA_API int ejk_page_tables_launch(const int32_t* query_lens, const int32_t* context_lens, int32_t* block_tables,
